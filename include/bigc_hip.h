@@ -16,7 +16,7 @@
  *   - every function returns 0 on success or a negative bigc_status; the message of the
  *     last failure on the calling thread is returned by bigc_last_error();
  *   - one handle per device and per model; a handle may be used from one thread at a time.
- *   - all tensors are IEEE fp32 and every accumulation is fp32; the GEMMs, the head_dim-64 attention core and the fused
+ *   - all tensors (but those of the sequence operators at the end, which also take f16 and bfloat16) are IEEE fp32 and every accumulation is fp32; the GEMMs, the head_dim-64 attention core and the fused
  *     role attention run on the f16 matrix cores with exactly split f32 operands (f32-level error; operands with
  *     |x| >= 32768 are redone on the f32 MFMA; bigc_linear_set_exact(1) selects the f32 MFMA kernels throughout), the
  *     other attention kernels on the f32 MFMA; indices are int32 on the device side (the Python host converts to the
@@ -682,6 +682,94 @@ BIGC_API int bigc_split_rows_f32(void* stream, const float* X, long ldx, void* Y
  * the store-bound FMA kernel.  An element the split form cannot hold sets *range_flag. */
 BIGC_API int bigc_linear_hr8out_f32(void* stream, const float* A, int lda, const float* W, int ldw, const float* bias, const float* residual, int ldr,
                            float* C, int ldc, void* Cs, long ldcs_bytes, int M, int N, int K, int act, int* range_flag);
+
+/* ------------------------------------------------------------------------------------
+ * Sequence operators: what lies between an attention layer's in-projection and its out-projection when the rows have an order
+ * -- position biases, caps and masks on the scores, shared key heads, norms and rotations of the heads.  They stand next to
+ * bigc_mha_core_f32 (no order, no masks, one key head per query head) and take IEEE f32, f16 and bfloat16 tensors; scores,
+ * softmax statistics, sums and parameter gradients are f32 whatever the tensors' type.  (models/ has no caller of its own.)
+ * Every row pointer, row stride and head stride has to be a multiple of 16 bytes (with one head its stride is not read).
+ * ---------------------------------------------------------------------------------- */
+
+#define BIGC_F32 0
+#define BIGC_F16 1
+#define BIGC_BF16 2
+
+/* Attention over ragged sequences.  Sequence s owns rows [q_off[s], q_off[s+1]) of q / o and rows [k_off[s], k_off[s+1]) of
+ * k / v; element (row, head h, column c) of q is q[row * ldq + h * hsq + c], likewise the others; query head h reads key head
+ * h / (n_head / n_kv_head).  With Lq, Lk rows the queries are the LAST rows of their sequence: query i stands at position
+ * i + Lk - Lq, and d = key - position.
+ *     x = scale * q . k;   c = softcap > 0 ? softcap * tanh(x / softcap) : x
+ *     score = c - slopes[h] * |d| + rel_table[rel_map[clip(d, -bias_radius, bias_radius) + bias_radius], h]
+ *     seen  = (no documents or q_doc[i] == k_doc[j] >= 0) and (j < prefix_len[s] or
+ *             ((!causal or d <= 0) and (window_left < 0 or -d <= window_left) and (window_right < 0 or d <= window_right)))
+ *     o = softmax over the seen keys of the scores, times v
+ * A query that sees no key (or only scores of -inf) has o = 0 and lse = -inf and gives no gradient; what a hidden place holds (NaN, Inf) is
+ * never part of a result.  slopes, rel_table + rel_map, prefix_len, q_doc + k_doc may be NULL.  Rows outside every sequence
+ * stay as they were.  Offsets are cut to [0, n_q] and [0, n_k] and lengths to max_q and max_k (which size the launch), map entries to the table. */
+typedef struct {
+    int32_t dtype;                     /* BIGC_F32 / BIGC_F16 / BIGC_BF16: q, k, v, o, d_o, dq, dk, dv */
+    int32_t n_seq, n_head, n_kv_head;  /* n_head a multiple of n_kv_head */
+    int32_t head_dim;                  /* a multiple of 8, at most 128 */
+    int32_t max_q, max_k;              /* the longest sequence's rows */
+    int32_t causal, window_left, window_right; /* windows: -1 = none */
+    int32_t bias_radius, n_bucket;     /* rel_map has 2 * bias_radius + 1 entries (bias_radius <= 2047), rel_table n_bucket rows of n_head */
+    float scale, softcap;              /* softcap 0: none */
+    int64_t n_q, n_k;                  /* rows of q / o and of k / v, below 2^31 */
+    const int32_t* q_off; const int32_t* k_off; /* (n_seq + 1) */
+    const float* slopes;               /* (n_head) */
+    const float* rel_table; const int32_t* rel_map;
+    const int32_t* prefix_len;         /* (n_seq) */
+    const int32_t* q_doc; const int32_t* k_doc; /* (n_q), (n_k); negative: padding */
+    const void* q; int64_t ldq, hsq;
+    const void* k; int64_t ldk, hsk;
+    const void* v; int64_t ldv, hsv;
+    void* o; int64_t ldo, hso;         /* bigc_seq_attn_bwd reads it */
+    float* lse;                        /* (n_q, n_head) log of the sum of exp(score); optional in the forward, read by the backward */
+    float* o32;                        /* (n_q, n_head, head_dim) o before its rounding; optional; read by the backward instead of o where given:
+                                        * f16 / bf16 rel_table gradients are then exact to f32 */
+    /* backward only */
+    const void* d_o; int64_t lddo, hsdo;
+    void* dq; int64_t lddq, hsdq;
+    void* dk; int64_t lddk, hsdk;      /* summed over the query heads of a key head */
+    void* dv; int64_t lddv, hsdv;
+    float* d_rel_table;                /* (n_bucket, n_head), overwritten; may be NULL */
+} bigc_seq_attn;
+
+/* bytes of the workspace (16-byte aligned) of one call; depends on the sizes, masks and biases in *a, not on the tensors; 0 for arguments that the call would refuse */
+BIGC_API size_t bigc_seq_attn_workspace_bytes(const bigc_seq_attn* a, int backward);
+/* Forward.  Few query rows over many keys are split over the keys and joined; repeats bit for bit. */
+BIGC_API int bigc_seq_attn_fwd(void* stream, const bigc_seq_attn* a, void* workspace, size_t workspace_bytes);
+/* Backward from lse and o (or o32) of the forward; every sum in a fixed order, no atomics: repeats bit for bit. */
+BIGC_API int bigc_seq_attn_bwd(void* stream, const bigc_seq_attn* a, void* workspace, size_t workspace_bytes);
+
+/* RMS norm of every query and key head and the rotation of its first 2 * n_freq columns by the row's position, in one launch:
+ *     y = x / sqrt(mean(x^2) + eps) * w;   (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = pos[row] * inv_freq[f]
+ * with t taken in 64 bits (any int32 position), pairs (f, f + n_freq), or (2 f, 2 f + 1) when interleaved.  w NULL: 1. n_freq 0: no rotation. */
+typedef struct {
+    int32_t dtype, n_q_head, n_k_head, head_dim; /* head_dim a multiple of 8, at most 256; either head count may be 0 */
+    int32_t n_freq, interleaved;       /* 2 * n_freq <= head_dim */
+    float eps;
+    int64_t n_rows;                    /* below 2^31 */
+    const int32_t* pos;                /* (n_rows) */
+    const double* inv_freq;            /* (n_freq) */
+    const float* wq; const float* wk;  /* (head_dim) */
+    const void* q; int64_t ldq, hsq;
+    const void* k; int64_t ldk, hsk;
+    void* q_out; int64_t ldqo, hsqo;   /* may be q itself with its strides */
+    void* k_out; int64_t ldko, hsko;
+    /* backward only: gradients of q_out / k_out in, of q / k and of the weights out (dwq, dwk (head_dim) f32, overwritten, may be NULL) */
+    const void* dq_out; int64_t lddqo, hsdqo;
+    const void* dk_out; int64_t lddko, hsdko;
+    void* dq; int64_t lddq, hsdq;
+    void* dk; int64_t lddk, hsdk;
+    float* dwq; float* dwk;
+} bigc_head_norm;
+
+BIGC_API int bigc_head_norm_rope_fwd(void* stream, const bigc_head_norm* a);
+BIGC_API size_t bigc_head_norm_rope_workspace_bytes(const bigc_head_norm* a);
+/* Backward from the forward's inputs (nothing else is saved); weight gradients summed in a fixed order. */
+BIGC_API int bigc_head_norm_rope_bwd(void* stream, const bigc_head_norm* a, void* workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

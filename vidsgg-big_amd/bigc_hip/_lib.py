@@ -55,6 +55,29 @@ class grd_batch(ctypes.Structure):
                 ("total_rows", ctypes.c_int64), ("vid_row_off", c_void_p), ("q_vid", c_void_p), ("q_row_off", c_void_p), ("vid_len", c_void_p)]
 
 
+class bigc_seq_attn(ctypes.Structure):
+    _fields_ = [("dtype", c_int32), ("n_seq", c_int32), ("n_head", c_int32), ("n_kv_head", c_int32), ("head_dim", c_int32),
+                ("max_q", c_int32), ("max_k", c_int32), ("causal", c_int32), ("window_left", c_int32), ("window_right", c_int32),
+                ("bias_radius", c_int32), ("n_bucket", c_int32), ("scale", c_float), ("softcap", c_float), ("n_q", c_int64),
+                ("n_k", c_int64), ("q_off", c_void_p), ("k_off", c_void_p), ("slopes", c_void_p), ("rel_table", c_void_p),
+                ("rel_map", c_void_p), ("prefix_len", c_void_p), ("q_doc", c_void_p), ("k_doc", c_void_p), ("q", c_void_p),
+                ("ldq", c_int64), ("hsq", c_int64), ("k", c_void_p), ("ldk", c_int64), ("hsk", c_int64), ("v", c_void_p), ("ldv", c_int64),
+                ("hsv", c_int64), ("o", c_void_p), ("ldo", c_int64), ("hso", c_int64), ("lse", c_void_p), ("o32", c_void_p),
+                ("d_o", c_void_p), ("lddo", c_int64), ("hsdo", c_int64), ("dq", c_void_p), ("lddq", c_int64), ("hsdq", c_int64),
+                ("dk", c_void_p), ("lddk", c_int64), ("hsdk", c_int64), ("dv", c_void_p), ("lddv", c_int64), ("hsdv", c_int64),
+                ("d_rel_table", c_void_p)]
+
+
+class bigc_head_norm(ctypes.Structure):
+    _fields_ = [("dtype", c_int32), ("n_q_head", c_int32), ("n_k_head", c_int32), ("head_dim", c_int32), ("n_freq", c_int32),
+                ("interleaved", c_int32), ("eps", c_float), ("n_rows", c_int64), ("pos", c_void_p), ("inv_freq", c_void_p),
+                ("wq", c_void_p), ("wk", c_void_p), ("q", c_void_p), ("ldq", c_int64), ("hsq", c_int64), ("k", c_void_p), ("ldk", c_int64),
+                ("hsk", c_int64), ("q_out", c_void_p), ("ldqo", c_int64), ("hsqo", c_int64), ("k_out", c_void_p), ("ldko", c_int64),
+                ("hsko", c_int64), ("dq_out", c_void_p), ("lddqo", c_int64), ("hsdqo", c_int64), ("dk_out", c_void_p), ("lddko", c_int64),
+                ("hsdko", c_int64), ("dq", c_void_p), ("lddq", c_int64), ("hsdq", c_int64), ("dk", c_void_p), ("lddk", c_int64),
+                ("hsdk", c_int64), ("dwq", c_void_p), ("dwk", c_void_p)]
+
+
 _SIGS = {
     "bigc_last_error": (c_char_p, []),
     "bigc_build_info": (c_char_p, []),
@@ -185,6 +208,13 @@ _SIGS = {
     "bigc_train_workspace_bytes": (c_size_t, [c_void_p, POINTER(bigc_batch)]),
     "bigc_train_forward": (c_int, [c_void_p, c_void_p, POINTER(bigc_batch), c_void_p, c_size_t, c_void_p, c_void_p]),
     "bigc_train_backward": (c_int, [c_void_p, c_void_p, POINTER(bigc_batch), c_void_p, c_size_t, c_void_p, c_int, c_void_p]),
+    # sequence operators
+    "bigc_seq_attn_workspace_bytes": (c_size_t, [POINTER(bigc_seq_attn), c_int]),
+    "bigc_seq_attn_fwd": (c_int, [c_void_p, POINTER(bigc_seq_attn), c_void_p, c_size_t]),
+    "bigc_seq_attn_bwd": (c_int, [c_void_p, POINTER(bigc_seq_attn), c_void_p, c_size_t]),
+    "bigc_head_norm_rope_fwd": (c_int, [c_void_p, POINTER(bigc_head_norm)]),
+    "bigc_head_norm_rope_workspace_bytes": (c_size_t, [POINTER(bigc_head_norm)]),
+    "bigc_head_norm_rope_bwd": (c_int, [c_void_p, POINTER(bigc_head_norm), c_void_p, c_size_t]),
     # grounding scorer
     "bigc_dwconv_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int]),
     "grd_coattention_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int]),
