@@ -38,44 +38,37 @@ def rel_bucket_map(n_bucket, max_distance, two_sided=True, radius=None):
     return torch.tensor(out, dtype=torch.int32)
 
 
-def _rows(name, t, like, shape):
+def _rows(name, t, dtype, device, shape):
     """(address, row stride, head stride) of a (rows, heads, columns) tensor whose columns lie side by side"""
-    assert isinstance(t, torch.Tensor) and t.dim() == 3, "%s: a (rows, heads, columns) tensor" % name
-    assert t.dtype == like.dtype and t.device == like.device, "%s: %s on %s next to %s on %s" % (name, t.dtype, t.device, like.dtype, like.device)
-    assert tuple(t.shape) == tuple(shape), "%s: shape %s, not %s" % (name, tuple(t.shape), tuple(shape))
+    assert isinstance(t, torch.Tensor), "%s: a tensor" % name
+    assert t.dtype is dtype and t.device == device, "%s: %s on %s next to %s on %s" % (name, t.dtype, t.device, dtype, device)
+    assert t.shape == shape, "%s: shape %s, not %s" % (name, tuple(t.shape), tuple(shape))
     s = t.stride()
-    assert s[2] == 1 or t.shape[2] == 1, "%s: the columns of a head have to lie side by side (strides %s)" % (name, s)
+    assert s[2] == 1 or shape[2] == 1, "%s: the columns of a head have to lie side by side (strides %s)" % (name, s)
     return t.data_ptr(), s[0], s[1]
 
 
 def _vector(name, t, dtype, shape, device):
     if t is None:
         return None
-    assert isinstance(t, torch.Tensor) and t.dtype == dtype and t.device == device, "%s: a %s tensor on %s" % (name, dtype, device)
-    assert tuple(t.shape) == tuple(shape) and t.is_contiguous(), "%s: contiguous, of shape %s (not %s)" % (name, tuple(shape), tuple(t.shape))
+    assert isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device, "%s: a %s tensor on %s" % (name, dtype, device)
+    assert t.shape == shape and t.is_contiguous(), "%s: contiguous, of shape %s (not %s)" % (name, tuple(shape), tuple(t.shape))
     return t.data_ptr()
 
 
-class _On(object):
-    """the device's current stream; the device is current inside (a launch goes to the current device)"""
-
-    def __init__(self, device):
-        assert device.type == "cuda", "the operators run on a GPU (tensors are on %s)" % device
-        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
-        self.device = device
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+def _heads(name, t):
+    assert isinstance(t, torch.Tensor) and t.dim() == 3 and t.dtype in _DTYPES, "%s: a (rows, heads, columns) tensor of f32, f16 or bf16" % name
+    return t.shape
 
 
-def _workspace(lib, nbytes, device):
-    return torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
+def _on(device):
+    """A guard that makes the tensors' device the current one (a launch goes to the current device), or None where it is"""
+    assert device.type == "cuda", "the operators run on a GPU (tensors are on %s)" % device
+    return None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)            # torch.cuda.current_stream(device).cuda_stream, without the objects
 
 
 class SavedAttention(object):
@@ -96,46 +89,39 @@ def attend(q, k, v, q_off, k_off, max_q, max_k, scale=None, softcap=0.0, slopes=
     behind / ahead, -1 for no limit; prefix_len (n_seq) int32: the first keys of a sequence are seen by all its rows; q_doc, k_doc (n_q), (n_k)
     int32: rows see keys of their own document, a negative number is padding.  A row that sees nothing gives 0.
     -> o (n_q, n_head, head_dim), or (o, SavedAttention) with ``save``; rows outside every sequence are not written (0 unless ``out`` is given)."""
+    shape = _heads("q", q)
+    dtype, dev, hd = q.dtype, q.device, shape[2]
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return attend(q, k, v, q_off, k_off, max_q, max_k, scale, softcap, slopes, rel_table, rel_map, causal, window, prefix_len, q_doc, k_doc, out, save)
     lib = _lib.load()
-    assert isinstance(q, torch.Tensor) and q.dim() == 3 and q.dtype in _DTYPES, "q: a (rows, heads, columns) tensor of f32, f16 or bf16"
-    n_q, n_head, hd = q.shape
-    assert isinstance(k, torch.Tensor) and k.dim() == 3, "k: a (rows, heads, columns) tensor"
-    n_k, n_kv = k.shape[0], k.shape[1]
-    dev, n_seq = q.device, q_off.shape[0] - 1
-    a = bigc_seq_attn()
-    a.dtype, a.n_seq, a.n_head, a.n_kv_head, a.head_dim, a.max_q, a.max_k = _DTYPES[q.dtype], n_seq, n_head, n_kv, hd, max_q, max_k
-    a.causal, (a.window_left, a.window_right) = bool(causal), window
-    a.scale, a.softcap = hd ** -0.5 if scale is None else scale, softcap
-    a.n_q, a.n_k = n_q, n_k
-    a.q, a.ldq, a.hsq = _rows("q", q, q, (n_q, n_head, hd))
-    a.k, a.ldk, a.hsk = _rows("k", k, q, (n_k, n_kv, hd))
-    a.v, a.ldv, a.hsv = _rows("v", v, q, (n_k, n_kv, hd))
-    a.q_off = _vector("q_off", q_off, torch.int32, (n_seq + 1,), dev)
-    a.k_off = _vector("k_off", k_off, torch.int32, (n_seq + 1,), dev)
-    a.slopes = _vector("slopes", slopes, torch.float32, (n_head,), dev)
+    kshape = (_heads("k", k)[0], k.shape[1], hd)
+    n_q, n_head, n_seq = shape[0], shape[1], q_off.shape[0] - 1
+    assert (q_doc is None) == (k_doc is None), "q_doc and k_doc come together"
+    n_bucket = radius = 0
     if rel_table is not None or rel_map is not None:
         assert rel_table is not None and rel_map is not None, "rel_table and rel_map come together"
         assert rel_table.dim() == 2 and rel_map.dim() == 1 and rel_map.shape[0] % 2 == 1, "rel_table (n_bucket, n_head), rel_map (2 R + 1)"
-        a.bias_radius, a.n_bucket = rel_map.shape[0] // 2, rel_table.shape[0]
-        a.rel_table = _vector("rel_table", rel_table, torch.float32, (a.n_bucket, n_head), dev)
-        a.rel_map = _vector("rel_map", rel_map, torch.int32, (rel_map.shape[0],), dev)
-    a.prefix_len = _vector("prefix_len", prefix_len, torch.int32, (n_seq,), dev)
-    a.q_doc = _vector("q_doc", q_doc, torch.int32, (n_q,), dev)
-    a.k_doc = _vector("k_doc", k_doc, torch.int32, (n_k,), dev)
-    assert (q_doc is None) == (k_doc is None), "q_doc and k_doc come together"
-    with _On(dev) as stream:
-        need = lib.bigc_seq_attn_workspace_bytes(ctypes.byref(a), 0)
-        o = torch.zeros((n_q, n_head, hd), dtype=q.dtype, device=dev) if out is None else out
-        a.o, a.ldo, a.hso = _rows("out", o, q, (n_q, n_head, hd))
-        lse = o32 = None
-        if save:
-            lse = torch.empty((n_q, n_head), dtype=torch.float32, device=dev)
-            a.lse = lse.data_ptr()
-            if q.dtype != torch.float32:
-                o32 = torch.empty((n_q, n_head, hd), dtype=torch.float32, device=dev)
-                a.o32 = o32.data_ptr()
-        ws = _workspace(lib, need, dev)
-        _lib.check(lib.bigc_seq_attn_fwd(stream, ctypes.byref(a), _lib.ptr(ws), need))
+        n_bucket, radius = rel_table.shape[0], rel_map.shape[0] // 2
+    i32, f32 = torch.int32, torch.float32
+    o = q.new_zeros(shape) if out is None else out
+    lse = o32 = None
+    if save:
+        lse = q.new_empty((n_q, n_head), dtype=f32)
+        if dtype is not f32:
+            o32 = q.new_empty(shape, dtype=f32)
+    a = bigc_seq_attn(                                                   # the fields in the structure's order
+        _DTYPES[dtype], n_seq, n_head, kshape[1], hd, max_q, max_k, 1 if causal else 0, window[0], window[1], radius, n_bucket,
+        hd ** -0.5 if scale is None else scale, softcap, n_q, kshape[0],
+        _vector("q_off", q_off, i32, (n_seq + 1,), dev), _vector("k_off", k_off, i32, (n_seq + 1,), dev), _vector("slopes", slopes, f32, (n_head,), dev),
+        _vector("rel_table", rel_table, f32, (n_bucket, n_head), dev), _vector("rel_map", rel_map, i32, (2 * radius + 1,), dev),
+        _vector("prefix_len", prefix_len, i32, (n_seq,), dev), _vector("q_doc", q_doc, i32, (n_q,), dev), _vector("k_doc", k_doc, i32, (kshape[0],), dev),
+        *_rows("q", q, dtype, dev, shape), *_rows("k", k, dtype, dev, kshape), *_rows("v", v, dtype, dev, kshape), *_rows("out", o, dtype, dev, shape),
+        _lib.ptr(lse), _lib.ptr(o32))
+    need = lib.bigc_seq_attn_workspace_bytes(ctypes.byref(a), 0)
+    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+    _lib.check(lib.bigc_seq_attn_fwd(_stream(dev), ctypes.byref(a), _lib.ptr(ws), need))
     if not save:
         return o
     return o, SavedAttention(a, (q, k, v, q_off, k_off, slopes, rel_table, rel_map, prefix_len, q_doc, k_doc), o, lse, o32)
@@ -144,73 +130,75 @@ def attend(q, k, v, q_off, k_off, max_q, max_k, scale=None, softcap=0.0, slopes=
 def attend_bwd(saved, d_o):
     """Gradients of ``attend`` for the output's gradient ``d_o`` -> (dq, dk, dv, d_rel_table or None); dk, dv summed over the query heads of a key
     head.  Rows outside every sequence get 0.  Repeats bit for bit."""
-    lib = _lib.load()
     q, k, v = saved.tensors[:3]
-    rel_table = saved.tensors[6]
+    guard = _on(q.device)
+    if guard is not None:
+        with guard:
+            return attend_bwd(saved, d_o)
+    lib = _lib.load()
     a = bigc_seq_attn()
     ctypes.memmove(ctypes.byref(a), ctypes.byref(saved.args), ctypes.sizeof(a))
-    a.d_o, a.lddo, a.hsdo = _rows("d_o", d_o, q, q.shape)
-    with _On(q.device) as stream:
-        dq, dk, dv = (torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        for name, t in (("q", dq), ("k", dk), ("v", dv)):
-            setattr(a, "d" + name, t.data_ptr())
-            setattr(a, "ldd" + name, t.stride(0))
-            setattr(a, "hsd" + name, t.stride(1))
-        dt = None
-        if rel_table is not None:
-            dt = torch.empty_like(rel_table)
-            a.d_rel_table = dt.data_ptr()
-        need = lib.bigc_seq_attn_workspace_bytes(ctypes.byref(a), 1)
-        ws = _workspace(lib, need, q.device)
-        _lib.check(lib.bigc_seq_attn_bwd(stream, ctypes.byref(a), _lib.ptr(ws), need))
+    a.d_o, a.lddo, a.hsdo = _rows("d_o", d_o, q.dtype, q.device, q.shape)
+    dq, dk, dv = q.new_zeros(q.shape), k.new_zeros(k.shape), v.new_zeros(v.shape)
+    a.dq, a.lddq, a.hsdq = _rows("dq", dq, q.dtype, q.device, q.shape)
+    a.dk, a.lddk, a.hsdk = _rows("dk", dk, q.dtype, q.device, k.shape)
+    a.dv, a.lddv, a.hsdv = _rows("dv", dv, q.dtype, q.device, v.shape)
+    dt = None
+    if saved.tensors[6] is not None:
+        dt = torch.empty_like(saved.tensors[6])
+        a.d_rel_table = dt.data_ptr()
+    need = lib.bigc_seq_attn_workspace_bytes(ctypes.byref(a), 1)
+    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+    _lib.check(lib.bigc_seq_attn_bwd(_stream(q.device), ctypes.byref(a), _lib.ptr(ws), need))
     return dq, dk, dv, dt
 
 
 def _norm_args(q, k, wq, wk, pos, inv_freq, eps, interleaved):
-    assert isinstance(q, torch.Tensor) and q.dim() == 3 and q.dtype in _DTYPES, "q: a (rows, heads, columns) tensor of f32, f16 or bf16"
-    n, h, hd = q.shape
-    assert isinstance(k, torch.Tensor) and k.dim() == 3, "k: a (rows, heads, columns) tensor"
-    a, dev = bigc_head_norm(), q.device
-    a.dtype, a.n_q_head, a.n_k_head, a.head_dim, a.n_rows = _DTYPES[q.dtype], h, k.shape[1], hd, n
-    a.interleaved, a.eps = bool(interleaved), eps
-    a.q, a.ldq, a.hsq = _rows("q", q, q, (n, h, hd))
-    a.k, a.ldk, a.hsk = _rows("k", k, q, (n, k.shape[1], hd))
-    a.wq = _vector("wq", wq, torch.float32, (hd,), dev)
-    a.wk = _vector("wk", wk, torch.float32, (hd,), dev)
-    if inv_freq is not None:
-        a.n_freq = inv_freq.shape[0]
-        a.inv_freq = _vector("inv_freq", inv_freq, torch.float64, (inv_freq.shape[0],), dev)
-        a.pos = _vector("pos", pos, torch.int32, (n,), dev)
-    return a
+    shape, kshape = _heads("q", q), _heads("k", k)
+    dtype, dev, n, hd = q.dtype, q.device, shape[0], shape[2]
+    n_freq = 0 if inv_freq is None else inv_freq.shape[0]
+    assert inv_freq is None or pos is not None, "inv_freq without pos"
+    f32 = torch.float32
+    return bigc_head_norm(                                               # the fields in the structure's order
+        _DTYPES[dtype], shape[1], kshape[1], hd, n_freq, 1 if interleaved else 0, eps, n, _vector("pos", pos, torch.int32, (n,), dev),
+        _vector("inv_freq", inv_freq, torch.float64, (n_freq,), dev), _vector("wq", wq, f32, (hd,), dev), _vector("wk", wk, f32, (hd,), dev),
+        *_rows("q", q, dtype, dev, shape), *_rows("k", k, dtype, dev, (n, kshape[1], hd)))
 
 
 def head_norm_rope(q, k, wq, wk, pos, inv_freq, eps=1e-6, interleaved=False, out=None):
     """RMS norm of every head of ``q`` (rows, n_head, head_dim) and ``k`` (rows, n_kv_head, head_dim) times ``wq`` / ``wk`` (head_dim) f32 (None:
     1), then the rotation of the first 2 * len(inv_freq) columns by pos[row] * inv_freq (int32 (rows), f64; inv_freq None: no rotation).  q and k may be
     slices of one projection's output (16-byte strides); ``out``: a pair of tensors, which may be (q, k) themselves.  -> (q', k')"""
-    lib = _lib.load()
     a = _norm_args(q, k, wq, wk, pos, inv_freq, eps, interleaved)
-    with _On(q.device) as stream:
-        qo, ko = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)) if out is None else out
-        a.q_out, a.ldqo, a.hsqo = _rows("out[0]", qo, q, q.shape)
-        a.k_out, a.ldko, a.hsko = _rows("out[1]", ko, q, k.shape)
-        _lib.check(lib.bigc_head_norm_rope_fwd(stream, ctypes.byref(a)))
+    dtype, dev = q.dtype, q.device
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return head_norm_rope(q, k, wq, wk, pos, inv_freq, eps, interleaved, out)
+    qo, ko = (q.new_empty(q.shape), k.new_empty(k.shape)) if out is None else out
+    a.q_out, a.ldqo, a.hsqo = _rows("out[0]", qo, dtype, dev, q.shape)
+    a.k_out, a.ldko, a.hsko = _rows("out[1]", ko, dtype, dev, k.shape)
+    _lib.check(_lib.load().bigc_head_norm_rope_fwd(_stream(dev), ctypes.byref(a)))
     return qo, ko
 
 
 def head_norm_rope_bwd(d_q, d_k, q, k, wq, wk, pos, inv_freq, eps=1e-6, interleaved=False):
     """Gradients of ``head_norm_rope`` for those of its outputs, from its inputs as they were -> (dq, dk, dwq, dwk); a weight that is None gets None."""
-    lib = _lib.load()
     a = _norm_args(q, k, wq, wk, pos, inv_freq, eps, interleaved)
-    a.dq_out, a.lddqo, a.hsdqo = _rows("d_q", d_q, q, q.shape)
-    a.dk_out, a.lddko, a.hsdko = _rows("d_k", d_k, q, k.shape)
-    with _On(q.device) as stream:
-        dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-        a.dq, a.lddq, a.hsdq = dq.data_ptr(), dq.stride(0), dq.stride(1)
-        a.dk, a.lddk, a.hsdk = dk.data_ptr(), dk.stride(0), dk.stride(1)
-        dwq, dwk = (None if w is None else torch.empty_like(w) for w in (wq, wk))
-        a.dwq, a.dwk = _lib.ptr(dwq), _lib.ptr(dwk)
-        need = lib.bigc_head_norm_rope_workspace_bytes(ctypes.byref(a))
-        ws = _workspace(lib, need, q.device)
-        _lib.check(lib.bigc_head_norm_rope_bwd(stream, ctypes.byref(a), _lib.ptr(ws), need))
+    dtype, dev = q.dtype, q.device
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return head_norm_rope_bwd(d_q, d_k, q, k, wq, wk, pos, inv_freq, eps, interleaved)
+    lib = _lib.load()
+    a.dq_out, a.lddqo, a.hsdqo = _rows("d_q", d_q, dtype, dev, q.shape)
+    a.dk_out, a.lddko, a.hsdko = _rows("d_k", d_k, dtype, dev, k.shape)
+    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+    a.dq, a.lddq, a.hsdq = _rows("dq", dq, dtype, dev, q.shape)
+    a.dk, a.lddk, a.hsdk = _rows("dk", dk, dtype, dev, k.shape)
+    dwq, dwk = (None if w is None else torch.empty_like(w) for w in (wq, wk))
+    a.dwq, a.dwk = _lib.ptr(dwq), _lib.ptr(dwk)
+    need = lib.bigc_head_norm_rope_workspace_bytes(ctypes.byref(a))
+    ws = q.new_empty((need,), dtype=torch.uint8)
+    _lib.check(lib.bigc_head_norm_rope_bwd(_stream(dev), ctypes.byref(a), _lib.ptr(ws), need))
     return dq, dk, dwq, dwk

@@ -1,93 +1,243 @@
 // RMS norm of every query / key head and the position rotation of its columns, forward and backward.
+//
+// Bound by memory: an element is read once and written once (the backward reads two and writes one) for some ten operations.  A lane holds 16
+// bytes of one head's columns (E = 4 f32 or 8 half values), LPH = 2^n lanes hold a head, so that the mean of squares is a butterfly of
+// log2 LPH steps inside a wave and no head leaves its wave.  What is not a head's own value lies in LDS as coefficients per column, built once per
+// row: the forward's y = r (x A + partner B) with A = w cos, B = +- w_partner sin (two multiplies and one fma an element), the backward's cos,
+// +- sin and w.  With few registers (many waves on a CU) rather than loads ahead: prefetching the next head, or two heads in flight with
+// weights and angles in registers, measured 139 - 142 us where this order of work took 79 (16384 rows of 32 + 8 heads of 128, f16).
 #include "sequence.h"
 #include <math.h>
 
 namespace {
-constexpr int ROW_BLOCKS = 256;                                // blocks of the backward: each sums its rows' weight gradients
+constexpr int MAX_WAVES = 8, THREADS = 64 * MAX_WAVES;         // of a block at most
+constexpr int MAX_FREQ = 128;
+constexpr int ROWS_PER_BLOCK = 4;
+constexpr int BWD_BLOCKS = 1024;                                // of the backward: each sums its rows' weight gradients (four blocks on every CU)
 
-__device__ __forceinline__ float wave_sum(float x) {
-    for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m);
+enum { TURN_NONE, TURN_HALVES, TURN_PAIRS, TURN_ANY };          // how a chunk meets its partner columns: none; a whole chunk n_freq columns away; inside the chunk; column by column
+
+// cosine and sine of t = pos * inv_freq.  The angle is taken in turns, in 64 bits (t has up to 31 bits before the point), cut to an eighth of a turn
+// around the nearest quarter, and only that rest, which 32 bits hold to 2^-27 of a turn, goes through the f32 functions.
+__device__ __forceinline__ float2 turn(int pos, double inv_freq) {
+    const double x = (double)pos * (inv_freq * 0.15915494309189533577);
+    const double rest = x - rint(x), quarter = rint(rest * 4.0);
+    float s, c;
+    sincospif(2.0f * (float)(rest - quarter * 0.25), &s, &c);
+    const int k = (int)quarter & 3;
+    const float a = k & 1 ? s : c, b = k & 1 ? c : s;
+    return make_float2(k == 1 || k == 2 ? -a : a, k >= 2 ? -b : b);
+}
+
+template <typename T> struct Chunk {
+    static constexpr int E = 16 / sizeof(T);
+    uint4 raw;
+    __device__ __forceinline__ float operator[](int e) const { return (float)((const T*)&raw)[e]; }
+};
+
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_chunk(const T* p, bool live) {
+    Chunk<T> c;
+    c.raw = live ? *(const uint4*)p : make_uint4(0, 0, 0, 0);
+    return c;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, const float* y) {
+    T v[16 / sizeof(T)];
+    for (int e = 0; e < (int)(16 / sizeof(T)); ++e) v[e] = (T)y[e];
+    *(uint4*)p = *(const uint4*)v;
+}
+
+// The column a column is turned with, and whether it is the first of the pair (itself, where nothing turns)
+__device__ __forceinline__ int partner_of(const bigc_head_norm& a, int col) {
+    if (col >= 2 * a.n_freq) return col;
+    return a.interleaved ? col ^ 1 : col < a.n_freq ? col + a.n_freq : col - a.n_freq;
+}
+
+// place of a column's coefficient in LDS: lanes read the four of a quarter chunk side by side
+template <int E> __device__ __forceinline__ int slot(int col, int chunks) { return (col % E / 4 * chunks + col / E) * 4 + col % 4; }
+
+template <int E>
+__device__ __forceinline__ void coefficients(const float* table, int ch, int chunks, float* out) {
+    for (int p = 0; p < E / 4; ++p) *(float4*)(out + 4 * p) = *(const float4*)(table + (p * chunks + ch) * 4);
+}
+
+// the partners' values of a chunk that the head's lanes hold
+template <typename T, int TURN>
+__device__ __forceinline__ void partners(const bigc_head_norm& a, const Chunk<T>& x, const T* head, int ch, bool live, float* o) {
+    constexpr int E = 16 / sizeof(T);
+    if (TURN == TURN_HALVES) {
+        Chunk<T> y;
+        const int half = a.n_freq / E, from = (threadIdx.x & 63) + (ch < half ? half : ch < 2 * half ? -half : 0);
+        y.raw.x = __shfl(x.raw.x, from); y.raw.y = __shfl(x.raw.y, from); y.raw.z = __shfl(x.raw.z, from); y.raw.w = __shfl(x.raw.w, from);
+        for (int e = 0; e < E; ++e) o[e] = y[e];
+    } else {
+        for (int e = 0; e < E; ++e) o[e] = TURN == TURN_PAIRS ? x[e ^ 1] : TURN == TURN_ANY && live ? (float)head[partner_of(a, ch * E + e)] : 0.f;
+    }
+}
+
+__device__ __forceinline__ float head_sum(float x, int lph) {
+    for (int m = lph >> 1; m; m >>= 1) x += __shfl_xor(x, m);
     return x;
 }
 
-// One wave per head row; columns in LDS.  back: x = dy, rotated by -t.
-__device__ void rotate(const bigc_head_norm& a, float* y, int pos, bool back) {
-    for (int f = threadIdx.x; f < a.n_freq; f += 64) {
-        double sn, cs;
-        sincos((double)pos * a.inv_freq[f], &sn, &cs);
-        const float c = (float)cs, s = back ? -(float)sn : (float)sn;
-        const int i = a.interleaved ? 2 * f : f, j = a.interleaved ? 2 * f + 1 : f + a.n_freq;
-        const float u = y[i], v = y[j];
-        y[i] = u * c - v * s;
-        y[j] = v * c + u * s;
+// Forward: `rows` rows in a block, whose threads take the heads of a row in turn (blockIdx.y: a part of them).
+// LDS: per row A and B of the queries and of the keys.
+template <typename T, int TURN>
+__global__ __launch_bounds__(THREADS) void head_norm_fwd(bigc_head_norm a, int lph, int rows) {
+    constexpr int E = 16 / sizeof(T);
+    extern __shared__ float4 lds4[];
+    __shared__ float2 angle[ROWS_PER_BLOCK][MAX_FREQ];
+    float* tables = (float*)lds4;                               // [row][q, k][A, B][head_dim]
+    const long row0 = (long)blockIdx.x * rows;
+    const int n = (int)min((long)rows, a.n_rows - row0), heads = a.n_q_head + a.n_k_head, per = blockDim.x / lph, hd = a.head_dim, chunks = hd / E;
+    if (TURN != TURN_NONE) {
+        for (int i = threadIdx.x; i < n * a.n_freq; i += blockDim.x) angle[i / a.n_freq][i % a.n_freq] = turn(a.pos[row0 + i / a.n_freq], a.inv_freq[i % a.n_freq]);
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < n * 2 * hd; i += blockDim.x) {
+        const int c = i % hd, of = i / hd;                      // of = 2 row + (key)
+        const float* w = of & 1 ? a.wk : a.wq;
+        float A = w ? w[c] : 1.f, B = 0.f;
+        if (TURN != TURN_NONE && c < 2 * a.n_freq) {
+            const int o = partner_of(a, c);
+            const float2 t = angle[of >> 1][a.interleaved ? c >> 1 : min(c, o)];
+            B = (w ? w[o] : 1.f) * (c < o ? -t.y : t.y);
+            A *= t.x;
+        }
+        tables[of * 2 * hd + slot<E>(c, chunks)] = A;
+        tables[of * 2 * hd + hd + slot<E>(c, chunks)] = B;
     }
     __syncthreads();
-}
-
-template <typename T>
-__global__ __launch_bounds__(64) void head_rows_fwd(bigc_head_norm a) {
-    __shared__ float y[256];
-    const int lane = threadIdx.x, heads = a.n_q_head + a.n_k_head;
-    int h = blockIdx.x % heads;
-    const long row = blockIdx.x / heads;
-    const bool key = h >= a.n_q_head;
-    if (key) h -= a.n_q_head;
-    const T* x = key ? (const T*)a.k + row * a.ldk + h * a.hsk : (const T*)a.q + row * a.ldq + h * a.hsq;
-    T* o = key ? (T*)a.k_out + row * a.ldko + h * a.hsko : (T*)a.q_out + row * a.ldqo + h * a.hsqo;
-    const float* w = key ? a.wk : a.wq;
-    float ss = 0.f;
-    for (int c = lane; c < a.head_dim; c += 64) { const float v = (float)x[c]; y[c] = v; ss += v * v; }
-    const float r = 1.f / sqrtf(wave_sum(ss) / a.head_dim + a.eps);
-    for (int c = lane; c < a.head_dim; c += 64) y[c] *= r * (w ? w[c] : 1.f);
-    __syncthreads();
-    rotate(a, y, a.pos ? a.pos[row] : 0, false);
-    for (int c = lane; c < a.head_dim; c += 64) o[c] = (T)y[c];
-}
-
-template <typename T>
-__global__ __launch_bounds__(64) void head_rows_bwd(bigc_head_norm a, float* part) {
-    __shared__ float y[256];
-    const int lane = threadIdx.x, heads = a.n_q_head + a.n_k_head;
-    float dw[2][4] = {};
-    for (long e = blockIdx.x; e < a.n_rows * heads; e += ROW_BLOCKS) {
-        int h = (int)(e % heads);
-        const long row = e / heads;
-        const bool key = h >= a.n_q_head;
-        if (key) h -= a.n_q_head;
-        const T* x = key ? (const T*)a.k + row * a.ldk + h * a.hsk : (const T*)a.q + row * a.ldq + h * a.hsq;
-        const T* g = key ? (const T*)a.dk_out + row * a.lddko + h * a.hsdko : (const T*)a.dq_out + row * a.lddqo + h * a.hsdqo;
-        T* o = key ? (T*)a.dk + row * a.lddk + h * a.hsdk : (T*)a.dq + row * a.lddq + h * a.hsdq;
-        const float* w = key ? a.wk : a.wq;
-        float ss = 0.f, dot = 0.f, xv[4];
-        __syncthreads();
-        for (int t = 0; t < 4; ++t) {
-            const int c = lane + 64 * t;
-            xv[t] = c < a.head_dim ? (float)x[c] : 0.f;
-            if (c < a.head_dim) y[c] = (float)g[c];
-            ss += xv[t] * xv[t];
-        }
-        __syncthreads();
-        rotate(a, y, a.pos ? a.pos[row] : 0, true);
-        const float r = 1.f / sqrtf(wave_sum(ss) / a.head_dim + a.eps);
-        for (int t = 0; t < 4; ++t) {
-            const int c = lane + 64 * t;
-            if (c < a.head_dim) { dw[key][t] += y[c] * xv[t] * r; dot += y[c] * (w ? w[c] : 1.f) * xv[t] * r; }
-        }
-        dot = wave_sum(dot) / a.head_dim;
-        for (int t = 0; t < 4; ++t) {
-            const int c = lane + 64 * t;
-            if (c < a.head_dim) o[c] = (T)(r * (y[c] * (w ? w[c] : 1.f) - xv[t] * r * dot));
+    const int ch = threadIdx.x % lph;
+    const float inv_d = 1.f / hd;
+    for (int r = 0; r < n; ++r) {
+        const long row = row0 + r;
+        for (int h0 = blockIdx.y * per; h0 < heads; h0 += gridDim.y * per) {
+            const int h = h0 + threadIdx.x / lph;               // the wave stays together: lanes without a head hold zeros
+            const bool key = h >= a.n_q_head, live = ch < chunks && h < heads;
+            const T* head = key ? (const T*)a.k + row * a.ldk + (h - a.n_q_head) * a.hsk : (const T*)a.q + row * a.ldq + h * a.hsq;
+            const Chunk<T> x = load_chunk(head + ch * E, live);
+            float y[E], o[E], A[E], B[E], ss = 0.f;
+            partners<T, TURN>(a, x, head, ch, live, o);
+            for (int e = 0; e < E; ++e) ss += x[e] * x[e];
+            const float f = 1.f / sqrtf(head_sum(ss, lph) * inv_d + a.eps);
+            if (!live) continue;                                // (whole heads: the other lanes of the wave need nothing of these any more)
+            const float* t = tables + (2 * r + key) * 2 * hd;
+            coefficients<E>(t, ch, chunks, A);
+            if (TURN != TURN_NONE) coefficients<E>(t + hd, ch, chunks, B);
+            for (int e = 0; e < E; ++e) y[e] = f * (TURN == TURN_NONE ? x[e] * A[e] : x[e] * A[e] + o[e] * B[e]);
+            store_chunk((key ? (T*)a.k_out + row * a.ldko + (h - a.n_q_head) * a.hsko : (T*)a.q_out + row * a.ldqo + h * a.hsqo) + ch * E, y);
         }
     }
-    for (int i = 0; i < 2; ++i)
-        for (int t = 0; t < 4; ++t) part[((long)blockIdx.x * 2 + i) * 256 + lane + 64 * t] = dw[i][t];
 }
 
-__global__ __launch_bounds__(256) void head_weight_grad(bigc_head_norm a, const float* part) {
+// Backward: dn = dy turned back, dw += dn xhat, dx = r (dn w - xhat mean(dn w xhat)), xhat = x r.  Block b takes rows b, b + gridDim.x, ...
+// LDS: w of queries and keys, two rows' cos and +- sin (the next row's are written while the last one's may still be read).
+template <typename T, int TURN>
+__global__ __launch_bounds__(THREADS) void head_norm_bwd(bigc_head_norm a, int lph, float* part) {
+    constexpr int E = 16 / sizeof(T);
+    extern __shared__ float4 lds4[];
+    float* weights = (float*)lds4;                              // [q, k][head_dim]
+    const int heads = a.n_q_head + a.n_k_head, per = blockDim.x / lph, hd = a.head_dim, chunks = hd / E;
+    float* turns = weights + 2 * hd;                            // [2][cos, sin][head_dim]
+    float* sums = turns + 4 * hd;                               // [threads][E]
+    for (int i = threadIdx.x; i < 2 * hd; i += blockDim.x) {
+        const float* w = i >= hd ? a.wk : a.wq;
+        weights[(i >= hd ? hd : 0) + slot<E>(i % hd, chunks)] = w ? w[i % hd] : 1.f;
+    }
+    for (int i = threadIdx.x; i < 2 * hd; i += blockDim.x) {    // what does not turn
+        turns[i / hd * 2 * hd + slot<E>(i % hd, chunks)] = 1.f;
+        turns[i / hd * 2 * hd + hd + slot<E>(i % hd, chunks)] = 0.f;
+    }
+    __syncthreads();
+    float dwq[E], dwk[E];
+    for (int e = 0; e < E; ++e) dwq[e] = dwk[e] = 0.f;
+    const int ch = threadIdx.x % lph;
+    const float inv_d = 1.f / hd;
+    int flip = 0;
+    for (long row = blockIdx.x; row < a.n_rows; row += gridDim.x, flip ^= 1) {
+        float* t = turns + flip * 2 * hd;
+        if (TURN != TURN_NONE) {
+            for (int f = threadIdx.x; f < a.n_freq; f += blockDim.x) {
+                const float2 v = turn(a.pos[row], a.inv_freq[f]);
+                const int c = slot<E>(a.interleaved ? 2 * f : f, chunks), o = slot<E>(a.interleaved ? 2 * f + 1 : f + a.n_freq, chunks);
+                t[c] = t[o] = v.x;
+                t[hd + c] = v.y;
+                t[hd + o] = -v.y;
+            }
+            __syncthreads();
+        }
+        for (int h0 = 0; h0 < heads; h0 += per) {
+            const int h = h0 + threadIdx.x / lph;
+            const bool key = h >= a.n_q_head, live = ch < chunks && h < heads;
+            const int hh = key ? h - a.n_q_head : h;
+            const Chunk<T> x = load_chunk((key ? (const T*)a.k + row * a.ldk + hh * a.hsk : (const T*)a.q + row * a.ldq + hh * a.hsq) + ch * E, live);
+            const T* up = key ? (const T*)a.dk_out + row * a.lddko + hh * a.hsdko : (const T*)a.dq_out + row * a.lddqo + hh * a.hsdqo;
+            const Chunk<T> g = load_chunk(up + ch * E, live);
+            float dn[E], o[E], c[E], s[E], w[E], ss = 0.f, dot = 0.f;
+            partners<T, TURN>(a, g, up, ch, live, o);
+            const int at = min(ch, chunks - 1);
+            coefficients<E>(weights + key * hd, at, chunks, w);
+            if (TURN != TURN_NONE) { coefficients<E>(t, at, chunks, c); coefficients<E>(t + hd, at, chunks, s); }
+            for (int e = 0; e < E; ++e) {
+                dn[e] = TURN == TURN_NONE ? g[e] : g[e] * c[e] + o[e] * s[e];       // 0 in lanes without a head
+                ss += x[e] * x[e];
+            }
+            const float r = 1.f / sqrtf(head_sum(ss, lph) * inv_d + a.eps);
+            for (int e = 0; e < E; ++e) {
+                const float hat = x[e] * r, d = dn[e] * hat;
+                if (key) dwk[e] += live ? d : 0.f; else dwq[e] += live ? d : 0.f;
+                dn[e] *= w[e];
+                dot += dn[e] * hat;
+            }
+            dot = head_sum(dot, lph) * inv_d;
+            for (int e = 0; e < E; ++e) dn[e] = r * (dn[e] - x[e] * r * dot);
+            if (live) store_chunk((key ? (T*)a.dk + row * a.lddk + hh * a.hsdk : (T*)a.dq + row * a.lddq + hh * a.hsdq) + ch * E, dn);
+        }
+    }
+    if (!part) return;
+    for (int i = 0; i < 2; ++i) {                               // the block's threads of one chunk, in their order
+        __syncthreads();
+        for (int e = 0; e < E; ++e) sums[threadIdx.x * E + e] = i ? dwk[e] : dwq[e];
+        __syncthreads();
+        for (int cc = threadIdx.x; cc < a.head_dim; cc += blockDim.x) {
+            float x = 0.f;
+            for (int t = cc / E; t < (int)blockDim.x; t += lph) x += sums[t * E + cc % E];
+            part[((long)blockIdx.x * 2 + i) * a.head_dim + cc] = x;
+        }
+    }
+}
+
+// 32 columns of one weight (blockIdx.y: 0 wq, 1 wk) in a block: eight threads a column, each every eighth partial sum, joined in order
+__global__ __launch_bounds__(256) void head_weight_grad(bigc_head_norm a, const float* part, int blocks) {
+    __shared__ float sums[8][32];
+    const int c = blockIdx.x * 32 + threadIdx.x % 32, g = threadIdx.x / 32;
     float x = 0.f;
-    for (int b = 0; b < ROW_BLOCKS; ++b) x += part[((long)b * 2 + blockIdx.x) * 256 + threadIdx.x];
-    float* dw = blockIdx.x ? a.dwk : a.dwq;
-    if (dw && threadIdx.x < a.head_dim) dw[threadIdx.x] = x;
+    if (c < a.head_dim)
+        for (int b = g; b < blocks; b += 8) x += part[((long)b * 2 + blockIdx.y) * a.head_dim + c];
+    sums[g][threadIdx.x % 32] = x;
+    __syncthreads();
+    float* dw = blockIdx.y ? a.dwk : a.dwq;
+    if (g == 0 && c < a.head_dim && dw) {
+        for (int i = 1; i < 8; ++i) x += sums[i][threadIdx.x];
+        dw[c] = x;
+    }
+}
+
+// Lanes of a head, how its columns are turned, and the waves of a block: of 4 to 8 waves the number that leaves fewest of them without a head in
+// a row's last round (40 heads, four to a wave: five waves, two rounds).
+struct Shape { int lph, turn, rounds, waves; };
+Shape shape_of(const bigc_head_norm& a) {
+    const int e = 16 / seq_size(a.dtype);
+    int lph = 1;
+    while (lph * e < a.head_dim) lph *= 2;
+    const int need = cdiv((a.n_q_head + a.n_k_head) * lph, 64);
+    int waves = need < 4 ? need : 4;
+    for (int w = 5; w <= MAX_WAVES && w <= need; ++w)
+        if (cdiv(need, w) * w < cdiv(need, waves) * waves || w == need) waves = w;
+    return {lph, a.n_freq == 0 ? TURN_NONE : a.interleaved ? TURN_PAIRS : a.n_freq % e == 0 ? TURN_HALVES : TURN_ANY, cdiv(need, waves), waves};
 }
 
 int check_rows(const bigc_head_norm& a, const char* who, const char* what, const void* p, int64_t ld, int64_t hs, int heads) {
@@ -115,6 +265,13 @@ int check_args(const bigc_head_norm* ap, const char* who) {
     return BIGC_OK;
 }
 
+int bwd_blocks(const bigc_head_norm& a) { return (int)(a.n_rows < 1 ? 1 : a.n_rows < BWD_BLOCKS ? a.n_rows : BWD_BLOCKS); }
+
+#define TURNS(turn, T, kernel, grid, threads, lds, stream, ...) do { \
+    if (turn == TURN_NONE) kernel<T, TURN_NONE><<<grid, threads, lds, stream>>>(__VA_ARGS__); \
+    else if (turn == TURN_HALVES) kernel<T, TURN_HALVES><<<grid, threads, lds, stream>>>(__VA_ARGS__); \
+    else if (turn == TURN_PAIRS) kernel<T, TURN_PAIRS><<<grid, threads, lds, stream>>>(__VA_ARGS__); \
+    else kernel<T, TURN_ANY><<<grid, threads, lds, stream>>>(__VA_ARGS__); } while (0);
 #define SEQ_DISPATCH(dtype, F) do { if ((dtype) == BIGC_F32) { F(float) } else if ((dtype) == BIGC_F16) { F(f16_t) } else { F(bf16_t) } } while (0)
 }  // namespace
 
@@ -129,7 +286,13 @@ extern "C" int bigc_head_norm_rope_fwd(void* stream, const bigc_head_norm* ap) {
     if ((rc = check_rows(a, who, "k_out", a.k_out, a.ldko, a.hsko, a.n_k_head)) != BIGC_OK) return rc;
     if (a.n_rows == 0) return BIGC_OK;
     ProfScope prof(stream, FAM_LAYERNORM, 0, 0);
-#define F(T) head_rows_fwd<T><<<(unsigned)(a.n_rows * (a.n_q_head + a.n_k_head)), 64, 0, (hipStream_t)stream>>>(a);
+    // Four rows a block, all heads of each; while that would leave CUs without a block, one row and one round of heads a block instead (a call of a
+    // few rows is latency: its threads then make one trip through memory).
+    const Shape sh = shape_of(a);
+    const bool few = a.n_rows < ROWS_PER_BLOCK * 1024;
+    const int rows = few ? 1 : ROWS_PER_BLOCK;
+    const dim3 grid((unsigned)((a.n_rows + rows - 1) / rows), few ? sh.rounds : 1);
+#define F(T) TURNS(sh.turn, T, head_norm_fwd, grid, 64 * sh.waves, sizeof(float) * rows * 4 * a.head_dim, (hipStream_t)stream, a, sh.lph, rows)
     SEQ_DISPATCH(a.dtype, F);
 #undef F
     BIGC_LAUNCH_CHECK("head_norm_rope_fwd");
@@ -138,7 +301,7 @@ extern "C" int bigc_head_norm_rope_fwd(void* stream, const bigc_head_norm* ap) {
 
 extern "C" size_t bigc_head_norm_rope_workspace_bytes(const bigc_head_norm* a) {
     if (check_args(a, "head_norm_rope_workspace_bytes") != BIGC_OK) return 0;
-    return sizeof(float) * ROW_BLOCKS * 2 * 256;
+    return sizeof(float) * bwd_blocks(*a) * 2 * a->head_dim;
 }
 
 extern "C" int bigc_head_norm_rope_bwd(void* stream, const bigc_head_norm* ap, void* workspace, size_t workspace_bytes) {
@@ -157,10 +320,13 @@ extern "C" int bigc_head_norm_rope_bwd(void* stream, const bigc_head_norm* ap, v
         return bigc_fail(BIGC_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
     ProfScope prof(stream, FAM_BACKWARD, 0, 0);
     float* part = (float*)workspace;
-#define F(T) head_rows_bwd<T><<<ROW_BLOCKS, 64, 0, (hipStream_t)stream>>>(a, part);
+    const Shape sh = shape_of(a);
+    const bool weights = a.dwq || a.dwk;
+    const int blocks = bwd_blocks(a);
+#define F(T) TURNS(sh.turn, T, head_norm_bwd, blocks, 64 * sh.waves, sizeof(float) * (6 * a.head_dim + 64 * sh.waves * (16 / seq_size(a.dtype))), (hipStream_t)stream, a, sh.lph, weights ? part : nullptr)
     SEQ_DISPATCH(a.dtype, F);
 #undef F
-    if (a.dwq || a.dwk) head_weight_grad<<<2, 256, 0, (hipStream_t)stream>>>(a, part);
+    if (weights) head_weight_grad<<<dim3(cdiv(a.head_dim, 32), 2), 256, 0, (hipStream_t)stream>>>(a, part, blocks);
     BIGC_LAUNCH_CHECK("head_norm_rope_bwd");
     return BIGC_OK;
 }
