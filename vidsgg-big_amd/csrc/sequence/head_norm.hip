@@ -13,7 +13,7 @@ namespace {
 constexpr int MAX_WAVES = 8, THREADS = 64 * MAX_WAVES;         // of a block at most
 constexpr int MAX_FREQ = 128;
 constexpr int ROWS_PER_BLOCK = 4;
-constexpr int BWD_BLOCKS = 1024;                                // of the backward: each sums its rows' weight gradients (four blocks on every CU)
+constexpr int BWD_BLOCKS = 768;                                 // of the backward, each summing its rows' weight gradients: three of 8 waves on every CU
 
 enum { TURN_NONE, TURN_HALVES, TURN_PAIRS, TURN_ANY };          // how a chunk meets its partner columns: none; a whole chunk n_freq columns away; inside the chunk; column by column
 
@@ -135,8 +135,10 @@ __global__ __launch_bounds__(THREADS) void head_norm_fwd(bigc_head_norm a, int l
 
 // Backward: dn = dy turned back, dw += dn xhat, dx = r (dn w - xhat mean(dn w xhat)), xhat = x r.  Block b takes rows b, b + gridDim.x, ...
 // LDS: w of queries and keys, two rows' cos and +- sin (the next row's are written while the last one's may still be read).
+// Held to the registers of six waves a SIMD, so that all blocks run at once (8192 rows x 24 + 8 heads of 128, bf16, forward and backward: 87 us; 95 - 101
+// at four waves, 146 at eight, which spill).
 template <typename T, int TURN>
-__global__ __launch_bounds__(THREADS) void head_norm_bwd(bigc_head_norm a, int lph, float* part) {
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(6))) void head_norm_bwd(bigc_head_norm a, int lph, float* part) {
     constexpr int E = 16 / sizeof(T);
     extern __shared__ float4 lds4[];
     float* weights = (float*)lds4;                              // [q, k][head_dim]
@@ -210,20 +212,23 @@ __global__ __launch_bounds__(THREADS) void head_norm_bwd(bigc_head_norm a, int l
     }
 }
 
-// 32 columns of one weight (blockIdx.y: 0 wq, 1 wk) in a block: eight threads a column, each every eighth partial sum, joined in order
-__global__ __launch_bounds__(256) void head_weight_grad(bigc_head_norm a, const float* part, int blocks) {
-    __shared__ float sums[8][32];
+// 32 columns of one weight (blockIdx.y: 0 wq, 1 wk) in a block: 32 threads a column, each every 32nd partial sum (eight of them on their way at a
+// time: with eight threads a column, one after the other, this took 35 us, as long as the backward itself), joined in order
+__global__ __launch_bounds__(1024) void head_weight_grad(bigc_head_norm a, const float* part, int blocks) {
+    __shared__ float sums[32][33];
     const int c = blockIdx.x * 32 + threadIdx.x % 32, g = threadIdx.x / 32;
     float x = 0.f;
-    if (c < a.head_dim)
-        for (int b = g; b < blocks; b += 8) x += part[((long)b * 2 + blockIdx.y) * a.head_dim + c];
+    for (int b0 = g; b0 < blocks; b0 += 32 * 8) {
+        float v[8];
+        for (int i = 0; i < 8; ++i) v[i] = b0 + 32 * i < blocks && c < a.head_dim ? part[((long)(b0 + 32 * i) * 2 + blockIdx.y) * a.head_dim + c] : 0.f;
+        for (int i = 0; i < 8; ++i) x += v[i];
+    }
     sums[g][threadIdx.x % 32] = x;
     __syncthreads();
+    x = sums[threadIdx.x % 32][g];                              // now column g of the block, one partial sum a lane
+    for (int m = 16; m; m >>= 1) x += __shfl_xor(x, m);
     float* dw = blockIdx.y ? a.dwk : a.dwq;
-    if (g == 0 && c < a.head_dim && dw) {
-        for (int i = 1; i < 8; ++i) x += sums[i][threadIdx.x];
-        dw[c] = x;
-    }
+    if (threadIdx.x % 32 == 0 && blockIdx.x * 32 + g < a.head_dim && dw) dw[blockIdx.x * 32 + g] = x;
 }
 
 // Lanes of a head, how its columns are turned, and the waves of a block: of 4 to 8 waves the number that leaves fewest of them without a head in
@@ -326,7 +331,7 @@ extern "C" int bigc_head_norm_rope_bwd(void* stream, const bigc_head_norm* ap, v
 #define F(T) TURNS(sh.turn, T, head_norm_bwd, blocks, 64 * sh.waves, sizeof(float) * (6 * a.head_dim + 64 * sh.waves * (16 / seq_size(a.dtype))), (hipStream_t)stream, a, sh.lph, weights ? part : nullptr)
     SEQ_DISPATCH(a.dtype, F);
 #undef F
-    if (weights) head_weight_grad<<<dim3(cdiv(a.head_dim, 32), 2), 256, 0, (hipStream_t)stream>>>(a, part, blocks);
+    if (weights) head_weight_grad<<<dim3(cdiv(a.head_dim, 32), 2), 1024, 0, (hipStream_t)stream>>>(a, part, blocks);
     BIGC_LAUNCH_CHECK("head_norm_rope_bwd");
     return BIGC_OK;
 }
