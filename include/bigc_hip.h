@@ -688,7 +688,7 @@ BIGC_API int bigc_linear_hr8out_f32(void* stream, const float* A, int lda, const
  * -- position biases, caps and masks on the scores, shared key heads, norms and rotations of the heads.  They stand next to
  * bigc_mha_core_f32 (no order, no masks, one key head per query head) and take IEEE f32, f16 and bfloat16 tensors; scores,
  * softmax statistics, sums and parameter gradients are f32 whatever the tensors' type.  (models/ has no caller of its own.)
- * Every row pointer, row stride and head stride has to be a multiple of 16 bytes (with one head its stride is not read).
+ * Every row pointer, row stride and head stride has to be a multiple of 16 bytes (with one head its stride is not read), a row stride at most 2^22 elements.
  * ---------------------------------------------------------------------------------- */
 
 #define BIGC_F32 0
@@ -704,8 +704,8 @@ BIGC_API int bigc_linear_hr8out_f32(void* stream, const float* A, int lda, const
  *     seen  = (no documents or q_doc[i] == k_doc[j] >= 0) and (j < prefix_len[s] or
  *             ((!causal or d <= 0) and (window_left < 0 or -d <= window_left) and (window_right < 0 or d <= window_right)))
  *     o = softmax over the seen keys of the scores, times v
- * A query that sees no key (or only scores of -inf) has o = 0 and lse = -inf and gives no gradient; what a hidden place holds (NaN, Inf) is
- * never part of a result.  slopes, rel_table + rel_map, prefix_len, q_doc + k_doc may be NULL.  Rows outside every sequence
+ * A query that sees no key (or only scores of -inf) has o = 0 and gives no gradient; what a hidden place holds (NaN, Inf) is never part of a
+ * result.  A bias of -inf hides its distances, the lowest finite values (below -2.3e38, which count as one) do not.  slopes, rel_table + rel_map, prefix_len, q_doc + k_doc may be NULL.  Rows outside every sequence
  * stay as they were.  Offsets are cut to [0, n_q] and [0, n_k] and lengths to max_q and max_k (which size the launch), map entries to the table. */
 typedef struct {
     int32_t dtype;                     /* BIGC_F32 / BIGC_F16 / BIGC_BF16: q, k, v, o, d_o, dq, dk, dv */
@@ -713,6 +713,7 @@ typedef struct {
     int32_t head_dim;                  /* a multiple of 8, at most 128 */
     int32_t max_q, max_k;              /* the longest sequence's rows */
     int32_t causal, window_left, window_right; /* windows: -1 = none */
+    int32_t zero_rest;                 /* not 0: rows outside every sequence of o (forward), dq, dk, dv (backward) become 0 instead of staying as they were */
     int32_t bias_radius, n_bucket;     /* rel_map has 2 * bias_radius + 1 entries (bias_radius <= 2047), rel_table n_bucket rows of n_head */
     float scale, softcap;              /* softcap 0: none */
     int64_t n_q, n_k;                  /* rows of q / o and of k / v, below 2^31 */
@@ -725,9 +726,10 @@ typedef struct {
     const void* k; int64_t ldk, hsk;
     const void* v; int64_t ldv, hsv;
     void* o; int64_t ldo, hso;         /* bigc_seq_attn_bwd reads it */
-    float* lse;                        /* (n_q, n_head) log of the sum of exp(score); optional in the forward, read by the backward */
-    float* o32;                        /* (n_q, n_head, head_dim) o before its rounding; optional; read by the backward instead of o where given:
-                                        * f16 / bf16 rel_table gradients are then exact to f32 */
+    float* stats;                      /* (n_q, n_head, 2): m and l of every row's softmax, P = 2^(score log2 e - m) / l (the log of the sum of exp is
+                                        * m ln 2 + ln l; l = 0: nothing seen); optional in the forward, read by the backward */
+    float* o32;                        /* (n_q, n_head, head_dim) o before its rounding, and for f16 / bf16 from probabilities of twice the bits; optional; read by
+                                        * the backward instead of o where given: sums of many dS, as rel_table's gradient, keep more bits than the tensors' type has */
     /* backward only */
     const void* d_o; int64_t lddo, hsdo;
     void* dq; int64_t lddq, hsdq;
@@ -740,7 +742,7 @@ typedef struct {
 BIGC_API size_t bigc_seq_attn_workspace_bytes(const bigc_seq_attn* a, int backward);
 /* Forward.  Few query rows over many keys are split over the keys and joined; repeats bit for bit. */
 BIGC_API int bigc_seq_attn_fwd(void* stream, const bigc_seq_attn* a, void* workspace, size_t workspace_bytes);
-/* Backward from lse and o (or o32) of the forward; every sum in a fixed order, no atomics: repeats bit for bit. */
+/* Backward from stats and o (or o32) of the forward; every sum in a fixed order, no atomics: repeats bit for bit. */
 BIGC_API int bigc_seq_attn_bwd(void* stream, const bigc_seq_attn* a, void* workspace, size_t workspace_bytes);
 
 /* RMS norm of every query and key head and the rotation of its first 2 * n_freq columns by the row's position, in one launch:

@@ -31,7 +31,7 @@ def attn(**kw):
         setattr(a, n, FAKE)
         setattr(a, {"d_o": "lddo"}.get(n, "ld" + n), 256)
         setattr(a, {"d_o": "hsdo"}.get(n, "hs" + n), 64)
-    a.lse = FAKE
+    a.stats = FAKE
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -62,7 +62,7 @@ def test_attention_refuses_rows(lib, kw):
     assert lib.bigc_seq_attn_bwd(None, ctypes.byref(a), FAKE, 1 << 40) == -1
 
 
-@pytest.mark.parametrize("kw", [dict(d_o=None), dict(dq=FAKE + 4), dict(lddk=3), dict(hsdv=1), dict(lse=None), dict(d_rel_table=FAKE)], ids=str)
+@pytest.mark.parametrize("kw", [dict(d_o=None), dict(dq=FAKE + 4), dict(lddk=3), dict(hsdv=1), dict(stats=None), dict(stats=FAKE + 4), dict(d_rel_table=FAKE)], ids=str)
 def test_attention_backward_refuses(lib, kw):
     assert lib.bigc_seq_attn_bwd(None, ctypes.byref(attn(**kw)), FAKE, 1 << 40) == -1
 

@@ -58,11 +58,11 @@ class grd_batch(ctypes.Structure):
 class bigc_seq_attn(ctypes.Structure):
     _fields_ = [("dtype", c_int32), ("n_seq", c_int32), ("n_head", c_int32), ("n_kv_head", c_int32), ("head_dim", c_int32),
                 ("max_q", c_int32), ("max_k", c_int32), ("causal", c_int32), ("window_left", c_int32), ("window_right", c_int32),
-                ("bias_radius", c_int32), ("n_bucket", c_int32), ("scale", c_float), ("softcap", c_float), ("n_q", c_int64),
+                ("zero_rest", c_int32), ("bias_radius", c_int32), ("n_bucket", c_int32), ("scale", c_float), ("softcap", c_float), ("n_q", c_int64),
                 ("n_k", c_int64), ("q_off", c_void_p), ("k_off", c_void_p), ("slopes", c_void_p), ("rel_table", c_void_p),
                 ("rel_map", c_void_p), ("prefix_len", c_void_p), ("q_doc", c_void_p), ("k_doc", c_void_p), ("q", c_void_p),
                 ("ldq", c_int64), ("hsq", c_int64), ("k", c_void_p), ("ldk", c_int64), ("hsk", c_int64), ("v", c_void_p), ("ldv", c_int64),
-                ("hsv", c_int64), ("o", c_void_p), ("ldo", c_int64), ("hso", c_int64), ("lse", c_void_p), ("o32", c_void_p),
+                ("hsv", c_int64), ("o", c_void_p), ("ldo", c_int64), ("hso", c_int64), ("stats", c_void_p), ("o32", c_void_p),
                 ("d_o", c_void_p), ("lddo", c_int64), ("hsdo", c_int64), ("dq", c_void_p), ("lddq", c_int64), ("hsdq", c_int64),
                 ("dk", c_void_p), ("lddk", c_int64), ("hsdk", c_int64), ("dv", c_void_p), ("lddv", c_int64), ("hsdv", c_int64),
                 ("d_rel_table", c_void_p)]

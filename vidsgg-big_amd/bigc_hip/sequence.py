@@ -8,6 +8,7 @@ may be captured into a graph (outputs and workspaces are torch allocations of th
 calls them from its ``backward``, as the training steps of this package do with theirs.
 """
 import ctypes
+import math
 
 import torch
 
@@ -72,11 +73,18 @@ def _stream(device):
 
 
 class SavedAttention(object):
-    """What ``attend(..., save=True)`` keeps for ``attend_bwd``: the arguments, the output (before its rounding too, for f16 / bf16) and the
-    rows' log-sum-exp.  The tensors must not change in between."""
+    """What ``attend(..., save=True)`` keeps for ``attend_bwd``: the arguments, the output (with more bits too, where an f16 / bf16 call has a
+    rel_table) and the rows' softmax statistics.  The tensors must not change in between."""
 
-    def __init__(self, args, tensors, o, lse, o32):
-        self.args, self.tensors, self.o, self.lse, self.o32 = args, tensors, o, lse, o32
+    def __init__(self, args, tensors, o, stats, o32):
+        self.args, self.tensors, self.o, self.stats, self.o32 = args, tensors, o, stats, o32
+
+    @property
+    def lse(self):
+        """(n_q, n_head) f32: log of the sum of exp of a row's scores, -inf where it sees nothing (rows outside every sequence: undefined)"""
+        m, l = self.stats.unbind(-1)
+        lowest = torch.finfo(torch.float32).min                          # stands for every score from there up to times ln 2
+        return torch.where(l == 0, torch.full_like(m, float("-inf")), torch.where(m == lowest, m, m * math.log(2.0) + torch.log(l)))
 
 
 def attend(q, k, v, q_off, k_off, max_q, max_k, scale=None, softcap=0.0, slopes=None, rel_table=None, rel_map=None, causal=False, window=(-1, -1),
@@ -105,26 +113,26 @@ def attend(q, k, v, q_off, k_off, max_q, max_k, scale=None, softcap=0.0, slopes=
         assert rel_table.dim() == 2 and rel_map.dim() == 1 and rel_map.shape[0] % 2 == 1, "rel_table (n_bucket, n_head), rel_map (2 R + 1)"
         n_bucket, radius = rel_table.shape[0], rel_map.shape[0] // 2
     i32, f32 = torch.int32, torch.float32
-    o = q.new_zeros(shape) if out is None else out
-    lse = o32 = None
+    o = q.new_empty(shape) if out is None else out
+    stats = o32 = None
     if save:
-        lse = q.new_empty((n_q, n_head), dtype=f32)
-        if dtype is not f32:
+        stats = q.new_empty((n_q, n_head, 2), dtype=f32)
+        if dtype is not f32 and rel_table is not None:                   # its gradient is f32: see o32 in bigc_hip.h
             o32 = q.new_empty(shape, dtype=f32)
     a = bigc_seq_attn(                                                   # the fields in the structure's order
-        _DTYPES[dtype], n_seq, n_head, kshape[1], hd, max_q, max_k, 1 if causal else 0, window[0], window[1], radius, n_bucket,
+        _DTYPES[dtype], n_seq, n_head, kshape[1], hd, max_q, max_k, 1 if causal else 0, window[0], window[1], 1 if out is None else 0, radius, n_bucket,
         hd ** -0.5 if scale is None else scale, softcap, n_q, kshape[0],
         _vector("q_off", q_off, i32, (n_seq + 1,), dev), _vector("k_off", k_off, i32, (n_seq + 1,), dev), _vector("slopes", slopes, f32, (n_head,), dev),
         _vector("rel_table", rel_table, f32, (n_bucket, n_head), dev), _vector("rel_map", rel_map, i32, (2 * radius + 1,), dev),
         _vector("prefix_len", prefix_len, i32, (n_seq,), dev), _vector("q_doc", q_doc, i32, (n_q,), dev), _vector("k_doc", k_doc, i32, (kshape[0],), dev),
         *_rows("q", q, dtype, dev, shape), *_rows("k", k, dtype, dev, kshape), *_rows("v", v, dtype, dev, kshape), *_rows("out", o, dtype, dev, shape),
-        _lib.ptr(lse), _lib.ptr(o32))
+        _lib.ptr(stats), _lib.ptr(o32))
     need = lib.bigc_seq_attn_workspace_bytes(ctypes.byref(a), 0)
     ws = q.new_empty((need,), dtype=torch.uint8) if need else None
     _lib.check(lib.bigc_seq_attn_fwd(_stream(dev), ctypes.byref(a), _lib.ptr(ws), need))
     if not save:
         return o
-    return o, SavedAttention(a, (q, k, v, q_off, k_off, slopes, rel_table, rel_map, prefix_len, q_doc, k_doc), o, lse, o32)
+    return o, SavedAttention(a, (q, k, v, q_off, k_off, slopes, rel_table, rel_map, prefix_len, q_doc, k_doc), o, stats, o32)
 
 
 def attend_bwd(saved, d_o):
@@ -139,7 +147,8 @@ def attend_bwd(saved, d_o):
     a = bigc_seq_attn()
     ctypes.memmove(ctypes.byref(a), ctypes.byref(saved.args), ctypes.sizeof(a))
     a.d_o, a.lddo, a.hsdo = _rows("d_o", d_o, q.dtype, q.device, q.shape)
-    dq, dk, dv = q.new_zeros(q.shape), k.new_zeros(k.shape), v.new_zeros(v.shape)
+    a.zero_rest = 1
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     a.dq, a.lddq, a.hsdq = _rows("dq", dq, q.dtype, q.device, q.shape)
     a.dk, a.lddk, a.hsdk = _rows("dk", dk, q.dtype, q.device, k.shape)
     a.dv, a.lddv, a.hsdv = _rows("dv", dv, q.dtype, q.device, v.shape)

@@ -1,6 +1,5 @@
 // Attention over ordered rows: entry points, checks, and the kernels.
-#include "sequence.h"
-#include <math.h>
+#include "attention_fwd.h"
 
 namespace {
 
@@ -35,51 +34,6 @@ __device__ Score score_of(const bigc_seq_attn& a, const float* qrow, const T* kr
     }
     r.s = x;
     return r;
-}
-
-template <typename T>
-__global__ __launch_bounds__(64) void rows_fwd(bigc_seq_attn a) {
-    __shared__ float qs[128];
-    const int lane = threadIdx.x, h = blockIdx.x % a.n_head;
-    const long r = blockIdx.x / a.n_head;
-    const int s = (int)(r / a.max_q), i = (int)(r % a.max_q);
-    const SeqSpan sp = seq_span(a, s);
-    if (i >= sp.nq) return;
-    const long row = sp.q0 + i;
-    const T* q = (const T*)a.q + row * a.ldq + h * a.hsq;
-    for (int c = lane; c < a.head_dim; c += 64) qs[c] = (float)q[c];
-    __syncthreads();
-    const int hk = h / (a.n_head / a.n_kv_head), pos = i + sp.nk - sp.nq;
-    const int prefix = a.prefix_len ? a.prefix_len[s] : 0, qdoc = a.q_doc ? a.q_doc[row] : 0;
-    float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
-    for (int j0 = 0; j0 < sp.nk; j0 += 64) {
-        const int j = j0 + lane;
-        float sc = -INFINITY;
-        bool seen = false;
-        if (j < sp.nk) {
-            const Score e = score_of<T>(a, qs, (const T*)a.k + (long)(sp.k0 + j) * a.ldk + hk * a.hsk, h, prefix, pos, j, qdoc, a.k_doc ? a.k_doc[sp.k0 + j] : 0);
-            sc = e.s; seen = e.seen;
-        }
-        const float mn = fmaxf(m, wave_max(sc)), ms = mn == -INFINITY ? 0.f : mn;
-        const float corr = expf(m - ms), p = seen ? expf(sc - ms) : 0.f;
-        l = l * corr + wave_sum(p);
-        m = mn;
-        o[0] *= corr; o[1] *= corr;
-        for (int jj = 0; jj < 64 && j0 + jj < sp.nk; ++jj) {
-            const float pj = __shfl(p, jj);
-            if (pj == 0.f) continue;
-            const T* v = (const T*)a.v + (long)(sp.k0 + j0 + jj) * a.ldv + hk * a.hsv;
-            for (int t = 0; t < 2; ++t) if (lane + 64 * t < a.head_dim) o[t] += pj * (float)v[lane + 64 * t];
-        }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (a.lse && lane == 0) a.lse[row * a.n_head + h] = l == 0.f ? -INFINITY : m + logf(l);
-    for (int t = 0; t < 2; ++t) {
-        const int c = lane + 64 * t;
-        if (c >= a.head_dim) continue;
-        ((T*)a.o)[row * a.ldo + h * a.hso + c] = (T)(o[t] * inv);
-        if (a.o32) a.o32[(row * a.n_head + h) * a.head_dim + c] = o[t] * inv;
-    }
 }
 
 // delta = dO . O per (row, head)
@@ -119,7 +73,7 @@ __global__ __launch_bounds__(64) void rows_dq(bigc_seq_attn a, const float* delt
         }
         __syncthreads();
         const int pos = i + sp.nk - sp.nq, prefix = a.prefix_len ? a.prefix_len[s] : 0, qdoc = a.q_doc ? a.q_doc[row] : 0;
-        const float lse = a.lse[row * a.n_head + h], dl = delta[row * a.n_head + h];
+        const float m = a.stats[2 * (row * a.n_head + h)], l = a.stats[2 * (row * a.n_head + h) + 1], dl = delta[row * a.n_head + h];
         float g[2] = {0.f, 0.f};
         for (int j0 = 0; j0 < sp.nk; j0 += 64) {
             const int j = j0 + lane;
@@ -127,11 +81,11 @@ __global__ __launch_bounds__(64) void rows_dq(bigc_seq_attn a, const float* delt
             int bin = 0;
             if (j < sp.nk) {
                 const Score e = score_of<T>(a, qs, (const T*)a.k + (long)(sp.k0 + j) * a.ldk + hk * a.hsk, h, prefix, pos, j, qdoc, a.k_doc ? a.k_doc[sp.k0 + j] : 0);
-                if (e.seen && lse != -INFINITY) {
+                if (e.seen && l != 0.f) {
                     const T* v = (const T*)a.v + (long)(sp.k0 + j) * a.ldv + hk * a.hsv;
                     float dp = 0.f;
                     for (int c = 0; c < a.head_dim; ++c) dp += go[c] * (float)v[c];
-                    ds = expf(e.s - lse) * (dp - dl);
+                    ds = exp2f(e.s * LOG2E - m) / l * (dp - dl);
                     dx = ds * e.dcap * a.scale;
                     bin = e.bin;
                     if (bin > 0 && bin < nbin - 1) bins[bin] += ds;      // the lanes' distances differ
@@ -178,13 +132,13 @@ __global__ __launch_bounds__(64) void rows_dkv(bigc_seq_attn a, const float* del
             float p = 0.f, ds = 0.f;
             if (i < sp.nq) {
                 const long qr = sp.q0 + i;
-                const float lse = a.lse[qr * a.n_head + h];
+                const float m = a.stats[2 * (qr * a.n_head + h)], l = a.stats[2 * (qr * a.n_head + h) + 1];
                 const Score e = score_of<T>(a, ks, (const T*)a.q + qr * a.ldq + h * a.hsq, h, prefix, i + sp.nk - sp.nq, j, a.q_doc ? a.q_doc[qr] : 0, kdoc);
-                if (e.seen && lse != -INFINITY) {
+                if (e.seen && l != 0.f) {
                     const T* go = (const T*)a.d_o + qr * a.lddo + h * a.hsdo;
                     float dp = 0.f;
                     for (int c = 0; c < a.head_dim; ++c) dp += vs[c] * (float)go[c];
-                    p = expf(e.s - lse);
+                    p = exp2f(e.s * LOG2E - m) / l;
                     ds = p * (dp - delta[qr * a.n_head + h]) * e.dcap * a.scale;
                 }
             }
@@ -230,9 +184,8 @@ __global__ __launch_bounds__(256) void rel_table_grad(bigc_seq_attn a, const flo
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
 
 struct Plan { size_t delta, by_dist, total; };
-Plan plan_of(const bigc_seq_attn& a, int backward) {
+Plan plan_of(const bigc_seq_attn& a) {
     Plan p = {0, 0, 0};
-    if (!backward) return p;
     p.by_dist = up(sizeof(float) * (size_t)a.n_q * a.n_head);
     p.total = p.by_dist + (a.d_rel_table ? up(sizeof(float) * BIN_BLOCKS * (size_t)a.n_head * (2 * a.bias_radius + 1)) : 0);
     return p;
@@ -244,7 +197,7 @@ int check_rows(const bigc_seq_attn& a, const char* who, const char* what, const 
     BIGC_CHECK_ARG(p, "%s: %s is NULL", who, what);
     BIGC_CHECK_ARG((uintptr_t)p % 16 == 0 && ld % e == 0 && (heads == 1 || hs % e == 0),
                    "%s: %s: address, row stride %ld and head stride %ld have to be multiples of 16 bytes", who, what, (long)ld, (long)hs);
-    BIGC_CHECK_ARG(ld >= 0 && (heads == 1 || hs >= 0), "%s: %s: negative stride", who, what);
+    BIGC_CHECK_ARG(ld >= 0 && ld <= (1 << 22) && (heads == 1 || hs >= 0), "%s: %s: row stride %ld (0 to 2^22 elements), head stride %ld", who, what, (long)ld, (long)hs);
     return BIGC_OK;
 }
 
@@ -257,6 +210,8 @@ int check_args(const bigc_seq_attn* ap, const char* who) {
     BIGC_CHECK_ARG(a.head_dim > 0 && a.head_dim <= 128 && a.head_dim % 8 == 0, "%s: head_dim %d (a multiple of 8 up to 128)", who, a.head_dim);
     BIGC_CHECK_ARG(a.n_q >= 0 && a.n_k >= 0 && a.n_q < (1ll << 31) && a.n_k < (1ll << 31) && a.max_q >= 0 && a.max_k >= 0, "%s: %ld query and %ld key rows, longest %d and %d",
                    who, (long)a.n_q, (long)a.n_k, a.max_q, a.max_k);
+    BIGC_CHECK_ARG((long)a.max_q + a.max_k < (1l << 31), "%s: %d queries and %d keys are too far apart", who, a.max_q, a.max_k);
+    BIGC_CHECK_ARG((double)a.n_q * a.n_head < 2147483648.0, "%s: %ld rows of %d heads are too many", who, (long)a.n_q, a.n_head);
     BIGC_CHECK_ARG(a.n_seq == 0 || (a.q_off && a.k_off), "%s: offsets are NULL", who);
     BIGC_CHECK_ARG(a.window_left >= -1 && a.window_right >= -1, "%s: window (%d, %d)", who, a.window_left, a.window_right);
     BIGC_CHECK_ARG(isfinite(a.scale) && isfinite(a.softcap) && a.softcap >= 0.f, "%s: scale %g, softcap %g", who, a.scale, a.softcap);
@@ -273,7 +228,7 @@ int check_args(const bigc_seq_attn* ap, const char* who) {
 
 extern "C" size_t bigc_seq_attn_workspace_bytes(const bigc_seq_attn* a, int backward) {
     if (check_args(a, "seq_attn_workspace_bytes") != BIGC_OK) return 0;
-    return plan_of(*a, backward).total;
+    return backward ? plan_of(*a).total : fwd_shape(*a).total;
 }
 
 extern "C" int bigc_seq_attn_fwd(void* stream, const bigc_seq_attn* ap, void* workspace, size_t workspace_bytes) {
@@ -285,15 +240,30 @@ extern "C" int bigc_seq_attn_fwd(void* stream, const bigc_seq_attn* ap, void* wo
     if ((rc = check_rows(a, who, "k", a.k, a.ldk, a.hsk, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
     if ((rc = check_rows(a, who, "v", a.v, a.ldv, a.hsv, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
     if ((rc = check_rows(a, who, "o", a.o, a.ldo, a.hso, a.n_q, a.n_head)) != BIGC_OK) return rc;
-    const Plan p = plan_of(a, 0);
-    if (workspace_bytes < p.total || (p.total && (!workspace || (uintptr_t)workspace % 16)))
-        return bigc_fail(BIGC_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.total);
-    const long n = (long)a.n_seq * a.max_q * a.n_head;
-    if (n == 0 || a.n_q == 0) return BIGC_OK;
+    BIGC_CHECK_ARG((uintptr_t)a.stats % 8 == 0 && (uintptr_t)a.o32 % 16 == 0, "%s: stats has to lie at a multiple of 8 bytes, o32 of 16", who);
+    const FwdShape sh = fwd_shape(a);
+    if (workspace_bytes < sh.total || (sh.total && (!workspace || (uintptr_t)workspace % 16)))
+        return bigc_fail(BIGC_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, sh.total);
+    if (a.n_q == 0) return BIGC_OK;
+    hipStream_t hs = (hipStream_t)stream;
     ProfScope prof(stream, FAM_MHA, 0, 0);
-#define F(T) rows_fwd<T><<<(unsigned)n, 64, 0, (hipStream_t)stream>>>(a);
-    SEQ_DISPATCH(a.dtype, F);
+    if (sh.blocks == 0) {                                       // no sequence, or none with a query
+        if (a.zero_rest) {
+#define F(T) zero_rows<T><<<256, 256, 0, hs>>>((T*)a.o, a.ldo, a.hso, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq);
+            SEQ_DISPATCH(a.dtype, F);
 #undef F
+        }
+    } else {
+        int2* ranges = (int2*)workspace;
+        float* part_o = (float*)((char*)workspace + sh.part_o);
+        float2* part_ml = (float2*)((char*)workspace + sh.part_ml);
+        const int range_tiles = (a.max_k + 63) / 64;
+        if (a.q_doc && range_tiles) doc_ranges<<<(unsigned)(((long)a.n_seq * range_tiles + 3) / 4), 256, 0, hs>>>(a, range_tiles, ranges);
+#define F(T) launch_fwd_dim<T>(hs, a, sh, ranges, part_o, part_ml); \
+        if (sh.splits > 1) attn_join<T><<<(unsigned)(((long)a.n_seq * a.max_q * a.n_head + 3) / 4), 256, 0, hs>>>(a, sh, part_o, part_ml);
+        SEQ_DISPATCH(a.dtype, F);
+#undef F
+    }
     BIGC_LAUNCH_CHECK("seq_attn_fwd");
     return BIGC_OK;
 }
@@ -311,9 +281,9 @@ extern "C" int bigc_seq_attn_bwd(void* stream, const bigc_seq_attn* ap, void* wo
     if ((rc = check_rows(a, who, "dq", a.dq, a.lddq, a.hsdq, a.n_q, a.n_head)) != BIGC_OK) return rc;
     if ((rc = check_rows(a, who, "dk", a.dk, a.lddk, a.hsdk, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
     if ((rc = check_rows(a, who, "dv", a.dv, a.lddv, a.hsdv, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
-    BIGC_CHECK_ARG(a.lse || a.n_q == 0, "%s: lse is NULL", who);
+    BIGC_CHECK_ARG(a.n_q == 0 || (a.stats && (uintptr_t)a.stats % 8 == 0), "%s: stats is NULL or not a multiple of 8 bytes", who);
     BIGC_CHECK_ARG(!a.d_rel_table || a.rel_table, "%s: d_rel_table without rel_table", who);
-    const Plan p = plan_of(a, 1);
+    const Plan p = plan_of(a);
     if (workspace_bytes < p.total || (p.total && (!workspace || (uintptr_t)workspace % 16)))
         return bigc_fail(BIGC_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.total);
     hipStream_t hs = (hipStream_t)stream;
@@ -323,6 +293,9 @@ extern "C" int bigc_seq_attn_bwd(void* stream, const bigc_seq_attn* ap, void* wo
     const long nk = (long)a.n_seq * a.max_k * a.n_kv_head;
     const size_t lds = a.d_rel_table ? sizeof(float) * (2 * a.bias_radius + 1) : 0;
 #define F(T) \
+    if (a.zero_rest && a.n_q) zero_rows<T><<<256, 256, 0, hs>>>((T*)a.dq, a.lddq, a.hsdq, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq); \
+    if (a.zero_rest && a.n_k) zero_rows<T><<<256, 256, 0, hs>>>((T*)a.dk, a.lddk, a.hsdk, a.n_k, a.n_kv_head, a.head_dim, a.k_off, a.n_seq); \
+    if (a.zero_rest && a.n_k) zero_rows<T><<<256, 256, 0, hs>>>((T*)a.dv, a.lddv, a.hsdv, a.n_k, a.n_kv_head, a.head_dim, a.k_off, a.n_seq); \
     if (a.n_q) rows_delta<T><<<(unsigned)(a.n_q * a.n_head), 64, 0, hs>>>(a, delta); \
     if ((a.n_q && a.n_seq) || a.d_rel_table) rows_dq<T><<<BIN_BLOCKS * a.n_head, 64, lds, hs>>>(a, delta, by_dist); \
     if (nk && a.n_k) rows_dkv<T><<<(unsigned)nk, 64, 0, hs>>>(a, delta);

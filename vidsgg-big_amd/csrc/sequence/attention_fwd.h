@@ -1,0 +1,392 @@
+// Forward of the attention over ordered rows.
+#pragma once
+#include "attention_tiles.h"
+
+namespace {
+
+// How a forward call is cut.  A tile's rows are (query, head) pairs of one key head: `pack` of a group's heads side by side, so that a key is read once
+// for all of them and a single token still fills rows.  many: four waves of 32 rows share every tile of keys; few (at most 32 rows in the
+// longest sequence): the four waves take the key tiles of the same 32 rows in turn, each through LDS of its own.
+struct FwdShape {
+    int pack, sub;                                              // heads a tile packs; packs of a group
+    int few, tiles, pairs;                                      // row tiles of the longest sequence; (sequence, key head, pack) triples
+    int chunk, splits;                                          // keys a block takes; chunks of the longest sequence
+    long blocks;
+    size_t lds, ranges, part_o, part_ml, total;                 // LDS; workspace: offsets of the parts and its size
+};
+
+template <typename T, int HD, bool FEW> struct FwdTile {
+    static constexpr int KEYS = FEW || sizeof(T) == 4 ? 32 : 64, SUBS = KEYS / 32;
+    static constexpr int WAVES = FEW && Geometry<T, HD>::ROW > 256 ? 2 : 4;         // (rows of 384 and 512 bytes: 160 KB of LDS hold the buffers of two)
+    static constexpr int TILE = KEYS * Geometry<T, HD>::ROW, BUF = 2 * TILE;        // bytes: one tile, K and V
+    static constexpr int STAGES = (FEW ? WAVES : 1) * 2 * BUF;                      // two buffers of a block (many) or of each wave (few)
+    static constexpr int DOCS = (FEW ? WAVES : 1) * 2 * 64 * 4;
+};
+
+// (pair, tile, chunk) of a block.  Blocks go to the eight XCDs in turn, each with an L2 of its own: all tiles of a pair, which read the same keys, are
+// put on one XCD; the pairs go round the XCDs when they are a multiple of eight, else every XCD gets one piece of the list.
+struct FwdPlace { int pair, tile, split; };
+__device__ __forceinline__ FwdPlace fwd_place(const FwdShape& sh, bool last_first) {
+    const int per = sh.tiles * sh.splits, xcd = blockIdx.x & 7, k = blockIdx.x >> 3;
+    long id;
+    if ((sh.pairs & 7) == 0) id = (long)(xcd + 8 * (k / per)) * per + k % per;
+    else {
+        const long q = sh.blocks >> 3, rest = sh.blocks & 7;
+        id = xcd * q + min((long)xcd, rest) + k;
+    }
+    const int pair = (int)(id / per), in = (int)(id % per), tile = in % sh.tiles;
+    return {pair, last_first ? sh.tiles - 1 - tile : tile, in / sh.tiles};
+}
+
+// rows of `t` outside [off[0], off[n_seq]) -> 0
+template <typename T>
+__device__ __forceinline__ void zero_outside(T* t, long ld, long hs, long n, int heads, int hd, const int* off, int n_seq) {
+    const long first = n_seq ? min(max((long)off[0], 0l), n) : 0, last = n_seq ? min(max((long)off[n_seq], first), n) : 0;
+    const int chunks = hd / (16 / (int)sizeof(T));
+    const long all = (first + n - last) * heads * chunks;
+    for (long e = (long)blockIdx.x * blockDim.x + threadIdx.x; e < all; e += (long)gridDim.x * blockDim.x) {
+        const long r = e / chunks / heads;
+        *(uint4*)(t + (r < first ? r : r - first + last) * ld + e / chunks % heads * hs + e % chunks * (16 / sizeof(T))) = make_uint4(0, 0, 0, 0);
+    }
+}
+
+// Least and greatest document of every 64 keys of a sequence; -1: padding among them
+__global__ __launch_bounds__(256) void doc_ranges(bigc_seq_attn a, int tiles, int2* ranges) {
+    const long w = (long)blockIdx.x * 4 + threadIdx.x / 64;
+    if (w >= (long)a.n_seq * tiles) return;
+    const SeqSpan sp = seq_span(a, (int)(w / tiles));
+    const int j = (int)(w % tiles) * 64 + (threadIdx.x & 63);
+    int lo = 0x7fffffff, hi = -1;
+    if (j < sp.nk) lo = hi = max(a.k_doc[sp.k0 + j], -1);
+    for (int m = 32; m; m >>= 1) { lo = min(lo, __shfl_xor(lo, m)); hi = max(hi, __shfl_xor(hi, m)); }
+    if ((threadIdx.x & 63) == 0) ranges[w] = make_int2(lo, hi);
+}
+
+// One pass over the keys with the running maximum m and sum l of every row:  o = sum 2^(s - m) v / l.
+//
+// A row's maximum is only moved when a score passes it by more than SLACK, so that the accumulators are rarely rescaled; p then lies in (0, 2^SLACK].
+// p is rounded to the tensors' type for its product with v (the one rounding inside; sums and statistics are f32 before it).  f16 ends at 2^-14, so that its p is
+// scaled by 2^LIFT (o32, which the exact gradient of the bias table is taken from, has p in two parts): with 2^(SLACK + LIFT) the largest, values down to 2^-39 of the row's largest still arrive.
+template <typename T> constexpr float SLACK = sizeof(T) == 4 ? 0.f : 8.f;
+template <> constexpr float SLACK<f16_t> = 4.f;
+template <typename T> constexpr float LIFT = 0.f;
+template <> constexpr float LIFT<f16_t> = 11.f;
+
+template <typename T, int HD, bool FEW>
+__global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW ? 1 : 2)) void attn_fwd(bigc_seq_attn a, FwdShape sh, const int2* ranges, float* part_o, float2* part_ml) {
+    typedef FwdTile<T, HD, FEW> F;
+    constexpr int DT = HD / 32, E = Geometry<T, HD>::E;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int shared_bad[4];
+    __shared__ int2 shared_docs[4];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
+    if (a.zero_rest) zero_outside((T*)a.o, a.ldo, a.hso, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq);
+
+    const FwdPlace at = fwd_place(sh, a.causal);
+    if (at.pair >= sh.pairs) return;
+    const int group = a.n_head / a.n_kv_head, s = at.pair / (a.n_kv_head * sh.sub), hk = at.pair / sh.sub % a.n_kv_head, head0 = hk * group + at.pair % sh.sub * sh.pack;
+    const SeqSpan sp = seq_span(a, s);
+    const int rows = sp.nq * sh.pack, first = at.tile * (FEW ? 32 : 128);
+    if (first >= rows || (at.split && at.split * sh.chunk >= sp.nk)) return;
+
+    // the wave's rows and the lane's
+    const int t0 = first + (FEW ? 0 : wave * 32), t = t0 + col;
+    const bool live = t < rows, wave_live = t0 < rows;
+    const int i = min(t, rows - 1) / sh.pack, head = head0 + min(t, rows - 1) % sh.pack, shift = sp.nk - sp.nq;
+    const long row = sp.q0 + i;
+    const ScoreRule rule(a);
+    const Reach reach(a);
+    const int prefix = a.prefix_len ? min(a.prefix_len[s], sp.nk) : 0;
+    const int pos = i + shift;
+    LaneRow me;
+    me.lo = reach.lo; me.hi = min(reach.hi, sp.nk - 1 - pos);   // keys behind the last are hidden by their distance
+    me.prefix = prefix - pos;
+    me.doc = 0;
+    me.slope2 = rule.slopes ? a.slopes[head] * LOG2E : 0.f;
+    me.bias = (head - head0) * (2 * rule.radius + 1);
+
+    char* docs_lds = lds + F::STAGES;
+    float* biases = (float*)(docs_lds + (a.q_doc ? F::DOCS : 0));
+    if (rule.table) load_biases(a, biases, head0, sh.pack);
+
+    // the wave's and the block's range of positions, and of documents
+    const int p_min = min(t0, rows - 1) / sh.pack + shift, p_max = min(t0 + 31, rows - 1) / sh.pack + shift;
+    const int b_min = first / sh.pack + shift, b_max = min(first + (FEW ? 31 : 127), rows - 1) / sh.pack + shift;
+    int doc_min = 0, doc_max = 0, block_doc_min = 0, block_doc_max = 0;
+    if (a.q_doc) {
+        me.doc = live ? a.q_doc[row] : -1;
+        int lo = live ? max(me.doc, -1) : 0x7fffffff, some = me.doc >= 0 ? me.doc : 0x7fffffff, most = me.doc;
+        for (int m = 32; m; m >>= 1) { lo = min(lo, __shfl_xor(lo, m)); some = min(some, __shfl_xor(some, m)); most = max(most, __shfl_xor(most, m)); }
+        doc_min = __builtin_amdgcn_readfirstlane(lo); doc_max = __builtin_amdgcn_readfirstlane(most);
+        if (lane == 0) shared_docs[wave] = make_int2(some, most);
+        __syncthreads();
+        block_doc_min = shared_docs[0].x; block_doc_max = shared_docs[0].y;
+        for (int w = 1; w < F::WAVES; ++w) { block_doc_min = min(block_doc_min, shared_docs[w].x); block_doc_max = max(block_doc_max, shared_docs[w].y); }
+    }
+    if (rule.table) __syncthreads();
+
+    // the block's key tiles: of its chunk those in the prefix or in reach of any of its rows
+    const int tile_begin = at.split * sh.chunk / F::KEYS, tile_end = min((sp.nk + F::KEYS - 1) / F::KEYS, (at.split + 1) * (sh.chunk / F::KEYS));
+    const int prefix_tiles = (prefix + F::KEYS - 1) / F::KEYS;
+    const long reach_lo = (long)b_min + reach.lo, reach_hi = (long)b_max + reach.hi;
+    const int reach_first = reach_lo <= 0 ? 0 : (int)min(reach_lo / F::KEYS, 0x7fffffl * 64), reach_last = reach_hi < 0 ? -1 : (int)min(reach_hi / F::KEYS, 0x7fffffl * 64);
+    const int stride = FEW ? F::WAVES : 1;
+    const int range_tiles = (a.max_k + 63) / 64;
+    const auto next_tile = [&](int k) {                          // the first of k, k + stride, ... with something to see, or tile_end
+        if (k >= prefix_tiles && k < reach_first) k += (reach_first - k + stride - 1) / stride * stride;
+        while (k < tile_end) {
+            const int c = k + lane * stride;
+            bool ok = c < tile_end && (c < prefix_tiles || (c >= reach_first && c <= reach_last));
+            if (ok && a.q_doc) {
+                const int2 r = ranges[(long)s * range_tiles + c * F::KEYS / 64];
+                ok = r.x <= block_doc_max && r.y >= block_doc_min;
+            }
+            const unsigned long long m = __ballot(ok);
+            if (m) return k + (int)__builtin_ctzll(m) * stride;
+            k += 64 * stride;
+        }
+        return tile_end;
+    };
+
+    typename Mat<T>::frag q[Geometry<T, HD>::STEPS];
+    load_lane_rows<T, HD>(q, (const T*)a.q + row * a.ldq + head * a.hsq, live, a.head_dim);
+    Stage<T, HD, F::KEYS, FEW ? 1 : F::WAVES> stage_k, stage_v;
+    stage_k.init((const T*)a.k + sp.k0 * a.ldk + hk * a.hsk, a.ldk, a.head_dim, FEW ? 0 : wave);
+    stage_v.init((const T*)a.v + sp.k0 * a.ldv + hk * a.hsv, a.ldv, a.head_dim, FEW ? 0 : wave);
+    char* const mine = lds + (FEW ? wave * 2 * F::BUF : 0);
+    int* const my_docs = (int*)(docs_lds) + (FEW ? wave * 128 : 0);
+    const int sw = FEW ? 0 : wave;
+    const auto copy_tile = [&](int k, int buf) {
+        stage_k.load(mine + buf * F::BUF, k * F::KEYS, sp.nk, sw);
+        stage_v.load(mine + buf * F::BUF + F::TILE, k * F::KEYS, sp.nk, sw);
+        if (a.q_doc && sw == 0)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.k_doc + sp.k0 + min(k * F::KEYS + lane, sp.nk - 1)),
+                                             LDS_PTR(void, my_docs + buf * 64), 4, 0, 0);
+    };
+    const auto arrived = [&] { if (FEW) wait_copies(); else wait_block(); };
+
+    f32x16 acc[DT];
+    float m = -INFINITY, l = 0.f;
+    for (int careful = 0; careful < 2; ++careful) {
+        for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+        m = -INFINITY; l = 0.f;
+        int k = __builtin_amdgcn_readfirstlane(next_tile(tile_begin + (FEW ? wave : 0))), buf = 0;
+        if (k < tile_end) copy_tile(k, 0);
+        arrived();
+        while (k < tile_end) {
+            const int after = __builtin_amdgcn_readfirstlane(next_tile(k + stride));
+            if (after < tile_end) copy_tile(after, buf ^ 1);
+            const char* const kt = mine + buf * F::BUF;
+            const char* const vt = kt + F::TILE;
+            if (careful) {                                       // products with the zeros behind head_dim stay zeros
+                stage_k.clear_tail((char*)kt, sw);
+                if (FEW) wait_copies(); else wait_block();
+            }
+            // what the wave sees of the tile: nothing, everything, or part
+            const int kb = k * F::KEYS, ke = min(kb + F::KEYS, sp.nk);
+            const int d_min = kb - p_max, d_max = kb + F::KEYS - 1 - p_min;
+            const bool seen = wave_live && (kb < prefix || (d_max >= reach.lo && d_min <= reach.hi));
+            bool full = kb + F::KEYS <= sp.nk && (ke <= prefix || (d_min >= reach.lo && d_max <= reach.hi));
+            if (a.q_doc && full) {
+                const int2 r = ranges[(long)s * range_tiles + kb / 64];
+                full = __builtin_amdgcn_readfirstlane(r.x >= 0 && r.x == r.y && doc_min == r.x && doc_max == r.x);
+            }
+            if (seen) {
+#pragma unroll 1
+                for (int u = 0; u < F::SUBS; ++u) {                 // 32 keys at a time
+                    f32x16 x;
+                    for (int e = 0; e < 16; ++e) x[e] = 0.f;
+                    for (int c = 0; c < Geometry<T, HD>::STEPS; ++c) x = Mat<T>::mul(rows_frag<T, HD>(kt, 32 * u, c), q[c], x);
+                    const int d0 = kb + 32 * u + 4 * hi - pos;
+                    make_scores<T, true, false>(x, nullptr, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (F::SUBS - 1 - u));
+                    if (!full) hide_scores<true>(x, me, d0, a.q_doc ? my_docs + buf * 64 + 32 * u + 4 * hi : nullptr);
+                    float top = x[0];
+                    for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const bool move = top > m + SLACK<T>;
+                    if (__ballot(move)) {
+                        const float c = move ? __builtin_amdgcn_exp2f(m - top) : 1.f;
+                        m = move ? top : m;
+                        l *= c;
+                        for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) acc[d][e] *= c;
+                    }
+                    const float base = (m == -INFINITY ? 0.f : m) - LIFT<T>;
+                    for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(x[e] - base);
+                    float sum = x[0];
+                    for (int e = 1; e < 16; ++e) sum += x[e];
+                    l += sum;
+                    if (careful) accumulate_seen<T, HD>(acc, vt, 32 * u, x);
+                    else Accumulate<T, HD>::add(acc, vt, 32 * u, x, a.o32 != nullptr);
+                }
+            }
+            arrived();
+            k = after; buf ^= 1;
+        }
+        // NaN or Inf in the result: it may come from a hidden place (0 times it is NaN), so that the rows are done again value by value
+        bool bad = false;
+        for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) bad |= !isfinite(acc[d][e]);
+        bad = __ballot(bad && live) != 0;
+        if (!FEW) {
+            if (lane == 0) shared_bad[wave] = bad;
+            wait_block();
+            bad = shared_bad[0] | shared_bad[1] | shared_bad[2] | shared_bad[3];
+            wait_block();
+        }
+        if (!bad) break;
+    }
+    l += __shfl_xor(l, 32);
+
+    if constexpr (FEW) {                                        // the waves' results of the same rows, joined in LDS: [wave][column][row], rows padded against bank conflicts
+        constexpr int PAD = 33;
+        __syncthreads();
+        float* const o_all = (float*)lds;
+        float* const ml_all = o_all + F::WAVES * HD * PAD;
+        static_assert(!FEW || ((F::WAVES * (HD * PAD + 2 * 32)) * 4 <= F::STAGES && F::STAGES <= 128 * 1024), "");
+        for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) o_all[(wave * HD + 32 * d + mfma_row(e, hi)) * PAD + col] = acc[d][e];
+        if (hi == 0) { ml_all[wave * 32 + col] = m; ml_all[(F::WAVES + wave) * 32 + col] = l; }
+        __syncthreads();
+        const int n = min(32, rows - first);
+        for (int e = threadIdx.x; e < n * a.head_dim; e += 64 * F::WAVES) {
+            const int r = e / a.head_dim, c = e % a.head_dim, rt = first + r;
+            float top = -INFINITY, sum = 0.f, o = 0.f;
+            for (int w = 0; w < F::WAVES; ++w) top = fmaxf(top, ml_all[w * 32 + r]);
+            const float base = top == -INFINITY ? 0.f : top;
+            for (int w = 0; w < F::WAVES; ++w) {
+                const float f = __builtin_amdgcn_exp2f(ml_all[w * 32 + r] - base);
+                if (f == 0.f && !isnan(ml_all[(F::WAVES + w) * 32 + r])) continue;
+                sum += f * ml_all[(F::WAVES + w) * 32 + r];
+                o += f * o_all[(w * HD + c) * PAD + r];
+            }
+            const long qrow = sp.q0 + rt / sh.pack;
+            const int h = head0 + rt % sh.pack;
+            const long rh = qrow * a.n_head + h;
+            if (sh.splits > 1) {
+                part_o[((long)at.split * a.n_q * a.n_head + rh) * a.head_dim + c] = o;
+                if (c == 0) part_ml[(long)at.split * a.n_q * a.n_head + rh] = make_float2(top, sum);
+            } else {
+                o *= sum == 0.f ? 0.f : 1.f / sum;
+                ((T*)a.o)[qrow * a.ldo + h * a.hso + c] = (T)o;
+                if (a.o32) a.o32[rh * a.head_dim + c] = o;
+                if (a.stats && c == 0) *(float2*)(a.stats + 2 * rh) = make_float2(top - LIFT<T>, sum);
+            }
+        }
+        return;
+    }
+    if (!live) return;
+    const long rh = row * a.n_head + head;
+    if (sh.splits > 1) {
+        float* o = part_o + ((long)at.split * a.n_q * a.n_head + rh) * a.head_dim;
+        for (int d = 0; d < DT; ++d)
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * d + 8 * g + 4 * hi;
+                if (c < a.head_dim) *(float4*)(o + c) = make_float4(acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]);
+            }
+        if (hi == 0) part_ml[(long)at.split * a.n_q * a.n_head + rh] = make_float2(m, l);
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int d = 0; d < DT; ++d)
+        for (int g = 0; g < 4; ++g) {
+            const int c = 32 * d + 8 * g + 4 * hi;
+            if (c >= a.head_dim) continue;
+            float y[4];
+            T z[4];
+            for (int e = 0; e < 4; ++e) { y[e] = acc[d][4 * g + e] * inv; z[e] = (T)y[e]; }
+            struct alignas(4 * sizeof(T)) Four { T v[4]; };
+            *(Four*)((T*)a.o + row * a.ldo + head * a.hso + c) = *(const Four*)z;
+            if (a.o32) *(float4*)(a.o32 + rh * a.head_dim + c) = make_float4(y[0], y[1], y[2], y[3]);
+        }
+    if (a.stats && hi == 0) *(float2*)(a.stats + 2 * rh) = make_float2(m - LIFT<T>, l);
+    (void)E;
+}
+
+// Joins the chunks of every (row, head): a wave each
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join(bigc_seq_attn a, FwdShape sh, const float* part_o, const float2* part_ml) {
+    const long w = (long)blockIdx.x * 4 + threadIdx.x / 64;
+    const int lane = threadIdx.x & 63, h = (int)(w % a.n_head);
+    const long r = w / a.n_head;
+    if (r >= (long)a.n_seq * a.max_q) return;
+    const int s = (int)(r / a.max_q), i = (int)(r % a.max_q);
+    const SeqSpan sp = seq_span(a, s);
+    if (i >= sp.nq) return;
+    const long row = sp.q0 + i, rh = row * a.n_head + h, stride = a.n_q * a.n_head;
+    const int n = max(1, (sp.nk + sh.chunk - 1) / sh.chunk);
+    float top = -INFINITY;
+    for (int k = 0; k < n; ++k) top = fmaxf(top, part_ml[k * stride + rh].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, o[2] = {0.f, 0.f};
+    for (int k = 0; k < n; ++k) {
+        const float2 ml = part_ml[k * stride + rh];
+        const float f = __builtin_amdgcn_exp2f(ml.x - base);
+        if (f == 0.f && !isnan(ml.y)) continue;
+        sum += f * ml.y;
+        for (int t = 0; t < 2; ++t)
+            if (lane + 64 * t < a.head_dim) o[t] += f * part_o[(k * stride + rh) * a.head_dim + lane + 64 * t];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int t = 0; t < 2; ++t) {
+        const int c = lane + 64 * t;
+        if (c >= a.head_dim) continue;
+        ((T*)a.o)[row * a.ldo + h * a.hso + c] = (T)(o[t] * inv);
+        if (a.o32) a.o32[rh * a.head_dim + c] = o[t] * inv;
+    }
+    if (a.stats && lane == 0) *(float2*)(a.stats + 2 * rh) = make_float2(top - LIFT<T>, sum);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void zero_rows(T* t, long ld, long hs, long n, int heads, int hd, const int* off, int n_seq) {
+    zero_outside(t, ld, hs, n, heads, hd, off, n_seq);
+}
+
+int tile_dim(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 96 ? 96 : 128; }
+size_t round_up(size_t n, size_t m) { return (n + m - 1) / m * m; }
+
+FwdShape fwd_shape(const bigc_seq_attn& a) {
+    FwdShape sh = {};
+    const int group = a.n_head / a.n_kv_head, nb = a.rel_table ? 2 * a.bias_radius + 1 : 0;
+    // heads packed in a tile: all of a group; with a bias by distance as many as have their biases in 4096 LDS entries (one head's may be 4095)
+    sh.pack = 1;
+    for (int p = 1; p <= group; ++p)
+        if (group % p == 0 && (long)p * nb <= 4096 && (long)p * a.max_q < (1l << 30)) sh.pack = p;
+    sh.sub = group / sh.pack;
+    sh.few = (long)a.max_q * sh.pack <= 32;
+    const int rows = sh.few ? 32 : 128, keys = sh.few || a.dtype == BIGC_F32 ? 32 : 64;
+    sh.tiles = (int)(((long)a.max_q * sh.pack + rows - 1) / rows);
+    sh.pairs = a.n_seq * a.n_kv_head * sh.sub;
+    // Keys a block takes.  While the row tiles alone do not give every CU its blocks (two; eight for few rows, where a block is a stream through memory and
+    // sequences differ in length), the keys are cut: to blocks of equal work over all sequences, none under 512 keys.
+    const long row_blocks = (long)sh.pairs * sh.tiles, want = sh.few ? 2048 : 512;
+    sh.chunk = (int)round_up(a.max_k > 0 ? a.max_k : 1, 64);
+    if (row_blocks && row_blocks < want) {
+        const long total = a.n_k < (long)a.n_seq * a.max_k ? a.n_k : (long)a.n_seq * a.max_k;        // keys of all sequences together, at most
+        long chunk = (total * (row_blocks / a.n_seq) + want - 1) / want;
+        chunk = chunk < 512 ? 512 : chunk;
+        if (chunk < sh.chunk) sh.chunk = (int)round_up(chunk, 4 * keys);
+    }
+    sh.splits = (int)((a.max_k + sh.chunk - 1) / sh.chunk);
+    if (sh.splits < 1) sh.splits = 1;
+    sh.blocks = row_blocks * sh.splits;
+    const int hd = tile_dim(a.head_dim), tile = keys * hd * seq_size(a.dtype);
+    sh.lds = (size_t)(!sh.few ? 1 : hd * seq_size(a.dtype) > 256 ? 2 : 4) * (4 * tile + (a.q_doc ? 512 : 0)) + sizeof(float) * sh.pack * nb;
+    sh.part_o = a.q_doc ? round_up(sizeof(int2) * (size_t)a.n_seq * ((a.max_k + 63) / 64), 256) : 0;
+    sh.part_ml = sh.part_o + (sh.splits > 1 ? round_up(sizeof(float) * (size_t)sh.splits * a.n_q * a.n_head * a.head_dim, 256) : 0);
+    sh.total = sh.part_ml + (sh.splits > 1 ? round_up(sizeof(float2) * (size_t)sh.splits * a.n_q * a.n_head, 256) : 0);
+    return sh;
+}
+
+template <typename T, int HD>
+void launch_fwd(hipStream_t s, const bigc_seq_attn& a, const FwdShape& sh, const int2* ranges, float* part_o, float2* part_ml) {
+    if (sh.few) attn_fwd<T, HD, true><<<(unsigned)sh.blocks, 64 * FwdTile<T, HD, true>::WAVES, sh.lds, s>>>(a, sh, ranges, part_o, part_ml);
+    else attn_fwd<T, HD, false><<<(unsigned)sh.blocks, 256, sh.lds, s>>>(a, sh, ranges, part_o, part_ml);
+}
+template <typename T>
+void launch_fwd_dim(hipStream_t s, const bigc_seq_attn& a, const FwdShape& sh, const int2* ranges, float* part_o, float2* part_ml) {
+    switch (tile_dim(a.head_dim)) {
+        case 32: launch_fwd<T, 32>(s, a, sh, ranges, part_o, part_ml); break;
+        case 64: launch_fwd<T, 64>(s, a, sh, ranges, part_o, part_ml); break;
+        case 96: launch_fwd<T, 96>(s, a, sh, ranges, part_o, part_ml); break;
+        default: launch_fwd<T, 128>(s, a, sh, ranges, part_o, part_ml); break;
+    }
+}
+}  // namespace

@@ -1,0 +1,290 @@
+// The parts that the attention kernels share: tiles of rows in LDS, matrix fragments, and the scores of a tile.
+//
+// Every kernel keeps one side of the attention in lanes (32 rows a wave, a row a lane and its twin 32 lanes on) and streams the other side through LDS:
+// the product of a streamed row-major tile (A operand, 32 rows) with the lanes' side (B operand) leaves element (streamed row, lane's row) in
+// register r of lane l at streamed row (r & 3) + 8 (r >> 2) + 4 (l >> 5).  That is already the B operand of the next product, whose A operand is the
+// streamed tile TRANSPOSED -- the order of a contraction is free, so the transposed tile is read in the register's order of rows and no value
+// changes lanes between the two products.
+#pragma once
+#include "sequence.h"
+#include <math.h>
+
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) bf16_t bf16x8;
+typedef __attribute__((ext_vector_type(8))) f16_t f16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+
+#define LDS_PTR(T, ...) ((__attribute__((address_space(3))) T*)(__VA_ARGS__))
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
+
+// Matrix instructions by type: f16 / bf16 contract 16 rows a step, f32 two.
+template <typename T> struct Mat;
+template <> struct Mat<bf16_t> {
+    typedef bf16x8 frag;
+    static __device__ __forceinline__ f32x16 mul(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<f16_t> {
+    typedef f16x8 frag;
+    static __device__ __forceinline__ f32x16 mul(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<float> {
+    typedef f32x4 frag;                                         // four steps of two: lane l's four values go with l's twin's four
+    static __device__ __forceinline__ f32x16 mul(frag a, frag b, f32x16 c) {
+        c = mfma32(a.x, b.x, c);
+        c = mfma32(a.y, b.y, c);
+        c = mfma32(a.z, b.z, c);
+        return mfma32(a.w, b.w, c);
+    }
+};
+
+// A tile of ROWS rows of HD columns in LDS, 16-byte chunks swizzled so that eight (sixteen) rows' chunks of one column, which a row-major fragment
+// reads together, and four rows' pairs of chunks, which a transposed one does, lie in different banks.
+template <typename T, int HD>
+struct Geometry {
+    static constexpr int E = 16 / (int)sizeof(T), CH = HD / E, ROW = HD * (int)sizeof(T), STEPS = CH / 2;      // chunks a row, bytes a row, fragments a row
+    static __device__ __forceinline__ int swizzle(int row) {
+        if (CH % 16 == 0) return ((row & 3) << 1) | (((row >> 2) & 1) << 3) | ((row >> 3) & 1);
+        if (CH % 8 == 0) return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
+        return (row >> 2) & 3;
+    }
+    static __device__ __forceinline__ int place(int row, int chunk) { return row * ROW + ((chunk ^ swizzle(row)) << 4); }
+};
+
+// A operand, row-major: rows row0 .. row0 + 31, columns of step `s`
+template <typename T, int HD>
+__device__ __forceinline__ typename Mat<T>::frag rows_frag(const char* tile, int row0, int s) {
+    const int l = threadIdx.x & 63;
+    return *LDS_PTR(const typename Mat<T>::frag, tile + Geometry<T, HD>::place(row0 + (l & 31), 2 * s + (l >> 5)));
+}
+
+// A operand, transposed: columns col0 .. col0 + 31, the 16 rows row0 + .. in the order in which a product's registers 8 u .. 8 u + 7 hold them (half types)
+template <typename T, int HD>
+__device__ __forceinline__ typename Mat<T>::frag cols_frag(const char* tile, int row0, int col0) {
+    const int l = threadIdx.x & 63, i = l & 15, hi = l >> 5;
+    const int chunk = (col0 >> 3) + ((l >> 4) & 1) * 2 + ((i >> 1) & 1), r = row0 + 4 * hi + (i >> 2);
+    union { s16x4 v[2]; typename Mat<T>::frag f; } u;
+    u.v[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, tile + Geometry<T, HD>::place(r, chunk) + (i & 1) * 8));
+    u.v[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, tile + Geometry<T, HD>::place(r + 8, chunk) + (i & 1) * 8));
+    return u.f;
+}
+
+// acc[d columns of a block of 32][lane's row] += sum over the 32 streamed rows from row0 of tile^T x values; `values` in a product's register order.
+// Half types round the values once; `twice`: what that leaves goes through a second product (2^-17 / 2^-22 of a value then remain).
+template <typename T, int HD>
+struct Accumulate;
+template <typename T, int HD>
+struct AccumulateHalf {
+    static __device__ __forceinline__ void add(f32x16* acc, const char* tile, int row0, const f32x16& v, bool twice = false) {
+        typename Mat<T>::frag b[2];
+        for (int e = 0; e < 8; ++e) { b[0][e] = (T)v[e]; b[1][e] = (T)v[8 + e]; }
+        for (int u = 0; u < 2; ++u)
+            for (int dt = 0; dt < HD / 32; ++dt) acc[dt] = Mat<T>::mul(cols_frag<T, HD>(tile, row0 + 16 * u, 32 * dt), b[u], acc[dt]);
+        if (!twice) return;
+        for (int u = 0; u < 2; ++u) {
+            typename Mat<T>::frag rest;
+            for (int e = 0; e < 8; ++e) rest[e] = (T)(v[8 * u + e] - (float)b[u][e]);
+            for (int dt = 0; dt < HD / 32; ++dt) acc[dt] = Mat<T>::mul(cols_frag<T, HD>(tile, row0 + 16 * u, 32 * dt), rest, acc[dt]);
+        }
+    }
+};
+template <int HD> struct Accumulate<bf16_t, HD> : AccumulateHalf<bf16_t, HD> {};
+template <int HD> struct Accumulate<f16_t, HD> : AccumulateHalf<f16_t, HD> {};
+template <int HD>
+struct Accumulate<float, HD> {
+    static __device__ __forceinline__ void add(f32x16* acc, const char* tile, int row0, const f32x16& v, bool = false) {
+        const int l = threadIdx.x & 63, hi = l >> 5, c = l & 31;
+        for (int r = 0; r < 16; ++r) {
+            const int row = row0 + mfma_row(r, hi);
+            for (int dt = 0; dt < HD / 32; ++dt)
+                acc[dt] = mfma32(*LDS_PTR(const float, tile + Geometry<float, HD>::place(row, dt * 8 + (c >> 2)) + (c & 3) * 4), v[r], acc[dt]);
+        }
+    }
+};
+
+// The same, one value at a time: a value of 0 takes no part, whatever its row of the tile holds.  For the calls whose tiles hold NaN or Inf in hidden places.
+template <typename T, int HD>
+__device__ __forceinline__ void accumulate_seen(f32x16* acc, const char* tile, int row0, const f32x16& v) {
+    const int l = threadIdx.x & 63, hi = l >> 5;
+#pragma unroll 1
+    for (int r = 0; r < 16; ++r) {
+        float mine = v[0];
+        for (int q = 1; q < 16; ++q) mine = r == q ? v[q] : mine;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+            const float p = __shfl(mine, (l & 31) + 32 * half);
+            const int row = row0 + mfma_row(r, half);
+            for (int dt = 0; dt < HD / 32; ++dt)
+                for (int e = 0; e < 16; ++e) {
+                    const int col = 32 * dt + mfma_row(e, hi);
+                    const float x = (float)*LDS_PTR(const T, tile + Geometry<T, HD>::place(row, col / Geometry<T, HD>::E) + col % Geometry<T, HD>::E * (int)sizeof(T));
+                    acc[dt][e] += p != 0.f ? p * x : 0.f;
+                }
+        }
+    }
+}
+
+// B operand: the lane's row, all steps, from memory (zeros behind head_dim and for rows that are not there)
+template <typename T, int HD>
+__device__ __forceinline__ void load_lane_rows(typename Mat<T>::frag* f, const T* row, bool live, int hd) {
+    const int hi = (threadIdx.x & 63) >> 5;
+    for (int s = 0; s < Geometry<T, HD>::STEPS; ++s) {
+        const int c = (2 * s + hi) * Geometry<T, HD>::E;
+        union { i32x4 raw; typename Mat<T>::frag f; } u;
+        u.raw = live && c < hd ? *(const i32x4*)(row + c) : i32x4{0, 0, 0, 0};
+        f[s] = u.f;
+    }
+}
+
+// Copies tiles of ROWS rows into LDS straight from memory, 16 bytes a lane; NW waves share the work.  A lane's offset from the tile's first row is the
+// same for every tile that is whole.  Behind head_dim the columns repeat the row's first chunk (their products are with zeros, or not stored).
+template <typename T, int HD, int ROWS, int NW>
+struct Stage {
+    typedef Geometry<T, HD> G;
+    static constexpr int N = ROWS * G::CH / 64 / NW;
+    static_assert(ROWS * G::CH % (64 * NW) == 0, "");
+    unsigned off[N];
+    const char* base;
+    long step;                                                  // bytes from row to row
+    int hd;
+
+    __device__ __forceinline__ int row_of(int i, int wave) const { return ((i * NW + wave) * 64 + (int)(threadIdx.x & 63)) / G::CH; }
+    __device__ __forceinline__ int chunk_of(int i, int wave) const {
+        const int c = (((i * NW + wave) * 64 + (int)(threadIdx.x & 63)) % G::CH) ^ G::swizzle(row_of(i, wave));
+        return c * G::E < hd ? c : 0;
+    }
+    __device__ __forceinline__ void init(const T* first_row, long ld, int head_dim, int wave) {
+        base = (const char*)first_row;
+        step = ld * (long)sizeof(T);
+        hd = head_dim;
+        for (int i = 0; i < N; ++i) off[i] = (unsigned)(row_of(i, wave) * step) + chunk_of(i, wave) * 16;
+    }
+    // rows row0 .. row0 + ROWS - 1 of n: those behind the last repeat it (n > 0)
+    __device__ __forceinline__ void load(char* tile, int row0, int n, int wave) const {
+        const char* from = base + row0 * step;
+        if (row0 + ROWS <= n) {
+            for (int i = 0; i < N; ++i)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + off[i]), LDS_PTR(void, tile + (i * NW + wave) * 1024), 16, 0, 0);
+        } else {
+            for (int i = 0; i < N; ++i) {
+                const int r = min(row_of(i, wave), n - 1 - row0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + r * step + chunk_of(i, wave) * 16),
+                                                 LDS_PTR(void, tile + (i * NW + wave) * 1024), 16, 0, 0);
+            }
+        }
+    }
+    // zeros behind head_dim (for tiles that may hold Inf, which a product with 0 would make NaN)
+    __device__ __forceinline__ void clear_tail(char* tile, int wave) const {
+        for (int i = 0; i < N; ++i) {
+            const int at = ((i * NW + wave) * 64 + (int)(threadIdx.x & 63)) % G::CH ^ G::swizzle(row_of(i, wave));
+            if (at * G::E >= hd) *LDS_PTR(i32x4, tile + ((i * NW + wave) * 64 + (threadIdx.x & 63)) * 16) = i32x4{0, 0, 0, 0};
+        }
+    }
+};
+
+// own copies have arrived / and everybody's, and nobody reads the buffer any more that the next copies go to
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void wait_block() {
+    wait_copies();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// ---- scores -----------------------------------------------------------------------------------------------------------------------------
+
+// What every score of a call has in common; scores are kept times log2 e (exp is then one instruction)
+struct ScoreRule {
+    float scale2, cap2, cap_in;                                 // scale log2 e; cap log2 e; 2 scale log2 e / cap (the argument of tanh, for 2^x)
+    float cap_y;                                                // scale / cap
+    bool cap, slopes, table;
+    int radius;
+    __device__ __forceinline__ ScoreRule(const bigc_seq_attn& a)
+        : scale2(a.scale * LOG2E), cap2(a.softcap * LOG2E), cap_in(a.softcap > 0.f ? 2.f * a.scale / a.softcap * LOG2E : 0.f), cap_y(a.softcap > 0.f ? a.scale / a.softcap : 0.f),
+          cap(a.softcap > 0.f), slopes(a.slopes != nullptr), table(a.rel_table != nullptr), radius(a.bias_radius) {}
+};
+
+// tanh(y) = 1 - 2 / (e^2y + 1).  Its error is a step of 1, not of the value: half types, whose operands are rounded more coarsely, live with that; f32 takes
+// small arguments through the odd series (to y^13: 2^-26 of the value at 0.5) and divides in full.
+template <typename T>
+__device__ __forceinline__ float soft_tanh(float x, const ScoreRule& r) {
+    const float e = __builtin_amdgcn_exp2f(x * r.cap_in) + 1.f;
+    if (sizeof(T) < 4) return 1.f - 2.f * __builtin_amdgcn_rcpf(e);
+    const float y = x * r.cap_y, z = y * y;
+    const float p = 1.f + z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315 + z * (62.f / 2835 + z * (-1382.f / 155925 + z * (21844.f / 6081075))))));
+    return fabsf(y) < 0.5f ? y * p : 1.f - 2.f / e;
+}
+
+// What a call lets a row see, by d = key - position of the query: [lo, hi] (wide enough for any two int32 places), and a prefix
+struct Reach {
+    int lo, hi;
+    __device__ __forceinline__ Reach(const bigc_seq_attn& a) {
+        lo = a.window_left < 0 ? -0x7fffffff : -a.window_left;
+        hi = a.causal ? 0 : a.window_right < 0 ? 0x7fffffff : a.window_right;
+        if (a.causal && a.window_right >= 0) hi = 0;
+    }
+};
+
+// A lane's row.  LANE_IS_QUERY: the key at distance d is seen when lo <= d <= hi or d < prefix; else (the lane is a key) when lo <= d <= hi.
+struct LaneRow {
+    int lo, hi, prefix, doc;
+    float slope2;                                               // slope log2 e
+    int bias;                                                   // first entry of its head's biases by distance
+};
+
+// bias by distance of `heads` heads from h0 on, times log2 e: the lowest finite value stays finite (it hides nothing), -inf stays -inf
+__device__ __forceinline__ void load_biases(const bigc_seq_attn& a, float* biases, int h0, int heads) {
+    const int nb = 2 * a.bias_radius + 1;
+    for (int e = threadIdx.x; e < heads * nb; e += blockDim.x) {
+        const float b = a.rel_table[(long)min(max(a.rel_map[e % nb], 0), a.n_bucket - 1) * a.n_head + h0 + e / nb];
+        const float s = b * LOG2E;
+        biases[e] = isinf(s) && !isinf(b) ? copysignf(3.402823466e38f, b) : s;
+    }
+}
+
+// place of register e's streamed row among the lane's half of 32, without the 4 (l >> 5)
+__device__ __forceinline__ constexpr int reg_row(int e) { return (e & 3) + 8 * (e >> 2); }
+
+// Products of 32 streamed rows with the lanes' rows -> scores, capped and biased.  d0: d of register 0; streamed keys count d up, streamed queries
+// down.  d_min, d_max: the least and the greatest d of the 32 x 32 (where all are beyond the radius one bias serves).  t: the tanh, for the backward.
+template <typename T, bool LANE_IS_QUERY, bool KEEP>
+__device__ __forceinline__ void make_scores(f32x16& x, f32x16* t, const ScoreRule& r, const LaneRow& l, const float* biases, int d0, int d_min, int d_max) {
+    if (r.cap) {
+        for (int e = 0; e < 16; ++e) {
+            const float y = soft_tanh<T>(x[e], r);
+            if (KEEP) (*t)[e] = y;
+            x[e] = r.cap2 * y;
+        }
+    } else {
+        for (int e = 0; e < 16; ++e) x[e] *= r.scale2;
+    }
+    if (r.slopes) {
+        for (int e = 0; e < 16; ++e) x[e] -= l.slope2 * fabsf((float)(LANE_IS_QUERY ? d0 + reg_row(e) : d0 - reg_row(e)));
+    }
+    if (r.table) {
+        const float* b = biases + l.bias + r.radius;
+        if (d_min >= r.radius || d_max <= -r.radius) {
+            const float v = *LDS_PTR(const float, b + (d_min >= r.radius ? r.radius : -r.radius));
+            for (int e = 0; e < 16; ++e) x[e] += v;
+        } else {
+            for (int e = 0; e < 16; ++e) x[e] += *LDS_PTR(const float, b + min(max(LANE_IS_QUERY ? d0 + reg_row(e) : d0 - reg_row(e), -r.radius), r.radius));
+        }
+    }
+}
+
+// hidden scores -> -inf; docs: the streamed rows' documents from register 0's row on, or null
+template <bool LANE_IS_QUERY>
+__device__ __forceinline__ void hide_scores(f32x16& x, const LaneRow& l, int d0, const int* docs) {
+    for (int g = 0; g < 4; ++g) {
+        i32x4 doc = {l.doc, l.doc, l.doc, l.doc};
+        if (docs) doc = *LDS_PTR(const i32x4, docs + 8 * g);
+        for (int e = 0; e < 4; ++e) {
+            const int d = LANE_IS_QUERY ? d0 + reg_row(4 * g + e) : d0 - reg_row(4 * g + e);
+                        const bool near = (d >= l.lo && d <= l.hi) || (LANE_IS_QUERY && d < l.prefix);
+            if (!near || doc[e] != l.doc || l.doc < 0) x[4 * g + e] = -INFINITY;
+        }
+    }
+}
+}  // namespace
