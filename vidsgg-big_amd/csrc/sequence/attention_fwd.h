@@ -50,14 +50,14 @@ __device__ __forceinline__ void zero_outside(T* t, long ld, long hs, long n, int
     }
 }
 
-// Least and greatest document of every 64 keys of a sequence; -1: padding among them
-__global__ __launch_bounds__(256) void doc_ranges(bigc_seq_attn a, int tiles, int2* ranges) {
+// Least and greatest document of every 64 keys (or queries) of a sequence; -1: padding among them
+__global__ __launch_bounds__(256) void doc_ranges(bigc_seq_attn a, bool keys, int tiles, int2* ranges) {
     const long w = (long)blockIdx.x * 4 + threadIdx.x / 64;
     if (w >= (long)a.n_seq * tiles) return;
     const SeqSpan sp = seq_span(a, (int)(w / tiles));
     const int j = (int)(w % tiles) * 64 + (threadIdx.x & 63);
     int lo = 0x7fffffff, hi = -1;
-    if (j < sp.nk) lo = hi = max(a.k_doc[sp.k0 + j], -1);
+    if (j < (keys ? sp.nk : sp.nq)) lo = hi = max(keys ? a.k_doc[sp.k0 + j] : a.q_doc[sp.q0 + j], -1);
     for (int m = 32; m; m >>= 1) { lo = min(lo, __shfl_xor(lo, m)); hi = max(hi, __shfl_xor(hi, m)); }
     if ((threadIdx.x & 63) == 0) ranges[w] = make_int2(lo, hi);
 }
