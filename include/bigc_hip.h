@@ -728,8 +728,8 @@ typedef struct {
     void* o; int64_t ldo, hso;         /* bigc_seq_attn_bwd reads it */
     float* stats;                      /* (n_q, n_head, 2): m and l of every row's softmax, P = 2^(score log2 e - m) / l (the log of the sum of exp is
                                         * m ln 2 + ln l; l = 0: nothing seen); optional in the forward, read by the backward */
-    float* o32;                        /* (n_q, n_head, head_dim) o before its rounding, and for f16 / bf16 from probabilities of twice the bits; optional; read by
-                                        * the backward instead of o where given: sums of many dS, as rel_table's gradient, keep more bits than the tensors' type has */
+    float* o32;                        /* (n_q, n_head, head_dim) o before its rounding, and for f16 / bf16 from probabilities of two to three times the bits; optional;
+                                        * read by the backward instead of o where given: P (dP - delta), delta = d_o . o, then is as exact as dP (training should) */
     /* backward only */
     const void* d_o; int64_t lddo, hsdo;
     void* dq; int64_t lddq, hsdq;

@@ -25,8 +25,8 @@ def attention(q, k, v, q_off, k_off, scale=None, softcap=0.0, slopes=None, rel_t
 
     The bound: u = 2^-24.  A score is off by at most c = (hd + 16) u (1 + max sum |q_c k_c| scale + max |bias|) (a sum of hd products, the cap and
     the biases added in f32), P by 2 c + (L + 16) u of itself (numerator and denominator), so o by (that + half_eps / 2) sum P |v| and its own
-    rounding; dP - delta by (hd + 16) u sum |dO| (|v| + |o|), and by sum |dO| times the error of the o that delta = dO . o is taken from: the stored o's
-    bound (half types), or, with a rel_table, that of an o of P in two parts (half_eps^2); dS by P times that plus its own relative error; the gradients sum those.
+    rounding; dP - delta by (hd + 16) u sum |dO| (|v| + |o|), and by sum |dO| times the error of the o that delta = dO . o is taken from, which for
+    half types is one of P in two parts (half_eps^2 instead of half_eps); dS by P times that plus its own relative error; the gradients sum those.
 
     Below the normal range a rounding step is no longer relative: a P under 2^-126 (f32's and bfloat16's smallest normal number) may be taken as 0,
     which is an absolute error of 2^-126, as large as such a P itself.  f16 reaches down to 2^-14 in steps of 2^-24 below it, so that a kernel that
@@ -96,7 +96,7 @@ def attention(q, k, v, q_off, k_off, scale=None, softcap=0.0, slopes=None, rel_t
             dP = G @ V.detach().t()
             dS = (Pa * (dP - (G * O.detach()).sum(1, keepdim=True))).abs()
             reach = Ga @ Va.t() + (Ga * (Pa @ Va)).sum(1, keepdim=True)
-            o_err = (p_err + r * half_eps + 2 * u) * (Pa @ Va) if T is not None or not half_eps else out["tol_o"][a:b, h]
+            o_err = (p_err + r * half_eps + 2 * u) * (Pa @ Va)
             eS = Pa * (Ga * o_err).sum(1, keepdim=True) + Pa * reach * ((hd + 16) * u * 2 + p_err) + dS * 4 * u + near * (low * reach + low_s * dS.max())
             n = (b - a + f - e + 16) * u
             sc = abs(scale) * (1 + 2 * c)

@@ -257,10 +257,11 @@ def test_strides(t):
     c = Case(t, [(50, 80), (3, 3)], heads=(4, 2), hd=40, pad_cols=8, causal=True)
     c.check()
     (q, k, v, go), kw = c.args(DEV)
-    base = c.run(train=False)["o"]
+    off = (c.q_off.to(DEV), c.k_off.to(DEV), c.max_q, c.max_k)
+    base = sequence.attend(q, k, v, *off, **kw)
     by_head = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
     out = torch.zeros(4, q.shape[0], 40, dtype=c.t, device=DEV).transpose(0, 1)
-    sequence.attend(*by_head, c.q_off.to(DEV), c.k_off.to(DEV), c.max_q, c.max_k, out=out, **kw)
+    sequence.attend(*by_head, *off, out=out, **kw)
     assert torch.equal(out, base)
 
 

@@ -73,8 +73,8 @@ def _stream(device):
 
 
 class SavedAttention(object):
-    """What ``attend(..., save=True)`` keeps for ``attend_bwd``: the arguments, the output (with more bits too, where an f16 / bf16 call has a
-    rel_table) and the rows' softmax statistics.  The tensors must not change in between."""
+    """What ``attend(..., save=True)`` keeps for ``attend_bwd``: the arguments, the output (with more bits too, for f16 / bf16)
+    and the rows' softmax statistics.  The tensors must not change in between."""
 
     def __init__(self, args, tensors, o, stats, o32):
         self.args, self.tensors, self.o, self.stats, self.o32 = args, tensors, o, stats, o32
@@ -117,7 +117,7 @@ def attend(q, k, v, q_off, k_off, max_q, max_k, scale=None, softcap=0.0, slopes=
     stats = o32 = None
     if save:
         stats = q.new_empty((n_q, n_head, 2), dtype=f32)
-        if dtype is not f32 and rel_table is not None:                   # its gradient is f32: see o32 in bigc_hip.h
+        if dtype is not f32:                                             # see o32 in bigc_hip.h
             o32 = q.new_empty(shape, dtype=f32)
     a = bigc_seq_attn(                                                   # the fields in the structure's order
         _DTYPES[dtype], n_seq, n_head, kshape[1], hd, max_q, max_k, 1 if causal else 0, window[0], window[1], 1 if out is None else 0, radius, n_bucket,

@@ -165,6 +165,8 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW ? 1 : 2)) v
     };
     const auto arrived = [&] { if (FEW) wait_copies(); else wait_block(); };
 
+    // o32, which the backward takes delta from, has p in as many parts as its use needs: two, or for the f32 gradient of a bias table what adds up to f32's bits
+    const int parts = !a.o32 ? 1 : rule.table && sizeof(T) == 2 && LIFT<T> == 0.f ? 3 : 2;
     f32x16 acc[DT];
     float m = -INFINITY, l = 0.f;
     for (int careful = 0; careful < 2; ++careful) {
@@ -216,7 +218,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW ? 1 : 2)) v
                     for (int e = 1; e < 16; ++e) sum += x[e];
                     l += sum;
                     if (careful) accumulate_seen<T, HD>(acc, vt, 32 * u, x);
-                    else Accumulate<T, HD>::add(acc, vt, 32 * u, x, a.o32 != nullptr);
+                    else Accumulate<T, HD>::add(acc, vt, 32 * u, x, parts);
                 }
             }
             arrived();

@@ -73,21 +73,24 @@ __device__ __forceinline__ typename Mat<T>::frag cols_frag(const char* tile, int
 }
 
 // acc[d columns of a block of 32][lane's row] += sum over the 32 streamed rows from row0 of tile^T x values; `values` in a product's register order.
-// Half types round the values once; `twice`: what that leaves goes through a second product (2^-17 / 2^-22 of a value then remain).
+// Half types round the values; what that leaves goes through further products (of k parts 2^-8k (bf16) or 2^-11k (f16) of a value remain).
 template <typename T, int HD>
 struct Accumulate;
 template <typename T, int HD>
 struct AccumulateHalf {
-    static __device__ __forceinline__ void add(f32x16* acc, const char* tile, int row0, const f32x16& v, bool twice = false) {
+    static __device__ __forceinline__ void add(f32x16* acc, const char* tile, int row0, const f32x16& v, int parts = 1) {
         typename Mat<T>::frag b[2];
         for (int e = 0; e < 8; ++e) { b[0][e] = (T)v[e]; b[1][e] = (T)v[8 + e]; }
         for (int u = 0; u < 2; ++u)
             for (int dt = 0; dt < HD / 32; ++dt) acc[dt] = Mat<T>::mul(cols_frag<T, HD>(tile, row0 + 16 * u, 32 * dt), b[u], acc[dt]);
-        if (!twice) return;
-        for (int u = 0; u < 2; ++u) {
-            typename Mat<T>::frag rest;
-            for (int e = 0; e < 8; ++e) rest[e] = (T)(v[8 * u + e] - (float)b[u][e]);
-            for (int dt = 0; dt < HD / 32; ++dt) acc[dt] = Mat<T>::mul(cols_frag<T, HD>(tile, row0 + 16 * u, 32 * dt), rest, acc[dt]);
+        if (parts == 1) return;
+        f32x16 rest = v;
+#pragma unroll 1
+        for (int k = 1; k < parts; ++k) {
+            for (int u = 0; u < 2; ++u)
+                for (int e = 0; e < 8; ++e) { rest[8 * u + e] -= (float)b[u][e]; b[u][e] = (T)rest[8 * u + e]; }
+            for (int u = 0; u < 2; ++u)
+                for (int dt = 0; dt < HD / 32; ++dt) acc[dt] = Mat<T>::mul(cols_frag<T, HD>(tile, row0 + 16 * u, 32 * dt), b[u], acc[dt]);
         }
     }
 };
@@ -95,7 +98,7 @@ template <int HD> struct Accumulate<bf16_t, HD> : AccumulateHalf<bf16_t, HD> {};
 template <int HD> struct Accumulate<f16_t, HD> : AccumulateHalf<f16_t, HD> {};
 template <int HD>
 struct Accumulate<float, HD> {
-    static __device__ __forceinline__ void add(f32x16* acc, const char* tile, int row0, const f32x16& v, bool = false) {
+    static __device__ __forceinline__ void add(f32x16* acc, const char* tile, int row0, const f32x16& v, int = 1) {
         const int l = threadIdx.x & 63, hi = l >> 5, c = l & 31;
         for (int r = 0; r < 16; ++r) {
             const int row = row0 + mfma_row(r, hi);
