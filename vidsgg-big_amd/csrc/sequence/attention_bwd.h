@@ -73,6 +73,16 @@ __device__ __forceinline__ void doc_bounds(int doc, bool live, int wave, int2* s
     for (int w = 1; w < 4; ++w) { block_min = min(block_min, shared[w].x); block_max = max(block_max, shared[w].y); }
 }
 
+// whether a lane of any of the block's four waves has `x`
+__device__ __forceinline__ bool any_wave(bool x, int wave, int* shared) {
+    x = __ballot(x) != 0;
+    if ((threadIdx.x & 63) == 0) shared[wave] = x;
+    wait_block();
+    x = shared[0] | shared[1] | shared[2] | shared[3];
+    wait_block();
+    return x;
+}
+
 // a block's streamed tiles: those before `ahead`, or in [first, last], and of a document the block has
 struct TileList {
     int end, ahead, first, last;
@@ -116,7 +126,7 @@ __device__ __forceinline__ void add_diagonals(const f32x16& v, float* bins, int 
 }
 
 template <typename T, int HD>
-__global__ __launch_bounds__(256, 2) void attn_bwd_q(bigc_seq_attn a, BwdShape sh, float* row_data, const int2* ranges, float* by_dist) {
+__global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 2)) void attn_bwd_q(bigc_seq_attn a, BwdShape sh, float* row_data, const int2* ranges, float* by_dist) {
     constexpr int DT = HD / 32, KEYS = BwdTile<T, HD>::KEYS, SUBS = KEYS / 32, TILE = KEYS * Geometry<T, HD>::ROW, BUF = 2 * TILE;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int2 shared_docs[4];
@@ -208,7 +218,8 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q(bigc_seq_attn a, BwdShape s
     f32x16 acc[DT];
     GradScale<T> scale;
     float below = 0.f, above = 0.f;                             // dS of distances at or beyond the radius, of 32 x 32s that lie there whole
-    for (int careful = 0; careful < 2; ++careful) {
+    const auto pass = [&](auto careful_) {
+        constexpr bool careful = decltype(careful_)::value;
         for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
         scale = GradScale<T>();
         below = above = 0.f;
@@ -221,7 +232,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q(bigc_seq_attn a, BwdShape s
             if (after < list.end) copy_tile(after, buf ^ 1);
             const char* const kt = lds + buf * BUF;
             const char* const vt = kt + TILE;
-            if (careful) {
+            if constexpr (careful) {
                 stage_k.clear_tail((char*)kt, wave);
                 stage_v.clear_tail((char*)vt, wave);
                 wait_block();
@@ -260,22 +271,18 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q(bigc_seq_attn a, BwdShape s
                     }
                     if (rule.cap) for (int e = 0; e < 16; ++e) x[e] *= 1.f - t[e] * t[e];
                     scale.fit(x, acc, DT);
-                    if (careful) accumulate_seen<T, HD>(acc, kt, 32 * u, x);
+                    if constexpr (careful) accumulate_seen<T, HD>(acc, kt, 32 * u, x);
                     else Accumulate<T, HD>::add(acc, kt, 32 * u, x);
                 }
             }
             wait_block();
             k = after; buf ^= 1;
         }
-        bool bad = false;
-        for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) bad |= !isfinite(acc[d][e]);
-        bad = __ballot(bad && live) != 0;
-        if (lane == 0) shared_bad[wave] = bad;
-        wait_block();
-        bad = shared_bad[0] | shared_bad[1] | shared_bad[2] | shared_bad[3];
-        wait_block();
-        if (!bad) break;
-    }
+    };
+    pass(std::false_type());
+    float check = 0.f;                                          // NaN or Inf: again, value by value (see attn_fwd)
+    for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) check += acc[d][e] * 0.f;
+    if (any_wave(check != 0.f && live, wave, shared_bad)) pass(std::true_type());
     if (nb) {
         for (int w = 32; w; w >>= 1) { below += __shfl_xor(below, w); above += __shfl_xor(above, w); }
         if (lane == 0) { bins[0] += below; bins[nbins - 1] += above; }
@@ -357,7 +364,8 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
 
     f32x16 dk[DT], dv[DT];
     GradScale<T> scale;
-    for (int careful = 0; careful < 2; ++careful) {
+    const auto pass = [&](auto careful_) {
+        constexpr bool careful = decltype(careful_)::value;
         for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
         scale = GradScale<T>();
 #pragma unroll 1
@@ -384,7 +392,7 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                 if (after < list.end) copy_tile(after, buf ^ 1);
                 const char* const qt = lds + buf * BUF;
                 const char* const ot = qt + TILE;
-                if (careful) {
+                if constexpr (careful) {
                     stage_q.clear_tail((char*)qt, wave);
                     stage_o.clear_tail((char*)ot, wave);
                     wait_block();
@@ -414,7 +422,7 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                                 x[4 * g + e] = careful && p == 0.f ? 0.f : p * l4[e];
                             }
                         }
-                        if (careful) accumulate_seen<T, HD>(dv, ot, 32 * u, x);
+                        if constexpr (careful) accumulate_seen<T, HD>(dv, ot, 32 * u, x);
                         else Accumulate<T, HD>::add(dv, ot, 32 * u, x);
                         for (int g = 0; g < 4; ++g) {
                             const f32x4 d4 = *LDS_PTR(const f32x4, rows + 128 + 8 * g);
@@ -425,7 +433,7 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                         }
                         if (rule.cap) for (int e = 0; e < 16; ++e) x[e] *= 1.f - t[e] * t[e];
                         scale.fit(x, dk, DT);
-                        if (careful) accumulate_seen<T, HD>(dk, qt, 32 * u, x);
+                        if constexpr (careful) accumulate_seen<T, HD>(dk, qt, 32 * u, x);
                         else Accumulate<T, HD>::add(dk, qt, 32 * u, x);
                     }
                 }
@@ -433,15 +441,11 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                 k = after; buf ^= 1;
             }
         }
-        bool bad = false;
-        for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) bad |= !isfinite(dk[d][e]) || !isfinite(dv[d][e]);
-        bad = __ballot(bad && live) != 0;
-        if (lane == 0) shared_bad[wave] = bad;
-        wait_block();
-        bad = shared_bad[0] | shared_bad[1] | shared_bad[2] | shared_bad[3];
-        wait_block();
-        if (!bad) break;
-    }
+    };
+    pass(std::false_type());
+    float check = 0.f;
+    for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) check += (dk[d][e] + dv[d][e]) * 0.f;
+    if (any_wave(check != 0.f && live, wave, shared_bad)) pass(std::true_type());
     if (!live) return;
     const float unlift = P_LIFT<T> == 0.f ? 1.f : 1.f / 16384.f, f = a.scale * scale.back() * unlift;
     static_assert(P_LIFT<f16_t> == 14.f, "");

@@ -1,6 +1,7 @@
 // Forward of the attention over ordered rows.
 #pragma once
 #include "attention_tiles.h"
+#include <type_traits>
 
 namespace {
 
@@ -72,8 +73,9 @@ template <> constexpr float SLACK<f16_t> = 4.f;
 template <typename T> constexpr float LIFT = 0.f;
 template <> constexpr float LIFT<f16_t> = 11.f;
 
-template <typename T, int HD, bool FEW>
-__global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW ? 1 : 2)) void attn_fwd(bigc_seq_attn a, FwdShape sh, const int2* ranges, float* part_o, float2* part_ml) {
+// PARTS: of p (see o32).
+template <typename T, int HD, bool FEW, int PARTS>
+__global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(T) == 4 && HD > 96) ? 1 : 2)) void attn_fwd(bigc_seq_attn a, FwdShape sh, const int2* ranges, float* part_o, float2* part_ml) {
     typedef FwdTile<T, HD, FEW> F;
     constexpr int DT = HD / 32, E = Geometry<T, HD>::E;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -165,11 +167,10 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW ? 1 : 2)) v
     };
     const auto arrived = [&] { if (FEW) wait_copies(); else wait_block(); };
 
-    // o32, which the backward takes delta from, has p in as many parts as its use needs: two, or for the f32 gradient of a bias table what adds up to f32's bits
-    const int parts = !a.o32 ? 1 : rule.table && sizeof(T) == 2 && LIFT<T> == 0.f ? 3 : 2;
     f32x16 acc[DT];
     float m = -INFINITY, l = 0.f;
-    for (int careful = 0; careful < 2; ++careful) {
+    const auto pass = [&](auto careful_) {
+        constexpr bool careful = decltype(careful_)::value;
         for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
         m = -INFINITY; l = 0.f;
         int k = __builtin_amdgcn_readfirstlane(next_tile(tile_begin + (FEW ? wave : 0))), buf = 0;
@@ -180,7 +181,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW ? 1 : 2)) v
             if (after < tile_end) copy_tile(after, buf ^ 1);
             const char* const kt = mine + buf * F::BUF;
             const char* const vt = kt + F::TILE;
-            if (careful) {                                       // products with the zeros behind head_dim stay zeros
+            if constexpr (careful) {                             // products with the zeros behind head_dim stay zeros
                 stage_k.clear_tail((char*)kt, sw);
                 if (FEW) wait_copies(); else wait_block();
             }
@@ -217,25 +218,26 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW ? 1 : 2)) v
                     float sum = x[0];
                     for (int e = 1; e < 16; ++e) sum += x[e];
                     l += sum;
-                    if (careful) accumulate_seen<T, HD>(acc, vt, 32 * u, x);
-                    else Accumulate<T, HD>::add(acc, vt, 32 * u, x, parts);
+                    if constexpr (careful) accumulate_seen<T, HD>(acc, vt, 32 * u, x);
+                    else Accumulate<T, HD>::add(acc, vt, 32 * u, x, PARTS);
                 }
             }
             arrived();
             k = after; buf ^= 1;
         }
-        // NaN or Inf in the result: it may come from a hidden place (0 times it is NaN), so that the rows are done again value by value
-        bool bad = false;
-        for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) bad |= !isfinite(acc[d][e]);
-        bad = __ballot(bad && live) != 0;
-        if (!FEW) {
-            if (lane == 0) shared_bad[wave] = bad;
-            wait_block();
-            bad = shared_bad[0] | shared_bad[1] | shared_bad[2] | shared_bad[3];
-            wait_block();
-        }
-        if (!bad) break;
+    };
+    pass(std::false_type());
+    // NaN or Inf in the result: it may come from a hidden place (0 times it is NaN), so that the rows are done again value by value
+    float check = 0.f;
+    for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) check += acc[d][e] * 0.f;
+    bool bad = __ballot(check != 0.f && live) != 0;             // NaN differs from 0
+    if (!FEW) {
+        if (lane == 0) shared_bad[wave] = bad;
+        wait_block();
+        bad = shared_bad[0] | shared_bad[1] | shared_bad[2] | shared_bad[3];
+        wait_block();
     }
+    if (bad) pass(std::true_type());
     l += __shfl_xor(l, 32);
 
     if constexpr (FEW) {                                        // the waves' results of the same rows, joined in LDS: [wave][column][row], rows padded against bank conflicts
@@ -377,10 +379,21 @@ FwdShape fwd_shape(const bigc_seq_attn& a) {
     return sh;
 }
 
+// p in as many parts as the use of o32 needs, which the backward takes delta from: two, or for the f32 gradient of a bias table what adds up to f32's bits
 template <typename T, int HD>
 void launch_fwd(hipStream_t s, const bigc_seq_attn& a, const FwdShape& sh, const int2* ranges, float* part_o, float2* part_ml) {
-    if (sh.few) attn_fwd<T, HD, true><<<(unsigned)sh.blocks, 64 * FwdTile<T, HD, true>::WAVES, sh.lds, s>>>(a, sh, ranges, part_o, part_ml);
-    else attn_fwd<T, HD, false><<<(unsigned)sh.blocks, 256, sh.lds, s>>>(a, sh, ranges, part_o, part_ml);
+    const int threads = sh.few ? 64 * FwdTile<T, HD, true>::WAVES : 256;
+#define LAUNCH(PARTS) do { \
+        if (sh.few) attn_fwd<T, HD, true, PARTS><<<(unsigned)sh.blocks, threads, sh.lds, s>>>(a, sh, ranges, part_o, part_ml); \
+        else attn_fwd<T, HD, false, PARTS><<<(unsigned)sh.blocks, threads, sh.lds, s>>>(a, sh, ranges, part_o, part_ml); \
+    } while (0)
+    if constexpr (sizeof(T) == 4) { LAUNCH(1); return; }
+    else {
+        if (!a.o32) LAUNCH(1);
+        else if (std::is_same<T, bf16_t>::value && a.rel_table) LAUNCH((std::is_same<T, bf16_t>::value ? 3 : 2));
+        else LAUNCH(2);
+    }
+#undef LAUNCH
 }
 template <typename T>
 void launch_fwd_dim(hipStream_t s, const bigc_seq_attn& a, const FwdShape& sh, const int2* ranges, float* part_o, float2* part_ml) {
