@@ -40,7 +40,7 @@ struct BwdShape {
     int q_tiles, k_tiles;                                       // of 128 rows, of the longest sequence
     int q_pairs, k_pairs;                                       // (sequence, head), (sequence, key head)
     size_t q_lds, k_lds;
-    size_t rows, q_ranges, k_ranges, bins, total;               // workspace: [3][n_head][n_q] m, 1 / l, delta; document ranges; sums by distance
+    size_t rows, q_ranges, k_ranges, bins, total;               // workspace: [3][n_head][n_q] P_LIFT - m, 1 / l, delta; document ranges; sums by distance
 };
 
 template <typename T, int HD> struct BwdTile {
@@ -90,6 +90,7 @@ struct TileList {
     int per64, doc_min, doc_max;                                // tiles of 64 rows
     __device__ __forceinline__ int next(int k) const {
         if (k >= ahead && k < first) k = first;
+        if (!ranges) return k >= end || (k >= ahead && k > last) ? end : k;
         while (k < end) {
             const int c = k + (int)(threadIdx.x & 63);
             bool ok = c < end && (c < ahead || (c >= first && c <= last));
@@ -125,6 +126,9 @@ __device__ __forceinline__ void add_diagonals(const f32x16& v, float* bins, int 
     }
 }
 
+template <typename T> constexpr float P_LIFT = 0.f;             // P reaches the product with dO as P 2^P_LIFT (f16 ends at 2^-14)
+template <> constexpr float P_LIFT<f16_t> = 14.f;
+
 template <typename T, int HD>
 __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 2)) void attn_bwd_q(bigc_seq_attn a, BwdShape sh, float* row_data, const int2* ranges, float* by_dist) {
     constexpr int DT = HD / 32, KEYS = BwdTile<T, HD>::KEYS, SUBS = KEYS / 32, TILE = KEYS * Geometry<T, HD>::ROW, BUF = 2 * TILE;
@@ -147,7 +151,7 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
     const int i0 = first + wave * 32, i = min(i0 + col, sp.nq - 1), shift = sp.nk - sp.nq, pos = i + shift;
     const bool live = i0 + col < sp.nq, wave_live = i0 < sp.nq;
     const long row = sp.q0 + i;
-    const ScoreRule rule(a);
+    const ScoreRule rule(a, T());
     const Reach reach(a);
     const int prefix = a.prefix_len ? min(a.prefix_len[s], sp.nk) : 0;
     LaneRow me;
@@ -190,7 +194,7 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
     if (ml.y == 0.f) delta = 0.f;
     if (live && hi == 0) {
         const long plane = a.n_q * a.n_head, at = head * a.n_q + row;
-        row_data[at] = m; row_data[plane + at] = inv_l; row_data[2 * plane + at] = delta;
+        row_data[at] = P_LIFT<T> - m; row_data[plane + at] = inv_l; row_data[2 * plane + at] = delta;
     }
     const float minus = -delta * inv_l;                         // dS = p (dP / l - delta / l)
 
@@ -252,15 +256,15 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
                     for (int c = 0; c < Geometry<T, HD>::STEPS; ++c) x = Mat<T>::mul(rows_frag<T, HD>(kt, 32 * u, c), q[c], x);
                     for (int c = 0; c < Geometry<T, HD>::STEPS; ++c) y = Mat<T>::mul(rows_frag<T, HD>(vt, 32 * u, c), go[c], y);
                     const int d0 = kb + 32 * u + 4 * hi - pos;
-                    make_scores<T, true, true>(x, &t, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (SUBS - 1 - u));
-                    if (!full) hide_scores<true>(x, me, d0, a.q_doc ? docs + buf * 64 + 32 * u + 4 * hi : nullptr);
-                    for (int e = 0; e < 16; ++e) {
-                        const float p = __builtin_amdgcn_exp2f(x[e] - m), ds = p * fmaf(y[e], inv_l, minus);
+                    const Linear sc = make_scores<T, true, true>(x, &t, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (SUBS - 1 - u));
+                    if (!full) hide_scores<true>(x, sc, me, d0, a.q_doc ? docs + buf * 64 + 32 * u + 4 * hi : nullptr);
+                    const float base = sc.c - m;
+                    for (int e = 0; e < 16; ++e) {              // rows that are not there: 0 (1 / l is 0)
+                        const float p = __builtin_amdgcn_exp2f(fmaf(x[e], sc.a, base)), ds = p * fmaf(y[e], inv_l, minus);
                         x[e] = careful && p == 0.f ? 0.f : ds;
                     }
                     if (nb) {
                         const int lo = d_min + 32 * u, up = d_max - 32 * (SUBS - 1 - u);
-                        if (!live) for (int e = 0; e < 16; ++e) x[e] = 0.f;
                         if (lo >= a.bias_radius || up <= -a.bias_radius) {
                             float sum = x[0];
                             for (int e = 1; e < 16; ++e) sum += x[e];
@@ -269,7 +273,7 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
                             add_diagonals(x, bins, kb + 32 * u - (i0 + shift), low);
                         }
                     }
-                    if (rule.cap) for (int e = 0; e < 16; ++e) x[e] *= 1.f - t[e] * t[e];
+                    if (rule.cap) for (int e = 0; e < 16; ++e) x[e] *= cap_slope<T>(t[e]);
                     scale.fit(x, acc, DT);
                     if constexpr (careful) accumulate_seen<T, HD>(acc, kt, 32 * u, x);
                     else Accumulate<T, HD>::add(acc, kt, 32 * u, x);
@@ -297,7 +301,7 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
         }
     }
     if (!live) return;
-    const float f = a.scale * scale.back();
+    const float f = a.scale * scale.back() * (rule.cap ? CAP_SLOPE<T> : 1.f);
     for (int d = 0; d < DT; ++d)
         for (int g = 0; g < 4; ++g) {
             const int c = 32 * d + 8 * g + 4 * hi;
@@ -307,9 +311,6 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
             *(Four*)((T*)a.dq + row * a.lddq + head * a.hsdq + c) = z;
         }
 }
-
-template <typename T> constexpr float P_LIFT = 0.f;             // P reaches the product with dO as P 2^P_LIFT (f16 ends at 2^-14)
-template <> constexpr float P_LIFT<f16_t> = 14.f;
 
 template <typename T, int HD>
 __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_bwd_kv(bigc_seq_attn a, BwdShape sh, const float* row_data, const int2* ranges) {
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
     const int j0 = first + wave * 32, j = min(j0 + col, sp.nk - 1), shift = sp.nk - sp.nq;
     const bool live = j0 + col < sp.nk, wave_live = j0 < sp.nk;
     const long row = sp.k0 + j;
-    const ScoreRule rule(a);
+    const ScoreRule rule(a, T());
     const Reach reach(a);
     const int prefix = a.prefix_len ? min(a.prefix_len[s], sp.nk) : 0;
     LaneRow me;                                                 // streamed queries behind the last are hidden by their distance
@@ -339,7 +340,7 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
     me.hi = j < prefix ? 0x7fffffff : reach.hi;
     me.prefix = 0; me.doc = 0; me.bias = 0;
 
-    // LDS: two buffers of Q and dO tiles; per buffer the rows' m, 1 / l, delta and documents (64 places each); biases of a head
+    // LDS: two buffers of Q and dO tiles; per buffer the rows' -m, 1 / l, delta and documents (64 places each); biases of a head
     char* const side = lds + 2 * BUF;
     float* const biases = (float*)(side + 2 * 4 * 256);
     int doc_min = 0, doc_max = 0, block_doc_min = 0, block_doc_max = 0;
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
             const auto copy_tile = [&](int k, int buf) {
                 stage_q.load(lds + buf * BUF, k * ROWS, sp.nq, wave);
                 stage_o.load(lds + buf * BUF + TILE, k * ROWS, sp.nq, wave);
-                const int at = min(k * ROWS + lane, sp.nq - 1);                            // one of m, 1 / l, delta and the documents a wave
+                const int at = min(k * ROWS + lane, sp.nq - 1);                            // one of -m, 1 / l, delta and the documents a wave
                 if (wave < 3 || a.q_doc) {
                     const void* from = wave < 3 ? (const void*)(row_data + wave * plane + head * a.n_q + sp.q0 + at) : (const void*)(a.q_doc + sp.q0 + at);
                     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, LDS_PTR(void, side + (buf * 4 + wave) * 256), 4, 0, 0);
@@ -413,12 +414,12 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                         for (int c = 0; c < Geometry<T, HD>::STEPS; ++c) x = Mat<T>::mul(rows_frag<T, HD>(qt, 32 * u, c), kf[c], x);
                         for (int c = 0; c < Geometry<T, HD>::STEPS; ++c) y = Mat<T>::mul(rows_frag<T, HD>(ot, 32 * u, c), vf[c], y);
                         const int d0 = j - shift - ib - 32 * u - 4 * hi;
-                        make_scores<T, false, true>(x, &t, rule, me, biases, d0, d_min + 32 * (SUBS - 1 - u), d_max - 32 * u);
-                        if (!full) hide_scores<false>(x, me, d0, a.q_doc ? (const int*)rows + 192 : nullptr);
+                        const Linear sc = make_scores<T, false, true>(x, &t, rule, me, biases, d0, d_min + 32 * (SUBS - 1 - u), d_max - 32 * u);
+                        if (!full) hide_scores<false>(x, sc, me, d0, a.q_doc ? (const int*)rows + 192 : nullptr);
                         for (int g = 0; g < 4; ++g) {
                             const f32x4 m4 = *LDS_PTR(const f32x4, rows + 8 * g), l4 = *LDS_PTR(const f32x4, rows + 64 + 8 * g);
                             for (int e = 0; e < 4; ++e) {
-                                const float p = __builtin_amdgcn_exp2f(x[4 * g + e] - m4[e] + P_LIFT<T>);
+                                const float p = __builtin_amdgcn_exp2f(fmaf(x[4 * g + e], sc.a, sc.c + m4[e]));
                                 x[4 * g + e] = careful && p == 0.f ? 0.f : p * l4[e];
                             }
                         }
@@ -431,7 +432,7 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                                 x[4 * g + e] = careful && p == 0.f ? 0.f : p * (y[4 * g + e] - d4[e]);
                             }
                         }
-                        if (rule.cap) for (int e = 0; e < 16; ++e) x[e] *= 1.f - t[e] * t[e];
+                        if (rule.cap) for (int e = 0; e < 16; ++e) x[e] *= cap_slope<T>(t[e]);
                         scale.fit(x, dk, DT);
                         if constexpr (careful) accumulate_seen<T, HD>(dk, qt, 32 * u, x);
                         else Accumulate<T, HD>::add(dk, qt, 32 * u, x);
@@ -447,7 +448,7 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
     for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) check += (dk[d][e] + dv[d][e]) * 0.f;
     if (any_wave(check != 0.f && live, wave, shared_bad)) pass(std::true_type());
     if (!live) return;
-    const float unlift = P_LIFT<T> == 0.f ? 1.f : 1.f / 16384.f, f = a.scale * scale.back() * unlift;
+    const float unlift = P_LIFT<T> == 0.f ? 1.f : 1.f / 16384.f, f = a.scale * scale.back() * unlift * (rule.cap ? CAP_SLOPE<T> : 1.f);
     static_assert(P_LIFT<f16_t> == 14.f, "");
     for (int d = 0; d < DT; ++d)
         for (int g = 0; g < 4; ++g) {

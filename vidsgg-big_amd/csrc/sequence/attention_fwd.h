@@ -96,7 +96,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
     const bool live = t < rows, wave_live = t0 < rows;
     const int i = min(t, rows - 1) / sh.pack, head = head0 + min(t, rows - 1) % sh.pack, shift = sp.nk - sp.nq;
     const long row = sp.q0 + i;
-    const ScoreRule rule(a);
+    const ScoreRule rule(a, T());
     const Reach reach(a);
     const int prefix = a.prefix_len ? min(a.prefix_len[s], sp.nk) : 0;
     const int pos = i + shift;
@@ -136,6 +136,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
     const int range_tiles = (a.max_k + 63) / 64;
     const auto next_tile = [&](int k) {                          // the first of k, k + stride, ... with something to see, or tile_end
         if (k >= prefix_tiles && k < reach_first) k += (reach_first - k + stride - 1) / stride * stride;
+        if (!a.q_doc) return k >= tile_end || (k >= prefix_tiles && k > reach_last) ? tile_end : k;
         while (k < tile_end) {
             const int c = k + lane * stride;
             bool ok = c < tile_end && (c < prefix_tiles || (c >= reach_first && c <= reach_last));
@@ -201,10 +202,12 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
                     for (int e = 0; e < 16; ++e) x[e] = 0.f;
                     for (int c = 0; c < Geometry<T, HD>::STEPS; ++c) x = Mat<T>::mul(rows_frag<T, HD>(kt, 32 * u, c), q[c], x);
                     const int d0 = kb + 32 * u + 4 * hi - pos;
-                    make_scores<T, true, false>(x, nullptr, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (F::SUBS - 1 - u));
-                    if (!full) hide_scores<true>(x, me, d0, a.q_doc ? my_docs + buf * 64 + 32 * u + 4 * hi : nullptr);
+                    const Linear s = make_scores<T, true, false>(x, nullptr, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (F::SUBS - 1 - u));
+                    if (!full) hide_scores<true>(x, s, me, d0, a.q_doc ? my_docs + buf * 64 + 32 * u + 4 * hi : nullptr);
                     float top = x[0];
-                    for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
+                    if (s.a < 0.f) { for (int e = 1; e < 16; ++e) top = fminf(top, x[e]); }
+                    else { for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]); }
+                    top = fmaf(top, s.a, s.c);
                     top = fmaxf(top, __shfl_xor(top, 32));
                     const bool move = top > m + SLACK<T>;
                     if (__ballot(move)) {
@@ -213,8 +216,8 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
                         l *= c;
                         for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) acc[d][e] *= c;
                     }
-                    const float base = (m == -INFINITY ? 0.f : m) - LIFT<T>;
-                    for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(x[e] - base);
+                    const float base = s.c - ((m == -INFINITY ? 0.f : m) - LIFT<T>);
+                    for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], s.a, base));
                     float sum = x[0];
                     for (int e = 1; e < 16; ++e) sum += x[e];
                     l += sum;

@@ -198,27 +198,36 @@ __device__ __forceinline__ void wait_block() {
 
 // ---- scores -----------------------------------------------------------------------------------------------------------------------------
 
-// What every score of a call has in common; scores are kept times log2 e (exp is then one instruction)
+// What every score of a call has in common; scores are kept times log2 e (exp is then one instruction).  Without a bias by distance a score is linear,
+// a v + c, in a value v: the product itself, or what the cap makes of it.
 struct ScoreRule {
-    float scale2, cap2, cap_in;                                 // scale log2 e; cap log2 e; 2 scale log2 e / cap (the argument of tanh, for 2^x)
-    float cap_y;                                                // scale / cap
+    float a, c;
+    float cap_in, cap_y;                                        // 2 scale log2 e / cap: the argument of tanh doubled, for 2^x; scale / cap
     bool cap, slopes, table;
     int radius;
-    __device__ __forceinline__ ScoreRule(const bigc_seq_attn& a)
-        : scale2(a.scale * LOG2E), cap2(a.softcap * LOG2E), cap_in(a.softcap > 0.f ? 2.f * a.scale / a.softcap * LOG2E : 0.f), cap_y(a.softcap > 0.f ? a.scale / a.softcap : 0.f),
-          cap(a.softcap > 0.f), slopes(a.slopes != nullptr), table(a.rel_table != nullptr), radius(a.bias_radius) {}
+    template <typename T> __device__ __forceinline__ ScoreRule(const bigc_seq_attn& q, T)
+        : a(q.scale * LOG2E), c(0.f), cap_in(0.f), cap_y(0.f), cap(q.softcap > 0.f), slopes(q.slopes != nullptr), table(q.rel_table != nullptr), radius(q.bias_radius) {
+        if (!cap) return;
+        cap_in = 2.f * q.scale / q.softcap * LOG2E;
+        cap_y = q.scale / q.softcap;
+        a = q.softcap * LOG2E;
+        if (sizeof(T) < 4) { c = a; a = -2.f * a; }
+    }
 };
 
-// tanh(y) = 1 - 2 / (e^2y + 1).  Its error is a step of 1, not of the value: half types, whose operands are rounded more coarsely, live with that; f32 takes
-// small arguments through the odd series (to y^13: 2^-26 of the value at 0.5) and divides in full.
+// The capped product's value.  Half types: v = 1 / (e^2y + 1), tanh y = 1 - 2 v -- its error is a step of 1, not of the value, which scores of half operands
+// live with.  f32: v = tanh y, small arguments through the odd series (to y^13: 2^-26 of the value at 0.5), the others with a division in full.
 template <typename T>
-__device__ __forceinline__ float soft_tanh(float x, const ScoreRule& r) {
+__device__ __forceinline__ float cap_value(float x, const ScoreRule& r) {
     const float e = __builtin_amdgcn_exp2f(x * r.cap_in) + 1.f;
-    if (sizeof(T) < 4) return 1.f - 2.f * __builtin_amdgcn_rcpf(e);
+    if (sizeof(T) < 4) return __builtin_amdgcn_rcpf(e);
     const float y = x * r.cap_y, z = y * y;
     const float p = 1.f + z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315 + z * (62.f / 2835 + z * (-1382.f / 155925 + z * (21844.f / 6081075))))));
     return fabsf(y) < 0.5f ? y * p : 1.f - 2.f / e;
 }
+// 1 - tanh^2, for half types without the factor CAP_SLOPE
+template <typename T> __device__ __forceinline__ float cap_slope(float v) { return sizeof(T) < 4 ? v - v * v : 1.f - v * v; }
+template <typename T> constexpr float CAP_SLOPE = sizeof(T) < 4 ? 4.f : 1.f;
 
 // What a call lets a row see, by d = key - position of the query: [lo, hi] (wide enough for any two int32 places), and a prefix
 struct Reach {
@@ -250,43 +259,55 @@ __device__ __forceinline__ void load_biases(const bigc_seq_attn& a, float* biase
 // place of register e's streamed row among the lane's half of 32, without the 4 (l >> 5)
 __device__ __forceinline__ constexpr int reg_row(int e) { return (e & 3) + 8 * (e >> 2); }
 
-// Products of 32 streamed rows with the lanes' rows -> scores, capped and biased.  d0: d of register 0; streamed keys count d up, streamed queries
-// down.  d_min, d_max: the least and the greatest d of the 32 x 32 (where all are beyond the radius one bias serves).  t: the tanh, for the backward.
+// Products of 32 streamed rows with the lanes' rows -> values v with score = a v + c (c the lane's own).  d0: d of register 0; streamed keys count d up,
+// streamed queries down.  d_min, d_max: the least and the greatest d of the 32 x 32: where all are beyond the radius one bias serves and goes into c; else the
+// biased scores themselves become the values.  kept: the capped values, for the backward.
+struct Linear { float a, c; };
 template <typename T, bool LANE_IS_QUERY, bool KEEP>
-__device__ __forceinline__ void make_scores(f32x16& x, f32x16* t, const ScoreRule& r, const LaneRow& l, const float* biases, int d0, int d_min, int d_max) {
+__device__ __forceinline__ Linear make_scores(f32x16& x, f32x16* kept, const ScoreRule& r, const LaneRow& l, const float* biases, int d0, int d_min, int d_max) {
     if (r.cap) {
-        for (int e = 0; e < 16; ++e) {
-            const float y = soft_tanh<T>(x[e], r);
-            if (KEEP) (*t)[e] = y;
-            x[e] = r.cap2 * y;
-        }
-    } else {
-        for (int e = 0; e < 16; ++e) x[e] *= r.scale2;
+        for (int e = 0; e < 16; ++e) x[e] = cap_value<T>(x[e], r);
+        if (KEEP) *kept = x;
     }
-    if (r.slopes) {
-        for (int e = 0; e < 16; ++e) x[e] -= l.slope2 * fabsf((float)(LANE_IS_QUERY ? d0 + reg_row(e) : d0 - reg_row(e)));
-    }
+    Linear s = {r.a, r.c};
+    const float* const b = biases + l.bias + r.radius;
+    bool one_by_one = r.slopes || r.a == 0.f;
+    const bool far = d_min >= r.radius || d_max <= -r.radius;
     if (r.table) {
-        const float* b = biases + l.bias + r.radius;
-        if (d_min >= r.radius || d_max <= -r.radius) {
+        one_by_one |= !far;
+        if (far) {                                              // (a bias so low that it swallows the score must do so)
+            const float v = *LDS_PTR(const float, b + (d_min >= r.radius ? r.radius : -r.radius));
+            s.c += v;
+            one_by_one |= __ballot(!(fabsf(s.c) < 1e30f)) != 0;
+        }
+    }
+    if (one_by_one) {
+        for (int e = 0; e < 16; ++e) x[e] = r.table && far ? x[e] * s.a + r.c : x[e] * s.a + s.c;
+        if (r.slopes) {
+            for (int e = 0; e < 16; ++e) x[e] -= l.slope2 * fabsf((float)(LANE_IS_QUERY ? d0 + reg_row(e) : d0 - reg_row(e)));
+        }
+        if (r.table && far) {
             const float v = *LDS_PTR(const float, b + (d_min >= r.radius ? r.radius : -r.radius));
             for (int e = 0; e < 16; ++e) x[e] += v;
-        } else {
+        } else if (r.table) {
             for (int e = 0; e < 16; ++e) x[e] += *LDS_PTR(const float, b + min(max(LANE_IS_QUERY ? d0 + reg_row(e) : d0 - reg_row(e), -r.radius), r.radius));
         }
+        s = {1.f, 0.f};
     }
+    return s;
 }
 
-// hidden scores -> -inf; docs: the streamed rows' documents from register 0's row on, or null
+// values of hidden scores -> those of the score -inf; docs: the streamed rows' documents from register 0's row on, or null
 template <bool LANE_IS_QUERY>
-__device__ __forceinline__ void hide_scores(f32x16& x, const LaneRow& l, int d0, const int* docs) {
+__device__ __forceinline__ void hide_scores(f32x16& x, const Linear& s, const LaneRow& l, int d0, const int* docs) {
+    const float hidden = s.a < 0.f ? INFINITY : -INFINITY;
     for (int g = 0; g < 4; ++g) {
         i32x4 doc = {l.doc, l.doc, l.doc, l.doc};
         if (docs) doc = *LDS_PTR(const i32x4, docs + 8 * g);
         for (int e = 0; e < 4; ++e) {
             const int d = LANE_IS_QUERY ? d0 + reg_row(4 * g + e) : d0 - reg_row(4 * g + e);
-                        const bool near = (d >= l.lo && d <= l.hi) || (LANE_IS_QUERY && d < l.prefix);
-            if (!near || doc[e] != l.doc || l.doc < 0) x[4 * g + e] = -INFINITY;
+            const bool near = ((d >= l.lo) & (d <= l.hi)) | (LANE_IS_QUERY & (d < l.prefix));
+            x[4 * g + e] = near & (doc[e] == l.doc) & (l.doc >= 0) ? x[4 * g + e] : hidden;
         }
     }
 }
