@@ -45,7 +45,7 @@ struct BwdShape {
 
 template <typename T, int HD> struct BwdTile {
     static constexpr int KEYS = sizeof(T) == 4 ? 32 : 64;                       // streamed rows of the dq kernel
-    static constexpr int ROWS = Geometry<T, HD>::ROW <= 192 ? 64 : 32;          // and of the dk, dv kernel
+    static constexpr int ROWS = Tile<T, HD, 32>::ROW <= 128 ? 64 : 32;          // and of the dk, dv kernel
 };
 constexpr int DIAG_PAD = 64;                                    // bins beyond the radius on both sides: a 32 x 32 that touches the radius reaches so far
 
@@ -131,7 +131,9 @@ template <> constexpr float P_LIFT<f16_t> = 14.f;
 
 template <typename T, int HD>
 __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 2)) void attn_bwd_q(bigc_seq_attn a, BwdShape sh, float* row_data, const int2* ranges, float* by_dist) {
-    constexpr int DT = HD / 32, KEYS = BwdTile<T, HD>::KEYS, SUBS = KEYS / 32, TILE = KEYS * Geometry<T, HD>::ROW, BUF = 2 * TILE;
+    constexpr int DT = HD / 32, KEYS = BwdTile<T, HD>::KEYS, SUBS = KEYS / 32;
+    typedef Tile<T, HD, KEYS> TL;
+    constexpr int TILE = TL::BYTES, BUF = 2 * TILE;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int2 shared_docs[4];
     __shared__ int shared_bad[4];
@@ -171,7 +173,7 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
     __syncthreads();
 
     // the rows' statistics and delta
-    typename Mat<T>::frag q[Geometry<T, HD>::STEPS], go[Geometry<T, HD>::STEPS];
+    typename Mat<T>::frag q[TL::STEPS], go[TL::STEPS];
     load_lane_rows<T, HD>(q, (const T*)a.q + row * a.ldq + head * a.hsq, live, a.head_dim);
     load_lane_rows<T, HD>(go, (const T*)a.d_o + row * a.lddo + head * a.hsdo, live, a.head_dim);
     const long rh = row * a.n_head + head;
@@ -179,16 +181,16 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
     const float m = ml.x == -INFINITY ? 0.f : ml.x, inv_l = ml.y == 0.f ? 0.f : 1.f / ml.y;
     float delta = 0.f;
     if (a.o32) {
-        for (int c = 0; c < Geometry<T, HD>::STEPS; ++c)
-            for (int e = 0; e < Geometry<T, HD>::E; ++e) {
-                const int at = (2 * c + hi) * Geometry<T, HD>::E + e;
+        for (int c = 0; c < TL::STEPS; ++c)
+            for (int e = 0; e < TL::E; ++e) {
+                const int at = (2 * c + hi) * TL::E + e;
                 if (live && at < a.head_dim) delta += (float)go[c][e] * a.o32[rh * a.head_dim + at];
             }
     } else {
-        typename Mat<T>::frag o[Geometry<T, HD>::STEPS];
+        typename Mat<T>::frag o[TL::STEPS];
         load_lane_rows<T, HD>(o, (const T*)a.o + row * a.ldo + head * a.hso, live, a.head_dim);
-        for (int c = 0; c < Geometry<T, HD>::STEPS; ++c)
-            for (int e = 0; e < Geometry<T, HD>::E; ++e) delta += (float)go[c][e] * (float)o[c][e];
+        for (int c = 0; c < TL::STEPS; ++c)
+            for (int e = 0; e < TL::E; ++e) delta += (float)go[c][e] * (float)o[c][e];
     }
     delta += __shfl_xor(delta, 32);
     if (ml.y == 0.f) delta = 0.f;
@@ -207,13 +209,15 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
     list.per64 = 64 / KEYS; list.doc_min = block_doc_min; list.doc_max = block_doc_max;
     const int p_min = min(i0, sp.nq - 1) + shift, p_max = min(i0 + 31, sp.nq - 1) + shift;
 
-    Stage<T, HD, KEYS, 4> stage_k, stage_v;
-    stage_k.init((const T*)a.k + sp.k0 * a.ldk + hk * a.hsk, a.ldk, a.head_dim, wave);
-    stage_v.init((const T*)a.v + sp.k0 * a.ldv + hk * a.hsv, a.ldv, a.head_dim, wave);
+    Stage<TL, 4> stage_k, stage_v;
+    stage_k.init(a.ldk, a.head_dim, wave);
+    stage_v.init(a.ldv, a.head_dim, wave);
+    const T* const k_rows = (const T*)a.k + sp.k0 * a.ldk + hk * a.hsk;
+    const T* const v_rows = (const T*)a.v + sp.k0 * a.ldv + hk * a.hsv;
     int* const docs = (int*)docs_lds;
     const auto copy_tile = [&](int k, int buf) {
-        stage_k.load(lds + buf * BUF, k * KEYS, sp.nk, wave);
-        stage_v.load(lds + buf * BUF + TILE, k * KEYS, sp.nk, wave);
+        stage_k.load(lds + buf * BUF, k_rows, k * KEYS, sp.nk, wave);
+        stage_v.load(lds + buf * BUF + TILE, v_rows, k * KEYS, sp.nk, wave);
         if (a.q_doc && wave == 0)
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.k_doc + sp.k0 + min(k * KEYS + lane, sp.nk - 1)), LDS_PTR(void, docs + buf * 64), 4, 0, 0);
     };
@@ -249,12 +253,11 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
                 full = __builtin_amdgcn_readfirstlane(r.x >= 0 && r.x == r.y && doc_min == r.x && doc_max == r.x);
             }
             if (seen) {
-#pragma unroll 1
                 for (int u = 0; u < SUBS; ++u) {
                     f32x16 x, y, t;
                     for (int e = 0; e < 16; ++e) x[e] = y[e] = 0.f;
-                    for (int c = 0; c < Geometry<T, HD>::STEPS; ++c) x = Mat<T>::mul(rows_frag<T, HD>(kt, 32 * u, c), q[c], x);
-                    for (int c = 0; c < Geometry<T, HD>::STEPS; ++c) y = Mat<T>::mul(rows_frag<T, HD>(vt, 32 * u, c), go[c], y);
+                    for (int c = 0; c < TL::STEPS; ++c) x = Mat<T>::mul(rows_frag<TL>(kt, 32 * u, c), q[c], x);
+                    for (int c = 0; c < TL::STEPS; ++c) y = Mat<T>::mul(rows_frag<TL>(vt, 32 * u, c), go[c], y);
                     const int d0 = kb + 32 * u + 4 * hi - pos;
                     const Linear sc = make_scores<T, true, true>(x, &t, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (SUBS - 1 - u));
                     if (!full) hide_scores<true>(x, sc, me, d0, a.q_doc ? docs + buf * 64 + 32 * u + 4 * hi : nullptr);
@@ -275,8 +278,8 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
                     }
                     if (rule.cap) for (int e = 0; e < 16; ++e) x[e] *= cap_slope<T>(t[e]);
                     scale.fit(x, acc, DT);
-                    if constexpr (careful) accumulate_seen<T, HD>(acc, kt, 32 * u, x);
-                    else Accumulate<T, HD>::add(acc, kt, 32 * u, x);
+                    if constexpr (careful) accumulate_seen<TL>(acc, kt, 32 * u, x);
+                    else accumulate<TL>(acc, kt, 32 * u, x);
                 }
             }
             wait_block();
@@ -314,7 +317,9 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
 
 template <typename T, int HD>
 __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_bwd_kv(bigc_seq_attn a, BwdShape sh, const float* row_data, const int2* ranges) {
-    constexpr int DT = HD / 32, ROWS = BwdTile<T, HD>::ROWS, SUBS = ROWS / 32, TILE = ROWS * Geometry<T, HD>::ROW, BUF = 2 * TILE;
+    constexpr int DT = HD / 32, ROWS = BwdTile<T, HD>::ROWS, SUBS = ROWS / 32;
+    typedef Tile<T, HD, ROWS> TL;
+    constexpr int TILE = TL::BYTES, BUF = 2 * TILE;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int2 shared_docs[4];
     __shared__ int shared_bad[4];
@@ -348,7 +353,7 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
         me.doc = live ? a.k_doc[row] : -1;
         doc_bounds(me.doc, live, wave, shared_docs, doc_min, doc_max, block_doc_min, block_doc_max);
     }
-    typename Mat<T>::frag kf[Geometry<T, HD>::STEPS], vf[Geometry<T, HD>::STEPS];
+    typename Mat<T>::frag kf[TL::STEPS], vf[TL::STEPS];
     load_lane_rows<T, HD>(kf, (const T*)a.k + row * a.ldk + hk * a.hsk, live, a.head_dim);
     load_lane_rows<T, HD>(vf, (const T*)a.v + row * a.ldv + hk * a.hsv, live, a.head_dim);
 
@@ -362,6 +367,9 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
     list.per64 = 64 / ROWS; list.doc_min = block_doc_min; list.doc_max = block_doc_max;
     const int j_min = min(j0, sp.nk - 1), j_max = min(j0 + 31, sp.nk - 1);
     const long plane = a.n_q * a.n_head;
+    Stage<TL, 4> stage_q, stage_o;
+    stage_q.init(a.ldq, a.head_dim, wave);
+    stage_o.init(a.lddo, a.head_dim, wave);
 
     f32x16 dk[DT], dv[DT];
     GradScale<T> scale;
@@ -373,12 +381,11 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
         for (int head = hk * group; head < (hk + 1) * group; ++head) {
             me.slope2 = rule.slopes ? a.slopes[head] * LOG2E : 0.f;
             if (rule.table) { __syncthreads(); load_biases(a, biases, head, 1); }          // (readable behind the first wait below)
-            Stage<T, HD, ROWS, 4> stage_q, stage_o;
-            stage_q.init((const T*)a.q + sp.q0 * a.ldq + head * a.hsq, a.ldq, a.head_dim, wave);
-            stage_o.init((const T*)a.d_o + sp.q0 * a.lddo + head * a.hsdo, a.lddo, a.head_dim, wave);
+            const T* const q_rows = (const T*)a.q + sp.q0 * a.ldq + head * a.hsq;
+            const T* const o_rows = (const T*)a.d_o + sp.q0 * a.lddo + head * a.hsdo;
             const auto copy_tile = [&](int k, int buf) {
-                stage_q.load(lds + buf * BUF, k * ROWS, sp.nq, wave);
-                stage_o.load(lds + buf * BUF + TILE, k * ROWS, sp.nq, wave);
+                stage_q.load(lds + buf * BUF, q_rows, k * ROWS, sp.nq, wave);
+                stage_o.load(lds + buf * BUF + TILE, o_rows, k * ROWS, sp.nq, wave);
                 const int at = min(k * ROWS + lane, sp.nq - 1);                            // one of -m, 1 / l, delta and the documents a wave
                 if (wave < 3 || a.q_doc) {
                     const void* from = wave < 3 ? (const void*)(row_data + wave * plane + head * a.n_q + sp.q0 + at) : (const void*)(a.q_doc + sp.q0 + at);
@@ -406,13 +413,12 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                     full = __builtin_amdgcn_readfirstlane(r.x >= 0 && r.x == r.y && doc_min == r.x && doc_max == r.x);
                 }
                 if (seen) {
-#pragma unroll 1
                     for (int u = 0; u < SUBS; ++u) {
                         const float* const rows = (const float*)(side + buf * 1024) + 32 * u + 4 * hi;
                         f32x16 x, y, t;
                         for (int e = 0; e < 16; ++e) x[e] = y[e] = 0.f;
-                        for (int c = 0; c < Geometry<T, HD>::STEPS; ++c) x = Mat<T>::mul(rows_frag<T, HD>(qt, 32 * u, c), kf[c], x);
-                        for (int c = 0; c < Geometry<T, HD>::STEPS; ++c) y = Mat<T>::mul(rows_frag<T, HD>(ot, 32 * u, c), vf[c], y);
+                        for (int c = 0; c < TL::STEPS; ++c) x = Mat<T>::mul(rows_frag<TL>(qt, 32 * u, c), kf[c], x);
+                        for (int c = 0; c < TL::STEPS; ++c) y = Mat<T>::mul(rows_frag<TL>(ot, 32 * u, c), vf[c], y);
                         const int d0 = j - shift - ib - 32 * u - 4 * hi;
                         const Linear sc = make_scores<T, false, true>(x, &t, rule, me, biases, d0, d_min + 32 * (SUBS - 1 - u), d_max - 32 * u);
                         if (!full) hide_scores<false>(x, sc, me, d0, a.q_doc ? (const int*)rows + 192 : nullptr);
@@ -423,8 +429,8 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                                 x[4 * g + e] = careful && p == 0.f ? 0.f : p * l4[e];
                             }
                         }
-                        if constexpr (careful) accumulate_seen<T, HD>(dv, ot, 32 * u, x);
-                        else Accumulate<T, HD>::add(dv, ot, 32 * u, x);
+                        if constexpr (careful) accumulate_seen<TL>(dv, ot, 32 * u, x);
+                        else accumulate<TL>(dv, ot, 32 * u, x);
                         for (int g = 0; g < 4; ++g) {
                             const f32x4 d4 = *LDS_PTR(const f32x4, rows + 128 + 8 * g);
                             for (int e = 0; e < 4; ++e) {
@@ -434,8 +440,8 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                         }
                         if (rule.cap) for (int e = 0; e < 16; ++e) x[e] *= cap_slope<T>(t[e]);
                         scale.fit(x, dk, DT);
-                        if constexpr (careful) accumulate_seen<T, HD>(dk, qt, 32 * u, x);
-                        else Accumulate<T, HD>::add(dk, qt, 32 * u, x);
+                        if constexpr (careful) accumulate_seen<TL>(dk, qt, 32 * u, x);
+                        else accumulate<TL>(dk, qt, 32 * u, x);
                     }
                 }
                 wait_block();
@@ -486,11 +492,11 @@ __global__ __launch_bounds__(1024) void rel_table_grad(bigc_seq_attn a, const fl
 
 BwdShape bwd_shape(const bigc_seq_attn& a) {
     BwdShape sh = {};
-    const int hd = tile_dim(a.head_dim), row = hd * seq_size(a.dtype), nb = a.rel_table ? 2 * a.bias_radius + 1 : 0;
+    const int row = tile_row(a), nb = a.rel_table ? 2 * a.bias_radius + 1 : 0;
     sh.q_tiles = cdiv(a.max_q, 128); sh.k_tiles = cdiv(a.max_k, 128);
     sh.q_pairs = a.n_seq * a.n_head; sh.k_pairs = a.n_seq * a.n_kv_head;
-    sh.q_lds = (size_t)4 * (a.dtype == BIGC_F32 ? 32 : 64) * row + (a.q_doc ? 512 : 0) + sizeof(float) * (nb + (a.d_rel_table ? 4 * (nb + 2 * DIAG_PAD) : 0));
-    sh.k_lds = (size_t)4 * (row <= 192 ? 64 : 32) * row + 2048 + sizeof(float) * nb;
+    sh.q_lds = (size_t)4 * tile_bytes(a.dtype == BIGC_F32 ? 32 : 64, row) + (a.q_doc ? 512 : 0) + sizeof(float) * (nb + (a.d_rel_table ? 4 * (nb + 2 * DIAG_PAD) : 0));
+    sh.k_lds = (size_t)4 * tile_bytes(row <= 128 ? 64 : 32, row) + 2048 + sizeof(float) * nb;
     sh.rows = 0;
     sh.q_ranges = round_up(sizeof(float) * 3 * (size_t)a.n_q * a.n_head, 256);
     sh.k_ranges = sh.q_ranges + (a.q_doc ? round_up(sizeof(int2) * (size_t)a.n_seq * ((a.max_q + 63) / 64), 256) : 0);

@@ -18,8 +18,9 @@ struct FwdShape {
 
 template <typename T, int HD, bool FEW> struct FwdTile {
     static constexpr int KEYS = FEW || sizeof(T) == 4 ? 32 : 64, SUBS = KEYS / 32;
-    static constexpr int WAVES = FEW && Geometry<T, HD>::ROW > 256 ? 2 : 4;         // (rows of 384 and 512 bytes: 160 KB of LDS hold the buffers of two)
-    static constexpr int TILE = KEYS * Geometry<T, HD>::ROW, BUF = 2 * TILE;        // bytes: one tile, K and V
+    typedef Tile<T, HD, KEYS> TL;
+    static constexpr int WAVES = FEW && TL::ROW > 256 ? 2 : 4;                      // (rows of 512 bytes: 160 KB of LDS hold the buffers of two)
+    static constexpr int TILE = TL::BYTES, BUF = 2 * TILE;                          // bytes: one tile, K and V
     static constexpr int STAGES = (FEW ? WAVES : 1) * 2 * BUF;                      // two buffers of a block (many) or of each wave (few)
     static constexpr int DOCS = (FEW ? WAVES : 1) * 2 * 64 * 4;
 };
@@ -77,7 +78,8 @@ template <> constexpr float LIFT<f16_t> = 11.f;
 template <typename T, int HD, bool FEW, int PARTS>
 __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(T) == 4 && HD > 96) ? 1 : 2)) void attn_fwd(bigc_seq_attn a, FwdShape sh, const int2* ranges, float* part_o, float2* part_ml) {
     typedef FwdTile<T, HD, FEW> F;
-    constexpr int DT = HD / 32, E = Geometry<T, HD>::E;
+    typedef typename F::TL TL;
+    constexpr int DT = HD / 32;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int shared_bad[4];
     __shared__ int2 shared_docs[4];
@@ -151,17 +153,19 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
         return tile_end;
     };
 
-    typename Mat<T>::frag q[Geometry<T, HD>::STEPS];
+    typename Mat<T>::frag q[TL::STEPS];
     load_lane_rows<T, HD>(q, (const T*)a.q + row * a.ldq + head * a.hsq, live, a.head_dim);
-    Stage<T, HD, F::KEYS, FEW ? 1 : F::WAVES> stage_k, stage_v;
-    stage_k.init((const T*)a.k + sp.k0 * a.ldk + hk * a.hsk, a.ldk, a.head_dim, FEW ? 0 : wave);
-    stage_v.init((const T*)a.v + sp.k0 * a.ldv + hk * a.hsv, a.ldv, a.head_dim, FEW ? 0 : wave);
+    Stage<TL, FEW ? 1 : F::WAVES> stage_k, stage_v;
+    const int sw = FEW ? 0 : wave;
+    stage_k.init(a.ldk, a.head_dim, sw);
+    stage_v.init(a.ldv, a.head_dim, sw);
+    const T* const k_rows = (const T*)a.k + sp.k0 * a.ldk + hk * a.hsk;
+    const T* const v_rows = (const T*)a.v + sp.k0 * a.ldv + hk * a.hsv;
     char* const mine = lds + (FEW ? wave * 2 * F::BUF : 0);
     int* const my_docs = (int*)(docs_lds) + (FEW ? wave * 128 : 0);
-    const int sw = FEW ? 0 : wave;
     const auto copy_tile = [&](int k, int buf) {
-        stage_k.load(mine + buf * F::BUF, k * F::KEYS, sp.nk, sw);
-        stage_v.load(mine + buf * F::BUF + F::TILE, k * F::KEYS, sp.nk, sw);
+        stage_k.load(mine + buf * F::BUF, k_rows, k * F::KEYS, sp.nk, sw);
+        stage_v.load(mine + buf * F::BUF + F::TILE, v_rows, k * F::KEYS, sp.nk, sw);
         if (a.q_doc && sw == 0)
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.k_doc + sp.k0 + min(k * F::KEYS + lane, sp.nk - 1)),
                                              LDS_PTR(void, my_docs + buf * 64), 4, 0, 0);
@@ -196,11 +200,10 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
                 full = __builtin_amdgcn_readfirstlane(r.x >= 0 && r.x == r.y && doc_min == r.x && doc_max == r.x);
             }
             if (seen) {
-#pragma unroll 1
                 for (int u = 0; u < F::SUBS; ++u) {                 // 32 keys at a time
                     f32x16 x;
                     for (int e = 0; e < 16; ++e) x[e] = 0.f;
-                    for (int c = 0; c < Geometry<T, HD>::STEPS; ++c) x = Mat<T>::mul(rows_frag<T, HD>(kt, 32 * u, c), q[c], x);
+                    for (int c = 0; c < TL::STEPS; ++c) x = Mat<T>::mul(rows_frag<TL>(kt, 32 * u, c), q[c], x);
                     const int d0 = kb + 32 * u + 4 * hi - pos;
                     const Linear s = make_scores<T, true, false>(x, nullptr, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (F::SUBS - 1 - u));
                     if (!full) hide_scores<true>(x, s, me, d0, a.q_doc ? my_docs + buf * 64 + 32 * u + 4 * hi : nullptr);
@@ -221,8 +224,8 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
                     float sum = x[0];
                     for (int e = 1; e < 16; ++e) sum += x[e];
                     l += sum;
-                    if constexpr (careful) accumulate_seen<T, HD>(acc, vt, 32 * u, x);
-                    else Accumulate<T, HD>::add(acc, vt, 32 * u, x, PARTS);
+                    if constexpr (careful) accumulate_seen<TL>(acc, vt, 32 * u, x);
+                    else accumulate<TL>(acc, vt, 32 * u, x, PARTS);
                 }
             }
             arrived();
@@ -248,7 +251,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
         __syncthreads();
         float* const o_all = (float*)lds;
         float* const ml_all = o_all + F::WAVES * HD * PAD;
-        static_assert(!FEW || ((F::WAVES * (HD * PAD + 2 * 32)) * 4 <= F::STAGES && F::STAGES <= 128 * 1024), "");
+        static_assert(!FEW || ((F::WAVES * (HD * PAD + 2 * 32)) * 4 <= F::STAGES && F::STAGES <= 136 * 1024), "");
         for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) o_all[(wave * HD + 32 * d + mfma_row(e, hi)) * PAD + col] = acc[d][e];
         if (hi == 0) { ml_all[wave * 32 + col] = m; ml_all[(F::WAVES + wave) * 32 + col] = l; }
         __syncthreads();
@@ -304,7 +307,6 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
             if (a.o32) *(float4*)(a.o32 + rh * a.head_dim + c) = make_float4(y[0], y[1], y[2], y[3]);
         }
     if (a.stats && hi == 0) *(float2*)(a.stats + 2 * rh) = make_float2(m - LIFT<T>, l);
-    (void)E;
 }
 
 // Joins the chunks of every (row, head): a wave each
@@ -347,6 +349,9 @@ __global__ __launch_bounds__(256) void zero_rows(T* t, long ld, long hs, long n,
 }
 
 int tile_dim(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 96 ? 96 : 128; }
+// bytes of a row and of a tile in LDS (see Tile)
+int tile_row(const bigc_seq_attn& a) { const int hd = tile_dim(a.head_dim); return (hd == 96 ? 128 : hd) * seq_size(a.dtype); }
+int tile_bytes(int rows, int row) { return rows * row / 1024 * (1024 + 32); }
 size_t round_up(size_t n, size_t m) { return (n + m - 1) / m * m; }
 
 FwdShape fwd_shape(const bigc_seq_attn& a) {
@@ -374,8 +379,8 @@ FwdShape fwd_shape(const bigc_seq_attn& a) {
     sh.splits = (int)((a.max_k + sh.chunk - 1) / sh.chunk);
     if (sh.splits < 1) sh.splits = 1;
     sh.blocks = row_blocks * sh.splits;
-    const int hd = tile_dim(a.head_dim), tile = keys * hd * seq_size(a.dtype);
-    sh.lds = (size_t)(!sh.few ? 1 : hd * seq_size(a.dtype) > 256 ? 2 : 4) * (4 * tile + (a.q_doc ? 512 : 0)) + sizeof(float) * sh.pack * nb;
+    const int row = tile_row(a), tile = tile_bytes(keys, row);
+    sh.lds = (size_t)(!sh.few ? 1 : row > 256 ? 2 : 4) * (4 * tile + (a.q_doc ? 512 : 0)) + sizeof(float) * sh.pack * nb;
     sh.part_o = a.q_doc ? round_up(sizeof(int2) * (size_t)a.n_seq * ((a.max_k + 63) / 64), 256) : 0;
     sh.part_ml = sh.part_o + (sh.splits > 1 ? round_up(sizeof(float) * (size_t)sh.splits * a.n_q * a.n_head * a.head_dim, 256) : 0);
     sh.total = sh.part_ml + (sh.splits > 1 ? round_up(sizeof(float2) * (size_t)sh.splits * a.n_q * a.n_head, 256) : 0);

@@ -41,48 +41,59 @@ template <> struct Mat<float> {
     }
 };
 
-// A tile of ROWS rows of HD columns in LDS, 16-byte chunks swizzled so that eight (sixteen) rows' chunks of one column, which a row-major fragment
-// reads together, and four rows' pairs of chunks, which a transposed one does, lie in different banks.
-template <typename T, int HD>
-struct Geometry {
-    static constexpr int E = 16 / (int)sizeof(T), CH = HD / E, ROW = HD * (int)sizeof(T), STEPS = CH / 2;      // chunks a row, bytes a row, fragments a row
-    static __device__ __forceinline__ int swizzle(int row) {
-        if (CH % 16 == 0) return ((row & 3) << 1) | (((row >> 2) & 1) << 3) | ((row >> 3) & 1);
-        if (CH % 8 == 0) return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
-        return (row >> 2) & 3;
-    }
-    static __device__ __forceinline__ int place(int row, int chunk) { return row * ROW + ((chunk ^ swizzle(row)) << 4); }
+// A tile of ROWS rows of HD columns in LDS, as the copies of 64 lanes x 16 bytes lay it down: copy b holds rows b, b + B, b + 2 B, ... one after the other
+// (B copies in all, 1024 bytes each, 32 bytes apart).  Eight rows' chunks of one column, which a row-major fragment reads together, and four rows' pairs
+// of chunks, which a transposed one does, then lie in different banks, and the place of a fragment is the lane's own plus a constant -- an address register for
+// each kind of fragment and no arithmetic in the loops (chunks swizzled by row, which do the same for the banks, took one per fragment, and spilled).
+// 96 columns lie in rows of 128.
+template <typename T_, int HD_, int ROWS_>
+struct Tile {
+    typedef T_ T;
+    static constexpr int HD = HD_, ROWS = ROWS_;
+    static constexpr int E = 16 / (int)sizeof(T), ROW = (HD == 96 ? 128 : HD) * (int)sizeof(T), CH = ROW / 16, STEPS = HD / E / 2;      // chunk's elements; bytes and chunks of a row; fragments of it
+    static constexpr int B = ROWS * ROW / 1024, PITCH = 1024 + 32, BYTES = B * PITCH;
+    static_assert(B >= 2 && B <= 16 && 32 % B == 0 && ROWS % B == 0, "");
+    static __device__ __forceinline__ int place(int row, int chunk) { return row % B * PITCH + row / B * ROW + chunk * 16; }
 };
 
-// A operand, row-major: rows row0 .. row0 + 31, columns of step `s`
-template <typename T, int HD>
-__device__ __forceinline__ typename Mat<T>::frag rows_frag(const char* tile, int row0, int s) {
+// A operand, row-major: rows row0 .. row0 + 31 (row0 a multiple of 32), columns of step `s`
+template <typename TL>
+__device__ __forceinline__ typename Mat<typename TL::T>::frag rows_frag(const char* tile, int row0, int s) {
     const int l = threadIdx.x & 63;
-    return *LDS_PTR(const typename Mat<T>::frag, tile + Geometry<T, HD>::place(row0 + (l & 31), 2 * s + (l >> 5)));
+    return *LDS_PTR(const typename Mat<typename TL::T>::frag, tile + TL::place(l & 31, l >> 5) + (row0 / TL::B * TL::ROW + 32 * s));
 }
 
-// A operand, transposed: columns col0 .. col0 + 31, the 16 rows row0 + .. in the order in which a product's registers 8 u .. 8 u + 7 hold them (half types)
-template <typename T, int HD>
-__device__ __forceinline__ typename Mat<T>::frag cols_frag(const char* tile, int row0, int col0) {
-    const int l = threadIdx.x & 63, i = l & 15, hi = l >> 5;
-    const int chunk = (col0 >> 3) + ((l >> 4) & 1) * 2 + ((i >> 1) & 1), r = row0 + 4 * hi + (i >> 2);
-    union { s16x4 v[2]; typename Mat<T>::frag f; } u;
-    u.v[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, tile + Geometry<T, HD>::place(r, chunk) + (i & 1) * 8));
-    u.v[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, tile + Geometry<T, HD>::place(r + 8, chunk) + (i & 1) * 8));
+// A operand, transposed: columns col0 .. col0 + 31, the 16 rows from row0 on (a multiple of 16) in the order in which a product's registers 8 u .. 8 u + 7
+// hold them (half types)
+template <typename TL>
+__device__ __forceinline__ typename Mat<typename TL::T>::frag cols_frag(const char* tile, int row0, int col0) {
+    const int l = threadIdx.x & 63, i = l & 15, r = 4 * (l >> 5) + (i >> 2);           // lanes 4 k .. 4 k + 3 of 16 point at row k's 16 columns, and get a column of the four rows each
+    const char* const at = tile + TL::place(r, ((l >> 4) & 1) * 2 + ((i >> 1) & 1)) + (i & 1) * 8;
+    const int first = row0 % TL::B * TL::PITCH + row0 / TL::B * TL::ROW + col0 * 2, second = (row0 + 8) % TL::B * TL::PITCH + (row0 + 8) / TL::B * TL::ROW + col0 * 2;
+    static_assert(8 % TL::B == 0 || TL::B == 16, "");                                  // row0 and row0 + 8 add to a lane's place without a carry
+    union { s16x4 v[2]; typename Mat<typename TL::T>::frag f; } u;
+    u.v[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, at + first));
+    u.v[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(LDS_PTR(s16x4, at + second));
     return u.f;
 }
 
 // acc[d columns of a block of 32][lane's row] += sum over the 32 streamed rows from row0 of tile^T x values; `values` in a product's register order.
 // Half types round the values; what that leaves goes through further products (of k parts 2^-8k (bf16) or 2^-11k (f16) of a value remain).
-template <typename T, int HD>
-struct Accumulate;
-template <typename T, int HD>
-struct AccumulateHalf {
-    static __device__ __forceinline__ void add(f32x16* acc, const char* tile, int row0, const f32x16& v, int parts = 1) {
+template <typename TL>
+__device__ __forceinline__ void accumulate(f32x16* acc, const char* tile, int row0, const f32x16& v, int parts = 1) {
+    typedef typename TL::T T;
+    if constexpr (sizeof(T) == 4) {
+        const int l = threadIdx.x & 63, hi = l >> 5, c = l & 31;
+        for (int r = 0; r < 16; ++r) {
+            const int row = mfma_row(r, 0);                     // + 4 (l >> 5), without a carry
+            const char* const at = tile + TL::place(4 * hi, c >> 2) + (c & 3) * 4 + (row0 + row) % TL::B * TL::PITCH + (row0 + row) / TL::B * TL::ROW;
+            for (int dt = 0; dt < TL::HD / 32; ++dt) acc[dt] = mfma32(*LDS_PTR(const float, at + 128 * dt), v[r], acc[dt]);
+        }
+    } else {
         typename Mat<T>::frag b[2];
         for (int e = 0; e < 8; ++e) { b[0][e] = (T)v[e]; b[1][e] = (T)v[8 + e]; }
         for (int u = 0; u < 2; ++u)
-            for (int dt = 0; dt < HD / 32; ++dt) acc[dt] = Mat<T>::mul(cols_frag<T, HD>(tile, row0 + 16 * u, 32 * dt), b[u], acc[dt]);
+            for (int dt = 0; dt < TL::HD / 32; ++dt) acc[dt] = Mat<T>::mul(cols_frag<TL>(tile, row0 + 16 * u, 32 * dt), b[u], acc[dt]);
         if (parts == 1) return;
         f32x16 rest = v;
 #pragma unroll 1
@@ -90,27 +101,15 @@ struct AccumulateHalf {
             for (int u = 0; u < 2; ++u)
                 for (int e = 0; e < 8; ++e) { rest[8 * u + e] -= (float)b[u][e]; b[u][e] = (T)rest[8 * u + e]; }
             for (int u = 0; u < 2; ++u)
-                for (int dt = 0; dt < HD / 32; ++dt) acc[dt] = Mat<T>::mul(cols_frag<T, HD>(tile, row0 + 16 * u, 32 * dt), b[u], acc[dt]);
+                for (int dt = 0; dt < TL::HD / 32; ++dt) acc[dt] = Mat<T>::mul(cols_frag<TL>(tile, row0 + 16 * u, 32 * dt), b[u], acc[dt]);
         }
     }
-};
-template <int HD> struct Accumulate<bf16_t, HD> : AccumulateHalf<bf16_t, HD> {};
-template <int HD> struct Accumulate<f16_t, HD> : AccumulateHalf<f16_t, HD> {};
-template <int HD>
-struct Accumulate<float, HD> {
-    static __device__ __forceinline__ void add(f32x16* acc, const char* tile, int row0, const f32x16& v, int = 1) {
-        const int l = threadIdx.x & 63, hi = l >> 5, c = l & 31;
-        for (int r = 0; r < 16; ++r) {
-            const int row = row0 + mfma_row(r, hi);
-            for (int dt = 0; dt < HD / 32; ++dt)
-                acc[dt] = mfma32(*LDS_PTR(const float, tile + Geometry<float, HD>::place(row, dt * 8 + (c >> 2)) + (c & 3) * 4), v[r], acc[dt]);
-        }
-    }
-};
+}
 
 // The same, one value at a time: a value of 0 takes no part, whatever its row of the tile holds.  For the calls whose tiles hold NaN or Inf in hidden places.
-template <typename T, int HD>
+template <typename TL>
 __device__ __forceinline__ void accumulate_seen(f32x16* acc, const char* tile, int row0, const f32x16& v) {
+    typedef typename TL::T T;
     const int l = threadIdx.x & 63, hi = l >> 5;
 #pragma unroll 1
     for (int r = 0; r < 16; ++r) {
@@ -120,10 +119,10 @@ __device__ __forceinline__ void accumulate_seen(f32x16* acc, const char* tile, i
         for (int half = 0; half < 2; ++half) {
             const float p = __shfl(mine, (l & 31) + 32 * half);
             const int row = row0 + mfma_row(r, half);
-            for (int dt = 0; dt < HD / 32; ++dt)
+            for (int dt = 0; dt < TL::HD / 32; ++dt)
                 for (int e = 0; e < 16; ++e) {
                     const int col = 32 * dt + mfma_row(e, hi);
-                    const float x = (float)*LDS_PTR(const T, tile + Geometry<T, HD>::place(row, col / Geometry<T, HD>::E) + col % Geometry<T, HD>::E * (int)sizeof(T));
+                    const float x = (float)*LDS_PTR(const T, tile + TL::place(row, 0) + col * (int)sizeof(T));
                     acc[dt][e] += p != 0.f ? p * x : 0.f;
                 }
         }
@@ -133,58 +132,53 @@ __device__ __forceinline__ void accumulate_seen(f32x16* acc, const char* tile, i
 // B operand: the lane's row, all steps, from memory (zeros behind head_dim and for rows that are not there)
 template <typename T, int HD>
 __device__ __forceinline__ void load_lane_rows(typename Mat<T>::frag* f, const T* row, bool live, int hd) {
+    constexpr int E = 16 / (int)sizeof(T);
     const int hi = (threadIdx.x & 63) >> 5;
-    for (int s = 0; s < Geometry<T, HD>::STEPS; ++s) {
-        const int c = (2 * s + hi) * Geometry<T, HD>::E;
+    for (int s = 0; s < HD / E / 2; ++s) {
+        const int c = (2 * s + hi) * E;
         union { i32x4 raw; typename Mat<T>::frag f; } u;
         u.raw = live && c < hd ? *(const i32x4*)(row + c) : i32x4{0, 0, 0, 0};
         f[s] = u.f;
     }
 }
 
-// Copies tiles of ROWS rows into LDS straight from memory, 16 bytes a lane; NW waves share the work.  A lane's offset from the tile's first row is the
-// same for every tile that is whole.  Behind head_dim the columns repeat the row's first chunk (their products are with zeros, or not stored).
-template <typename T, int HD, int ROWS, int NW>
+// Copies tiles into LDS straight from memory, 16 bytes a lane; NW waves share the work.  A lane's offset from the tile's first row is the same for every
+// tile that is whole.  Behind head_dim the columns repeat the row's first chunk (their products are with zeros, or not stored).
+template <typename TL, int NW>
 struct Stage {
-    typedef Geometry<T, HD> G;
-    static constexpr int N = ROWS * G::CH / 64 / NW;
-    static_assert(ROWS * G::CH % (64 * NW) == 0, "");
-    unsigned off[N];
-    const char* base;
+    typedef typename TL::T T;
+    static constexpr int N = TL::B / NW;
+    static_assert(TL::B % NW == 0, "");
+    unsigned off;                                               // of the first copy's rows; copy i's lie i NW rows on
     long step;                                                  // bytes from row to row
-    int hd;
+    int row, chunk, hd;                                         // the lane's place in the first copy
 
-    __device__ __forceinline__ int row_of(int i, int wave) const { return ((i * NW + wave) * 64 + (int)(threadIdx.x & 63)) / G::CH; }
-    __device__ __forceinline__ int chunk_of(int i, int wave) const {
-        const int c = (((i * NW + wave) * 64 + (int)(threadIdx.x & 63)) % G::CH) ^ G::swizzle(row_of(i, wave));
-        return c * G::E < hd ? c : 0;
-    }
-    __device__ __forceinline__ void init(const T* first_row, long ld, int head_dim, int wave) {
-        base = (const char*)first_row;
+    __device__ __forceinline__ void init(long ld, int head_dim, int wave) {
+        const int lane = threadIdx.x & 63;
         step = ld * (long)sizeof(T);
         hd = head_dim;
-        for (int i = 0; i < N; ++i) off[i] = (unsigned)(row_of(i, wave) * step) + chunk_of(i, wave) * 16;
+        row = lane / TL::CH * TL::B + wave;
+        chunk = lane % TL::CH;
+        off = (unsigned)(row * step) + (chunk * TL::E < hd ? chunk : 0) * 16;
     }
-    // rows row0 .. row0 + ROWS - 1 of n: those behind the last repeat it (n > 0)
-    __device__ __forceinline__ void load(char* tile, int row0, int n, int wave) const {
-        const char* from = base + row0 * step;
-        if (row0 + ROWS <= n) {
+    // rows row0 .. row0 + ROWS - 1 of the n from first_row on: those behind the last repeat it (n > 0)
+    __device__ __forceinline__ void load(char* tile, const T* first_row, int row0, int n, int wave) const {
+        const char* from = (const char*)first_row + row0 * step;
+        if (row0 + TL::ROWS <= n) {
             for (int i = 0; i < N; ++i)
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + off[i]), LDS_PTR(void, tile + (i * NW + wave) * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + i * NW * step + off), LDS_PTR(void, tile + (i * NW + wave) * TL::PITCH), 16, 0, 0);
         } else {
             for (int i = 0; i < N; ++i) {
-                const int r = min(row_of(i, wave), n - 1 - row0);
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + r * step + chunk_of(i, wave) * 16),
-                                                 LDS_PTR(void, tile + (i * NW + wave) * 1024), 16, 0, 0);
+                const int r = min(row + i * NW, n - 1 - row0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + r * step + (chunk * TL::E < hd ? chunk : 0) * 16),
+                                                 LDS_PTR(void, tile + (i * NW + wave) * TL::PITCH), 16, 0, 0);
             }
         }
     }
     // zeros behind head_dim (for tiles that may hold Inf, which a product with 0 would make NaN)
     __device__ __forceinline__ void clear_tail(char* tile, int wave) const {
-        for (int i = 0; i < N; ++i) {
-            const int at = ((i * NW + wave) * 64 + (int)(threadIdx.x & 63)) % G::CH ^ G::swizzle(row_of(i, wave));
-            if (at * G::E >= hd) *LDS_PTR(i32x4, tile + ((i * NW + wave) * 64 + (threadIdx.x & 63)) * 16) = i32x4{0, 0, 0, 0};
-        }
+        if (chunk * TL::E < hd) return;
+        for (int i = 0; i < N; ++i) *LDS_PTR(i32x4, tile + (i * NW + wave) * TL::PITCH + (threadIdx.x & 63) * 16) = i32x4{0, 0, 0, 0};
     }
 };
 
