@@ -735,7 +735,7 @@ typedef struct {
     void* dq; int64_t lddq, hsdq;
     void* dk; int64_t lddk, hsdk;      /* summed over the query heads of a key head */
     void* dv; int64_t lddv, hsdv;
-    float* d_rel_table;                /* (n_bucket, n_head), overwritten; may be NULL */
+    float* d_rel_table;                /* (n_bucket, n_head), overwritten; may be NULL; f32 heads over 64 columns: bias_radius <= 1023 */
 } bigc_seq_attn;
 
 /* bytes of the workspace (16-byte aligned) of one call; depends on the sizes, masks and biases in *a, not on the tensors; 0 for arguments that the call would refuse */

@@ -97,6 +97,7 @@ extern "C" int bigc_seq_attn_bwd(void* stream, const bigc_seq_attn* ap, void* wo
     if ((rc = check_rows(a, who, "dv", a.dv, a.lddv, a.hsdv, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
     BIGC_CHECK_ARG(a.n_q == 0 || (a.stats && (uintptr_t)a.stats % 8 == 0), "%s: stats is NULL or not a multiple of 8 bytes", who);
     BIGC_CHECK_ARG(!a.d_rel_table || a.rel_table, "%s: d_rel_table without rel_table", who);
+    BIGC_CHECK_ARG(!a.d_rel_table || a.dtype != BIGC_F32 || a.head_dim <= 64 || a.bias_radius <= 1023, "%s: d_rel_table of f32 heads over 64 columns: radius %d (at most 1023)", who, a.bias_radius);
     const BwdShape sh = bwd_shape(a);
     if (workspace_bytes < sh.total || (sh.total && (!workspace || (uintptr_t)workspace % 16)))
         return bigc_fail(BIGC_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, sh.total);
@@ -110,7 +111,7 @@ extern "C" int bigc_seq_attn_bwd(void* stream, const bigc_seq_attn* ap, void* wo
         doc_ranges<<<(unsigned)(((long)a.n_seq * kt + 3) / 4), 256, 0, hs>>>(a, true, kt, (int2*)(ws + sh.k_ranges));
     }
 #define F(T) \
-    launch_bwd_dim<T>(hs, a, sh, ws); \
+    launch_bwd_dim<typename std::conditional<std::is_same<T, float>::value, f32s, T>::type>(hs, a, sh, ws); \
     if (a.zero_rest && a.n_q && !q_blocks) zero_rows<T><<<256, 256, 0, hs>>>((T*)a.dq, a.lddq, a.hsdq, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq); \
     if (a.zero_rest && a.n_k && !k_blocks) { \
         zero_rows<T><<<256, 256, 0, hs>>>((T*)a.dk, a.lddk, a.hsdk, a.n_k, a.n_kv_head, a.head_dim, a.k_off, a.n_seq); \
@@ -119,7 +120,7 @@ extern "C" int bigc_seq_attn_bwd(void* stream, const bigc_seq_attn* ap, void* wo
     SEQ_DISPATCH(a.dtype, F);
 #undef F
     if (a.d_rel_table)
-        rel_table_grad<<<a.n_head, 1024, sizeof(float) * (2 * a.bias_radius + 1 + 1024), hs>>>(a, (const float*)(ws + sh.bins), q_blocks ? a.n_seq * sh.q_tiles : 0);
+        rel_table_grad<<<a.n_head, 1024, sizeof(float) * (2 * (2 * a.bias_radius + 1) + 1024), hs>>>(a, (const float*)(ws + sh.bins), q_blocks ? a.n_seq * sh.q_tiles : 0);
     BIGC_LAUNCH_CHECK("seq_attn_bwd");
     return BIGC_OK;
 }

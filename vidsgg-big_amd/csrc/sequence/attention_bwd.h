@@ -45,7 +45,7 @@ struct BwdShape {
 
 template <typename T, int HD> struct BwdTile {
     static constexpr int KEYS = sizeof(T) == 4 ? 32 : 64;                       // streamed rows of the dq kernel
-    static constexpr int ROWS = Tile<T, HD, 32>::ROW <= 128 ? 64 : 32;          // and of the dk, dv kernel
+    static constexpr int ROWS = sizeof(T) == 2 && HD <= 64 ? 64 : 32;          // and of the dk, dv kernel
 };
 constexpr int DIAG_PAD = 64;                                    // bins beyond the radius on both sides: a 32 x 32 that touches the radius reaches so far
 
@@ -130,7 +130,7 @@ template <typename T> constexpr float P_LIFT = 0.f;             // P reaches the
 template <> constexpr float P_LIFT<f16_t> = 14.f;
 
 template <typename T, int HD>
-__global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 2)) void attn_bwd_q(bigc_seq_attn a, BwdShape sh, float* row_data, const int2* ranges, float* by_dist) {
+__global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 32) ? 1 : 2)) void attn_bwd_q(bigc_seq_attn a, BwdShape sh, float* row_data, const int2* ranges, float* by_dist) {
     constexpr int DT = HD / 32, KEYS = BwdTile<T, HD>::KEYS, SUBS = KEYS / 32;
     typedef Tile<T, HD, KEYS> TL;
     constexpr int TILE = TL::BYTES, BUF = 2 * TILE;
@@ -233,7 +233,8 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
         below = above = 0.f;
         for (int e = lane; e < nbins; e += 64) bins[e] = 0.f;
         int k = list.next(0), buf = 0;
-        if (k < list.end) copy_tile(k, 0);
+        const auto finish_tile = [&](int buf) { stage_k.finish(lds + buf * BUF, wave); stage_v.finish(lds + buf * BUF + TILE, wave); };
+        if (k < list.end) { copy_tile(k, 0); finish_tile(0); }
         wait_block();
         while (k < list.end) {
             const int after = list.next(k + 1);
@@ -282,6 +283,7 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 64) ? 1 : 
                     else accumulate<TL>(acc, kt, 32 * u, x);
                 }
             }
+            if (after < list.end) finish_tile(buf ^ 1);
             wait_block();
             k = after; buf ^= 1;
         }
@@ -393,7 +395,8 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                 }
             };
             int k = list.next(0), buf = 0;
-            if (k < list.end) copy_tile(k, 0);
+            const auto finish_tile = [&](int buf) { stage_q.finish(lds + buf * BUF, wave); stage_o.finish(lds + buf * BUF + TILE, wave); };
+            if (k < list.end) { copy_tile(k, 0); finish_tile(0); }
             wait_block();
             while (k < list.end) {
                 const int after = list.next(k + 1);
@@ -444,6 +447,7 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                         else accumulate<TL>(dk, qt, 32 * u, x);
                     }
                 }
+                if (after < list.end) finish_tile(buf ^ 1);
                 wait_block();
                 k = after; buf ^= 1;
             }
@@ -467,36 +471,43 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
         }
 }
 
-// The table's gradient of one head: the blocks' sums by distance, added in order by four threads a bin, then the bins of every bucket
+// The table's gradient of one head: the blocks' sums by distance, added in order by four threads a bin (eight loads on their way at a time), then
+// the bins of every bucket by 32 threads each
 __global__ __launch_bounds__(1024) void rel_table_grad(bigc_seq_attn a, const float* by_dist, int blocks) {
-    extern __shared__ float total[];                            // [nb], then [4][256]
+    extern __shared__ float total[];                            // [nb] sums, [nb] buckets, then [4][256]
     const int nb = 2 * a.bias_radius + 1, h = blockIdx.x, lane = threadIdx.x & 255, part = threadIdx.x >> 8;
-    float* const parts = total + nb;
+    int* const bucket = (int*)(total + nb);
+    float* const parts = total + 2 * nb;
+    for (int b = threadIdx.x; b < nb; b += 1024) bucket[b] = min(max(a.rel_map[b], 0), a.n_bucket - 1);
     for (int b0 = 0; b0 < nb; b0 += 256) {
         const int b = b0 + lane;
         float x = 0.f;
-        if (b < nb)
-            for (int k = part; k < blocks; k += 4) x += by_dist[((long)k * a.n_head + h) * nb + b];
+        for (int k0 = part; k0 < blocks; k0 += 32) {
+            float v[8];
+            for (int i = 0; i < 8; ++i) v[i] = b < nb && k0 + 4 * i < blocks ? by_dist[((long)(k0 + 4 * i) * a.n_head + h) * nb + b] : 0.f;
+            for (int i = 0; i < 8; ++i) x += v[i];
+        }
         parts[part * 256 + lane] = x;
         __syncthreads();
         if (part == 0 && b < nb) total[b] = (parts[lane] + parts[256 + lane]) + (parts[512 + lane] + parts[768 + lane]);
         __syncthreads();
     }
-    for (int k = threadIdx.x; k < a.n_bucket; k += 1024) {
+    for (int k = threadIdx.x >> 5; k < a.n_bucket; k += 32) {
         float x = 0.f;
-        for (int b = 0; b < nb; ++b)
-            if (min(max(a.rel_map[b], 0), a.n_bucket - 1) == k) x += total[b];
-        a.d_rel_table[(long)k * a.n_head + h] = x;
+        for (int b = threadIdx.x & 31; b < nb; b += 32) x += bucket[b] == k ? total[b] : 0.f;
+        for (int m = 16; m; m >>= 1) x += __shfl_xor(x, m);
+        if ((threadIdx.x & 31) == 0) a.d_rel_table[(long)k * a.n_head + h] = x;
     }
 }
 
 BwdShape bwd_shape(const bigc_seq_attn& a) {
     BwdShape sh = {};
-    const int row = tile_row(a), nb = a.rel_table ? 2 * a.bias_radius + 1 : 0;
+    const bool split = a.dtype == BIGC_F32;
+    const int nb = a.rel_table ? 2 * a.bias_radius + 1 : 0;
     sh.q_tiles = cdiv(a.max_q, 128); sh.k_tiles = cdiv(a.max_k, 128);
     sh.q_pairs = a.n_seq * a.n_head; sh.k_pairs = a.n_seq * a.n_kv_head;
-    sh.q_lds = (size_t)4 * tile_bytes(a.dtype == BIGC_F32 ? 32 : 64, row) + (a.q_doc ? 512 : 0) + sizeof(float) * (nb + (a.d_rel_table ? 4 * (nb + 2 * DIAG_PAD) : 0));
-    sh.k_lds = (size_t)4 * tile_bytes(row <= 128 ? 64 : 32, row) + 2048 + sizeof(float) * nb;
+    sh.q_lds = (size_t)4 * tile_bytes(a, split ? 32 : 64, split) + (a.q_doc ? 512 : 0) + sizeof(float) * (nb + (a.d_rel_table ? 4 * (nb + 2 * DIAG_PAD) : 0));
+    sh.k_lds = (size_t)4 * tile_bytes(a, !split && tile_dim(a.head_dim) <= 64 ? 64 : 32, split) + 2048 + sizeof(float) * nb;
     sh.rows = 0;
     sh.q_ranges = round_up(sizeof(float) * 3 * (size_t)a.n_q * a.n_head, 256);
     sh.k_ranges = sh.q_ranges + (a.q_doc ? round_up(sizeof(int2) * (size_t)a.n_seq * ((a.max_q + 63) / 64), 256) : 0);

@@ -1,7 +1,6 @@
 // Forward of the attention over ordered rows.
 #pragma once
 #include "attention_tiles.h"
-#include <type_traits>
 
 namespace {
 
@@ -170,6 +169,10 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.k_doc + sp.k0 + min(k * F::KEYS + lane, sp.nk - 1)),
                                              LDS_PTR(void, my_docs + buf * 64), 4, 0, 0);
     };
+    const auto finish_tile = [&](int buf) {
+        stage_k.finish(mine + buf * F::BUF, sw);
+        stage_v.finish(mine + buf * F::BUF + F::TILE, sw);
+    };
     const auto arrived = [&] { if (FEW) wait_copies(); else wait_block(); };
 
     f32x16 acc[DT];
@@ -179,7 +182,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
         for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
         m = -INFINITY; l = 0.f;
         int k = __builtin_amdgcn_readfirstlane(next_tile(tile_begin + (FEW ? wave : 0))), buf = 0;
-        if (k < tile_end) copy_tile(k, 0);
+        if (k < tile_end) { copy_tile(k, 0); finish_tile(0); }
         arrived();
         while (k < tile_end) {
             const int after = __builtin_amdgcn_readfirstlane(next_tile(k + stride));
@@ -228,6 +231,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
                     else accumulate<TL>(acc, vt, 32 * u, x, PARTS);
                 }
             }
+            if (after < tile_end) finish_tile(buf ^ 1);
             arrived();
             k = after; buf ^= 1;
         }
@@ -349,9 +353,11 @@ __global__ __launch_bounds__(256) void zero_rows(T* t, long ld, long hs, long n,
 }
 
 int tile_dim(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 96 ? 96 : 128; }
-// bytes of a row and of a tile in LDS (see Tile)
-int tile_row(const bigc_seq_attn& a) { const int hd = tile_dim(a.head_dim); return (hd == 96 ? 128 : hd) * seq_size(a.dtype); }
-int tile_bytes(int rows, int row) { return rows * row / 1024 * (1024 + 32); }
+// bytes of a tile in LDS (see Tile); split: f32 in its three parts
+int tile_bytes(const bigc_seq_attn& a, int rows, bool split) {
+    const int hd = tile_dim(a.head_dim), columns = hd == 96 ? 128 : hd;
+    return (split ? 3 : 1) * (rows * columns * (split ? 2 : seq_size(a.dtype)) / 1024 * (1024 + 32));
+}
 size_t round_up(size_t n, size_t m) { return (n + m - 1) / m * m; }
 
 FwdShape fwd_shape(const bigc_seq_attn& a) {
@@ -379,7 +385,7 @@ FwdShape fwd_shape(const bigc_seq_attn& a) {
     sh.splits = (int)((a.max_k + sh.chunk - 1) / sh.chunk);
     if (sh.splits < 1) sh.splits = 1;
     sh.blocks = row_blocks * sh.splits;
-    const int row = tile_row(a), tile = tile_bytes(keys, row);
+    const int tile = tile_bytes(a, keys, a.dtype == BIGC_F32 && !sh.few), row = tile_dim(a.head_dim) * seq_size(a.dtype);
     sh.lds = (size_t)(!sh.few ? 1 : row > 256 ? 2 : 4) * (4 * tile + (a.q_doc ? 512 : 0)) + sizeof(float) * sh.pack * nb;
     sh.part_o = a.q_doc ? round_up(sizeof(int2) * (size_t)a.n_seq * ((a.max_k + 63) / 64), 256) : 0;
     sh.part_ml = sh.part_o + (sh.splits > 1 ? round_up(sizeof(float) * (size_t)sh.splits * a.n_q * a.n_head * a.head_dim, 256) : 0);
@@ -391,9 +397,11 @@ FwdShape fwd_shape(const bigc_seq_attn& a) {
 template <typename T, int HD>
 void launch_fwd(hipStream_t s, const bigc_seq_attn& a, const FwdShape& sh, const int2* ranges, float* part_o, float2* part_ml) {
     const int threads = sh.few ? 64 * FwdTile<T, HD, true>::WAVES : 256;
+    // (f32: few rows wait for memory, which is then copied as it is; many for the products, which then run on its parts)
+    typedef typename std::conditional<std::is_same<T, float>::value, f32s, T>::type Many;
 #define LAUNCH(PARTS) do { \
         if (sh.few) attn_fwd<T, HD, true, PARTS><<<(unsigned)sh.blocks, threads, sh.lds, s>>>(a, sh, ranges, part_o, part_ml); \
-        else attn_fwd<T, HD, false, PARTS><<<(unsigned)sh.blocks, threads, sh.lds, s>>>(a, sh, ranges, part_o, part_ml); \
+        else attn_fwd<Many, HD, false, PARTS><<<(unsigned)sh.blocks, threads, sh.lds, s>>>(a, sh, ranges, part_o, part_ml); \
     } while (0)
     if constexpr (sizeof(T) == 4) { LAUNCH(1); return; }
     else {

@@ -8,6 +8,7 @@
 #pragma once
 #include "sequence.h"
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
@@ -41,6 +42,49 @@ template <> struct Mat<float> {
     }
 };
 
+// f32 whose products run on the bf16 matrix instructions: a value is the sum of three bf16 (its first, second and third eight bits: the parts are cut
+// off, not rounded, so that nothing is lost), a product of two the sum of the six of their parts' products that reach 2^-16 of it; what is left out is under
+// 2^-21, on average 2^-24, of the product.  192 cycles for 16 steps of a 32 x 32 product, where the f32 instructions take 512; no range is lost (bf16 has f32's).
+struct f32s {
+    float x;
+    f32s() = default;
+    __device__ __forceinline__ f32s(float y) : x(y) {}
+    __device__ __forceinline__ operator float() const { return x; }
+};
+struct Parts {
+    bf16x8 h, m, l;
+    __device__ __forceinline__ float operator[](int e) const { return (float)h[e] + (float)m[e] + (float)l[e]; }
+};
+// two values' parts, in pairs
+__device__ __forceinline__ void split_pair(float a, float b, unsigned& h, unsigned& m, unsigned& l) {
+    constexpr unsigned HIGH = 0xffff0000u, BOTH = 0x07060302u;
+    const float ra = a - __uint_as_float(__float_as_uint(a) & HIGH), rb = b - __uint_as_float(__float_as_uint(b) & HIGH);
+    const float sa = ra - __uint_as_float(__float_as_uint(ra) & HIGH), sb = rb - __uint_as_float(__float_as_uint(rb) & HIGH);
+    h = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), BOTH);
+    m = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), BOTH);
+    l = __builtin_amdgcn_perm(__float_as_uint(sb), __float_as_uint(sa), BOTH);
+}
+// the same where values may be Inf or NaN, which are their own first part
+__device__ __forceinline__ void split_pair_any(float a, float b, unsigned& h, unsigned& m, unsigned& l) {
+    split_pair(a, b, h, m, l);
+    const unsigned keep = (isfinite(a) ? 0xffffu : 0u) | (isfinite(b) ? 0xffff0000u : 0u);
+    m &= keep;
+    l &= keep;
+    if (isnan(a)) h |= 0x40u;
+    if (isnan(b)) h |= 0x400000u;
+}
+template <> struct Mat<f32s> {
+    typedef Parts frag;
+    static __device__ __forceinline__ f32x16 mul(const frag& a, const frag& b, f32x16 c) {
+        c = Mat<bf16_t>::mul(a.l, b.h, c);
+        c = Mat<bf16_t>::mul(a.h, b.l, c);
+        c = Mat<bf16_t>::mul(a.m, b.m, c);
+        c = Mat<bf16_t>::mul(a.m, b.h, c);
+        c = Mat<bf16_t>::mul(a.h, b.m, c);
+        return Mat<bf16_t>::mul(a.h, b.h, c);
+    }
+};
+
 // A tile of ROWS rows of HD columns in LDS, as the copies of 64 lanes x 16 bytes lay it down: copy b holds rows b, b + B, b + 2 B, ... one after the other
 // (B copies in all, 1024 bytes each, 32 bytes apart).  Eight rows' chunks of one column, which a row-major fragment reads together, and four rows' pairs
 // of chunks, which a transposed one does, then lie in different banks, and the place of a fragment is the lane's own plus a constant -- an address register for
@@ -56,10 +100,22 @@ struct Tile {
     static __device__ __forceinline__ int place(int row, int chunk) { return row % B * PITCH + row / B * ROW + chunk * 16; }
 };
 
+// f32s: a tile of each part
+template <int HD_, int ROWS_>
+struct Tile<f32s, HD_, ROWS_> {
+    typedef f32s T;
+    typedef Tile<bf16_t, HD_, ROWS_> Part;
+    static constexpr int HD = HD_, ROWS = ROWS_, E = Part::E, ROW = Part::ROW, STEPS = Part::STEPS, BYTES = 3 * Part::BYTES;
+};
+
 // A operand, row-major: rows row0 .. row0 + 31 (row0 a multiple of 32), columns of step `s`
 template <typename TL>
 __device__ __forceinline__ typename Mat<typename TL::T>::frag rows_frag(const char* tile, int row0, int s) {
     const int l = threadIdx.x & 63;
+    if constexpr (std::is_same<typename TL::T, f32s>::value) {
+        typedef typename TL::Part P;
+        return {rows_frag<P>(tile, row0, s), rows_frag<P>(tile + P::BYTES, row0, s), rows_frag<P>(tile + 2 * P::BYTES, row0, s)};
+    } else
     return *LDS_PTR(const typename Mat<typename TL::T>::frag, tile + TL::place(l & 31, l >> 5) + (row0 / TL::B * TL::ROW + 32 * s));
 }
 
@@ -82,7 +138,18 @@ __device__ __forceinline__ typename Mat<typename TL::T>::frag cols_frag(const ch
 template <typename TL>
 __device__ __forceinline__ void accumulate(f32x16* acc, const char* tile, int row0, const f32x16& v, int parts = 1) {
     typedef typename TL::T T;
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (std::is_same<T, f32s>::value) {
+        typedef typename TL::Part P;
+        for (int u = 0; u < 2; ++u) {
+            union { unsigned w[4]; bf16x8 f; } h, m, l;
+            for (int e = 0; e < 4; ++e) split_pair(v[8 * u + 2 * e], v[8 * u + 2 * e + 1], h.w[e], m.w[e], l.w[e]);
+            const Parts b = {h.f, m.f, l.f};
+            for (int dt = 0; dt < TL::HD / 32; ++dt) {
+                const Parts a = {cols_frag<P>(tile, row0 + 16 * u, 32 * dt), cols_frag<P>(tile + P::BYTES, row0 + 16 * u, 32 * dt), cols_frag<P>(tile + 2 * P::BYTES, row0 + 16 * u, 32 * dt)};
+                acc[dt] = Mat<f32s>::mul(a, b, acc[dt]);
+            }
+        }
+    } else if constexpr (sizeof(T) == 4) {
         const int l = threadIdx.x & 63, hi = l >> 5, c = l & 31;
         for (int r = 0; r < 16; ++r) {
             const int row = mfma_row(r, 0);                     // + 4 (l >> 5), without a carry
@@ -122,7 +189,14 @@ __device__ __forceinline__ void accumulate_seen(f32x16* acc, const char* tile, i
             for (int dt = 0; dt < TL::HD / 32; ++dt)
                 for (int e = 0; e < 16; ++e) {
                     const int col = 32 * dt + mfma_row(e, hi);
-                    const float x = (float)*LDS_PTR(const T, tile + TL::place(row, 0) + col * (int)sizeof(T));
+                    float x;
+                    if constexpr (std::is_same<T, f32s>::value) {
+                        typedef typename TL::Part P;
+                        const char* const at = tile + P::place(row, 0) + col * 2;
+                        x = (float)*LDS_PTR(const bf16_t, at) + (float)*LDS_PTR(const bf16_t, at + P::BYTES) + (float)*LDS_PTR(const bf16_t, at + 2 * P::BYTES);
+                    } else {
+                        x = (float)*LDS_PTR(const T, tile + TL::place(row, 0) + col * (int)sizeof(T));
+                    }
                     acc[dt][e] += p != 0.f ? p * x : 0.f;
                 }
         }
@@ -132,8 +206,20 @@ __device__ __forceinline__ void accumulate_seen(f32x16* acc, const char* tile, i
 // B operand: the lane's row, all steps, from memory (zeros behind head_dim and for rows that are not there)
 template <typename T, int HD>
 __device__ __forceinline__ void load_lane_rows(typename Mat<T>::frag* f, const T* row, bool live, int hd) {
-    constexpr int E = 16 / (int)sizeof(T);
     const int hi = (threadIdx.x & 63) >> 5;
+    if constexpr (std::is_same<T, f32s>::value) {
+        for (int s = 0; s < HD / 16; ++s) {
+            const int c = 16 * s + 8 * hi;
+            union { f32x4 v[2]; float x[8]; } u;
+            for (int q = 0; q < 2; ++q) u.v[q] = live && c < hd ? *(const f32x4*)((const float*)row + c + 4 * q) : f32x4{0.f, 0.f, 0.f, 0.f};
+            union { unsigned w[4]; bf16x8 f; } h, m, l;
+            for (int e = 0; e < 4; ++e) split_pair_any(u.x[2 * e], u.x[2 * e + 1], h.w[e], m.w[e], l.w[e]);
+            f[s] = {h.f, m.f, l.f};
+        }
+        return;
+    }
+    constexpr int E = 16 / (int)sizeof(T);
+    if constexpr (!std::is_same<T, f32s>::value)
     for (int s = 0; s < HD / E / 2; ++s) {
         const int c = (2 * s + hi) * E;
         union { i32x4 raw; typename Mat<T>::frag f; } u;
@@ -175,11 +261,45 @@ struct Stage {
             }
         }
     }
+    // what is left to do between the copies' arrival and the barrier
+    __device__ __forceinline__ void finish(char*, int) const {}
     // zeros behind head_dim (for tiles that may hold Inf, which a product with 0 would make NaN)
     __device__ __forceinline__ void clear_tail(char* tile, int wave) const {
         if (chunk * TL::E < hd) return;
         for (int i = 0; i < N; ++i) *LDS_PTR(i32x4, tile + (i * NW + wave) * TL::PITCH + (threadIdx.x & 63) * 16) = i32x4{0, 0, 0, 0};
     }
+};
+
+// f32s: through registers, where the values fall into their parts; a thread has 16 bytes of a row at a time
+template <int HD, int ROWS, int NW>
+struct Stage<Tile<f32s, HD, ROWS>, NW> {
+    typedef typename Tile<f32s, HD, ROWS>::Part P;
+    static constexpr int PER_ROW = HD / 4, N = ROWS * PER_ROW / (64 * NW);
+    static_assert(ROWS * PER_ROW % (64 * NW) == 0, "");
+    long step;
+    int hd;
+    f32x4 v[N];
+    __device__ __forceinline__ int row_of(int i, int wave) const { return ((i * NW + wave) * 64 + (int)(threadIdx.x & 63)) / PER_ROW; }
+    __device__ __forceinline__ int col_of(int i, int wave) const { return ((i * NW + wave) * 64 + (int)(threadIdx.x & 63)) % PER_ROW * 4; }
+    __device__ __forceinline__ void init(long ld, int head_dim, int) { step = ld; hd = head_dim; }
+    __device__ __forceinline__ void load(char*, const f32s* first_row, int row0, int n, int wave) {
+        for (int i = 0; i < N; ++i) {
+            const int r = min(row0 + row_of(i, wave), n - 1), c = col_of(i, wave);
+            v[i] = c < hd ? *(const f32x4*)((const float*)first_row + r * step + c) : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    __device__ __forceinline__ void finish(char* tile, int wave) const {
+        typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
+        for (int i = 0; i < N; ++i) {
+            unsigned h[2], m[2], l[2];
+            for (int q = 0; q < 2; ++q) split_pair_any(v[i][2 * q], v[i][2 * q + 1], h[q], m[q], l[q]);
+            char* const at = tile + P::place(row_of(i, wave), 0) + col_of(i, wave) * 2;
+            *LDS_PTR(u32x2, at) = u32x2{h[0], h[1]};
+            *LDS_PTR(u32x2, at + P::BYTES) = u32x2{m[0], m[1]};
+            *LDS_PTR(u32x2, at + 2 * P::BYTES) = u32x2{l[0], l[1]};
+        }
+    }
+    __device__ __forceinline__ void clear_tail(char*, int) const {}
 };
 
 // own copies have arrived / and everybody's, and nobody reads the buffer any more that the next copies go to
