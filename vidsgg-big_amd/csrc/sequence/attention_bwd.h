@@ -37,15 +37,24 @@ template <> struct GradScale<f16_t> {
 };
 
 struct BwdShape {
-    int q_tiles, k_tiles;                                       // of 128 rows, of the longest sequence
+    int q_split, k_split;                                       // which form of the kernels (see BwdTile)
+    int q_tiles, k_tiles;                                       // of a block's rows, of the longest sequence
     int q_pairs, k_pairs;                                       // (sequence, head), (sequence, key head)
     size_t q_lds, k_lds;
     size_t rows, q_ranges, k_ranges, bins, total;               // workspace: [3][n_head][n_q] P_LIFT - m, 1 / l, delta; document ranges; sums by distance
 };
 
-template <typename T, int HD> struct BwdTile {
-    static constexpr int KEYS = sizeof(T) == 4 ? 32 : 64;                       // streamed rows of the dq kernel
-    static constexpr int ROWS = sizeof(T) == 2 && HD <= 64 ? 64 : 32;          // and of the dk, dv kernel
+// SPLIT: for launches of few blocks.  A block then has 32 rows instead of 128, and its waves take the streamed tiles of the same rows in turn, each through
+// LDS of its own; their sums are joined at the end, in order.  Not for f32s, where every wave would have to take its tiles apart by itself (clips of 8
+// videos, 256 whole blocks: 93 and 74 us whole, 152 and 95 us split).
+template <typename T, int HD, bool SPLIT, bool KV> struct BwdTile {
+    static constexpr int ROWS = sizeof(T) == 4 || SPLIT || (KV && HD > 64) ? 32 : 64, SUBS = ROWS / 32;          // streamed rows of a tile
+    typedef Tile<T, HD, ROWS> TL;
+    static constexpr int WAVES = 4, BLOCK_ROWS = SPLIT ? 32 : 128, NW = SPLIT ? 1 : 4, NBUF = 2;
+    static constexpr int TILE = TL::BYTES, BUF = 2 * TILE, STAGES = (SPLIT ? WAVES : 1) * NBUF * BUF;
+    static constexpr int SIDE = KV ? 1024 : 256, SIDES = (SPLIT ? WAVES : 1) * NBUF * SIDE;            // beside a tile: the streamed queries' -m, 1 / l, delta, documents; keys' documents
+    static constexpr int PAD = 33, JOIN = WAVES * HD * PAD * 4;
+    static_assert(!SPLIT || (JOIN <= STAGES && STAGES <= 140 * 1024), "");
 };
 constexpr int DIAG_PAD = 64;                                    // bins beyond the radius on both sides: a 32 x 32 that touches the radius reaches so far
 
@@ -63,14 +72,14 @@ __device__ __forceinline__ bool bwd_place(int pairs, int tiles, int& pair, int& 
 }
 
 // document range of the block's live lanes: [min of those >= 0, max], and of the wave's: [min with -1 for padding, max]
-__device__ __forceinline__ void doc_bounds(int doc, bool live, int wave, int2* shared, int& wave_min, int& wave_max, int& block_min, int& block_max) {
+__device__ __forceinline__ void doc_bounds(int doc, bool live, int wave, int2* shared, int& wave_min, int& wave_max, int& block_min, int& block_max, int waves = 4) {
     int lo = live ? max(doc, -1) : 0x7fffffff, some = live && doc >= 0 ? doc : 0x7fffffff, most = live ? doc : -1;
     for (int m = 32; m; m >>= 1) { lo = min(lo, __shfl_xor(lo, m)); some = min(some, __shfl_xor(some, m)); most = max(most, __shfl_xor(most, m)); }
     wave_min = __builtin_amdgcn_readfirstlane(lo); wave_max = __builtin_amdgcn_readfirstlane(most);
     if ((threadIdx.x & 63) == 0) shared[wave] = make_int2(some, most);
     __syncthreads();
     block_min = shared[0].x; block_max = shared[0].y;
-    for (int w = 1; w < 4; ++w) { block_min = min(block_min, shared[w].x); block_max = max(block_max, shared[w].y); }
+    for (int w = 1; w < waves; ++w) { block_min = min(block_min, shared[w].x); block_max = max(block_max, shared[w].y); }
 }
 
 // whether a lane of any of the block's four waves has `x`
@@ -83,29 +92,22 @@ __device__ __forceinline__ bool any_wave(bool x, int wave, int* shared) {
     return x;
 }
 
-// a block's streamed tiles: those before `ahead`, or in [first, last], and of a document the block has
-struct TileList {
-    int end, ahead, first, last;
-    const int2* ranges;                                         // by 64 rows, or null
-    int per64, doc_min, doc_max;                                // tiles of 64 rows
-    __device__ __forceinline__ int next(int k) const {
-        if (k >= ahead && k < first) k = first;
-        if (!ranges) return k >= end || (k >= ahead && k > last) ? end : k;
-        while (k < end) {
-            const int c = k + (int)(threadIdx.x & 63);
-            bool ok = c < end && (c < ahead || (c >= first && c <= last));
-            if (ok && ranges) {
-                const int2 r = ranges[c / per64];
-                ok = r.x <= doc_max && r.y >= doc_min;
-            }
-            const unsigned long long m = __ballot(ok);
-            if (m) return __builtin_amdgcn_readfirstlane(k + (int)__builtin_ctzll(m));
-            k += 64;
-        }
-        return end;
+
+// Joins the waves' sums for the same 32 rows (`f` times each wave's own) through LDS and stores them as rows of T
+template <typename T, typename B>
+__device__ __forceinline__ void join_rows(char* lds, const f32x16* acc, float f, int n, int hd, T* out, long ld) {
+    const int wave = threadIdx.x / 64, l = threadIdx.x & 63, hi = l >> 5, col = l & 31;
+    float* const all = (float*)lds;
+    __syncthreads();
+    for (int d = 0; d < B::TL::HD / 32; ++d) for (int e = 0; e < 16; ++e) all[(wave * B::TL::HD + 32 * d + mfma_row(e, hi)) * B::PAD + col] = acc[d][e] * f;
+    __syncthreads();
+    for (int e = threadIdx.x; e < n * hd; e += 64 * B::WAVES) {
+        const int r = e / hd, c = e % hd;
+        float x = 0.f;
+        for (int w = 0; w < B::WAVES; ++w) x += all[(w * B::TL::HD + c) * B::PAD + r];
+        out[r * ld + c] = (T)x;
     }
-};
-__device__ __forceinline__ int tile_floor(long row, int rows) { return row < 0 ? -1 : (int)min(row / rows, 0x3fffffffl); }
+}
 
 // Adds the 32 x 32 sums of `v` along its diagonals to bins (a wave's own): lane c of column c, register e of key e.  Lane s takes column (s + key) mod 32 of
 // every key, so that it holds diagonal -s where that did not wrap and 32 - s where it did.
@@ -129,11 +131,11 @@ __device__ __forceinline__ void add_diagonals(const f32x16& v, float* bins, int 
 template <typename T> constexpr float P_LIFT = 0.f;             // P reaches the product with dO as P 2^P_LIFT (f16 ends at 2^-14)
 template <> constexpr float P_LIFT<f16_t> = 14.f;
 
-template <typename T, int HD>
-__global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 32) ? 1 : 2)) void attn_bwd_q(bigc_seq_attn a, BwdShape sh, float* row_data, const int2* ranges, float* by_dist) {
-    constexpr int DT = HD / 32, KEYS = BwdTile<T, HD>::KEYS, SUBS = KEYS / 32;
-    typedef Tile<T, HD, KEYS> TL;
-    constexpr int TILE = TL::BYTES, BUF = 2 * TILE;
+template <typename T, int HD, bool SPLIT>
+__global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 32) ? 1 : 2)) void attn_bwd_q(bigc_seq_attn a, BwdShape sh, float* row_data, const int2* ranges, float* by_dist) {
+    typedef BwdTile<T, HD, SPLIT, false> B;
+    typedef typename B::TL TL;
+    constexpr int DT = HD / 32, KEYS = B::ROWS, SUBS = B::SUBS, TILE = B::TILE, BUF = B::BUF;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int2 shared_docs[4];
     __shared__ int shared_bad[4];
@@ -144,13 +146,13 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 32) ? 1 : 
     if (a.causal) tile = sh.q_tiles - 1 - tile;                 // the longest first
     const int s = pair / a.n_head, head = pair % a.n_head, hk = head / (a.n_head / a.n_kv_head);
     const SeqSpan sp = seq_span(a, s);
-    const int first = tile * 128, nb = a.d_rel_table ? 2 * a.bias_radius + 1 : 0, nbins = nb ? nb + 2 * DIAG_PAD : 0;
+    const int first = tile * B::BLOCK_ROWS, nb = a.d_rel_table ? 2 * a.bias_radius + 1 : 0, nbins = nb ? nb + 2 * DIAG_PAD : 0;
     float* const out_bins = nb ? by_dist + ((long)(s * sh.q_tiles + tile) * a.n_head + head) * nb : nullptr;
     if (first >= sp.nq) {
-        for (int e = threadIdx.x; e < nb; e += 256) out_bins[e] = 0.f;
+        for (int e = threadIdx.x; e < nb; e += 64 * B::WAVES) out_bins[e] = 0.f;
         return;
     }
-    const int i0 = first + wave * 32, i = min(i0 + col, sp.nq - 1), shift = sp.nk - sp.nq, pos = i + shift;
+    const int i0 = first + (SPLIT ? 0 : wave * 32), i = min(i0 + col, sp.nq - 1), shift = sp.nk - sp.nq, pos = i + shift;
     const bool live = i0 + col < sp.nq, wave_live = i0 < sp.nq;
     const long row = sp.q0 + i;
     const ScoreRule rule(a, T());
@@ -161,14 +163,14 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 32) ? 1 : 
     me.prefix = prefix - pos; me.doc = 0; me.bias = 0;
     me.slope2 = rule.slopes ? a.slopes[head] * LOG2E : 0.f;
 
-    char* const docs_lds = lds + 2 * BUF;
-    float* const biases = (float*)(docs_lds + (a.q_doc ? 512 : 0));
+    char* const docs_lds = lds + B::STAGES;
+    float* const biases = (float*)(docs_lds + (a.q_doc ? B::SIDES : 0));
     float* const bins = biases + (rule.table ? 2 * a.bias_radius + 1 : 0) + wave * nbins;
     if (rule.table) load_biases(a, biases, head, 1);
     int doc_min = 0, doc_max = 0, block_doc_min = 0, block_doc_max = 0;
     if (a.q_doc) {
         me.doc = live ? a.q_doc[row] : -1;
-        doc_bounds(me.doc, live, wave, shared_docs, doc_min, doc_max, block_doc_min, block_doc_max);
+        doc_bounds(me.doc, live, wave, shared_docs, doc_min, doc_max, block_doc_min, block_doc_max, B::WAVES);
     }
     __syncthreads();
 
@@ -194,7 +196,7 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 32) ? 1 : 
     }
     delta += __shfl_xor(delta, 32);
     if (ml.y == 0.f) delta = 0.f;
-    if (live && hi == 0) {
+    if (live && hi == 0 && (!SPLIT || wave == 0)) {
         const long plane = a.n_q * a.n_head, at = head * a.n_q + row;
         row_data[at] = P_LIFT<T> - m; row_data[plane + at] = inv_l; row_data[2 * plane + at] = delta;
     }
@@ -204,22 +206,32 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 32) ? 1 : 
     list.end = (sp.nk + KEYS - 1) / KEYS;
     list.ahead = (prefix + KEYS - 1) / KEYS;
     list.first = max(0, tile_floor((long)first + shift + reach.lo, KEYS));
-    list.last = tile_floor((long)min(first + 127, sp.nq - 1) + shift + reach.hi, KEYS);
+    list.last = tile_floor((long)min(first + B::BLOCK_ROWS - 1, sp.nq - 1) + shift + reach.hi, KEYS);
     list.ranges = a.q_doc ? ranges + (long)s * ((a.max_k + 63) / 64) : nullptr;
-    list.per64 = 64 / KEYS; list.doc_min = block_doc_min; list.doc_max = block_doc_max;
+    list.per64 = 64 / KEYS; list.doc_min = block_doc_min; list.doc_max = block_doc_max; list.stride = SPLIT ? B::WAVES : 1;
+    list.wave_min = doc_min; list.wave_max = doc_max;
     const int p_min = min(i0, sp.nq - 1) + shift, p_max = min(i0 + 31, sp.nq - 1) + shift;
 
-    Stage<TL, 4> stage_k, stage_v;
-    stage_k.init(a.ldk, a.head_dim, wave);
-    stage_v.init(a.ldv, a.head_dim, wave);
+    const int sw = SPLIT ? 0 : wave;
+    Stage<TL, B::NW> stage_k, stage_v;
+    stage_k.init(a.ldk, a.head_dim, sw);
+    stage_v.init(a.ldv, a.head_dim, sw);
     const T* const k_rows = (const T*)a.k + sp.k0 * a.ldk + hk * a.hsk;
     const T* const v_rows = (const T*)a.v + sp.k0 * a.ldv + hk * a.hsv;
-    int* const docs = (int*)docs_lds;
+    char* const mine = lds + (SPLIT ? wave * B::NBUF * BUF : 0);
+    int* const docs = (int*)docs_lds + (SPLIT ? wave * B::NBUF * 64 : 0);
+    const auto arrived = [&] { if (SPLIT) wait_copies(); else wait_block(); };
     const auto copy_tile = [&](int k, int buf) {
-        stage_k.load(lds + buf * BUF, k_rows, k * KEYS, sp.nk, wave);
-        stage_v.load(lds + buf * BUF + TILE, v_rows, k * KEYS, sp.nk, wave);
-        if (a.q_doc && wave == 0)
+        stage_k.load(mine + buf * BUF, k_rows, k * KEYS, sp.nk, sw);
+        stage_v.load(mine + buf * BUF + TILE, v_rows, k * KEYS, sp.nk, sw);
+    };
+    const auto copy_side = [&](int k, int buf) {
+        if (a.q_doc && sw == 0)
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(a.k_doc + sp.k0 + min(k * KEYS + lane, sp.nk - 1)), LDS_PTR(void, docs + buf * 64), 4, 0, 0);
+    };
+    const auto finish_tile = [&](int buf) {
+        stage_k.finish(mine + buf * BUF, sw);
+        stage_v.finish(mine + buf * BUF + TILE, sw);
     };
     const int low = -a.bias_radius - DIAG_PAD;                  // d of the first bin
 
@@ -232,27 +244,29 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 32) ? 1 : 
         scale = GradScale<T>();
         below = above = 0.f;
         for (int e = lane; e < nbins; e += 64) bins[e] = 0.f;
-        int k = list.next(0), buf = 0;
-        const auto finish_tile = [&](int buf) { stage_k.finish(lds + buf * BUF, wave); stage_v.finish(lds + buf * BUF + TILE, wave); };
-        if (k < list.end) { copy_tile(k, 0); finish_tile(0); }
-        wait_block();
+        list.restart();
+        int k = list.next(SPLIT ? wave : 0), buf = 0;
+        bool whole = list.whole;
+        if (k < list.end) { copy_tile(k, 0); copy_side(k, 0); finish_tile(0); }
+        arrived();
         while (k < list.end) {
-            const int after = list.next(k + 1);
-            if (after < list.end) copy_tile(after, buf ^ 1);
-            const char* const kt = lds + buf * BUF;
+            const int after = list.next(k + list.stride), other = buf ^ 1;
+            const bool after_whole = list.whole;
+            if (after < list.end) {
+                copy_tile(after, other);
+                copy_side(after, other);
+            }
+            const char* const kt = mine + buf * BUF;
             const char* const vt = kt + TILE;
             if constexpr (careful) {
-                stage_k.clear_tail((char*)kt, wave);
-                stage_v.clear_tail((char*)vt, wave);
-                wait_block();
+                stage_k.clear_tail((char*)kt, sw);
+                stage_v.clear_tail((char*)vt, sw);
+                arrived();
             }
             const int kb = k * KEYS, ke = min(kb + KEYS, sp.nk), d_min = kb - p_max, d_max = kb + KEYS - 1 - p_min;
             const bool seen = wave_live && (kb < prefix || (d_max >= reach.lo && d_min <= reach.hi));
             bool full = kb + KEYS <= sp.nk && (ke <= prefix || (d_min >= reach.lo && d_max <= reach.hi));
-            if (a.q_doc && full) {
-                const int2 r = list.ranges[kb / 64];
-                full = __builtin_amdgcn_readfirstlane(r.x >= 0 && r.x == r.y && doc_min == r.x && doc_max == r.x);
-            }
+            full &= whole;
             if (seen) {
                 for (int u = 0; u < SUBS; ++u) {
                     f32x16 x, y, t;
@@ -283,30 +297,34 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 32) ? 1 : 
                     else accumulate<TL>(acc, kt, 32 * u, x);
                 }
             }
-            if (after < list.end) finish_tile(buf ^ 1);
-            wait_block();
-            k = after; buf ^= 1;
+            if (after < list.end) finish_tile(other);
+            arrived();
+            k = after; buf = other; whole = after_whole;
         }
     };
     pass(std::false_type());
     float check = 0.f;                                          // NaN or Inf: again, value by value (see attn_fwd)
     for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) check += acc[d][e] * 0.f;
-    if (any_wave(check != 0.f && live, wave, shared_bad)) pass(std::true_type());
+    if (SPLIT ? __ballot(check != 0.f && live) != 0 : any_wave(check != 0.f && live, wave, shared_bad)) pass(std::true_type());
     if (nb) {
         for (int w = 32; w; w >>= 1) { below += __shfl_xor(below, w); above += __shfl_xor(above, w); }
         if (lane == 0) { bins[0] += below; bins[nbins - 1] += above; }
         __syncthreads();
         const float* all = biases + nb;
-        for (int e = threadIdx.x; e < nb; e += 256) {           // waves in order; the bins beyond the radius belong to the two ends
+        for (int e = threadIdx.x; e < nb; e += 64 * B::WAVES) { // waves in order; the bins beyond the radius belong to the two ends
             float sum = 0.f;
             const int from = e == 0 ? 0 : e + DIAG_PAD, to = e == nb - 1 ? nbins : e + DIAG_PAD + 1;
-            for (int w = 0; w < 4; ++w)
+            for (int w = 0; w < B::WAVES; ++w)
                 for (int b = from; b < to; ++b) sum += all[w * nbins + b];
             out_bins[e] = sum;
         }
     }
-    if (!live) return;
     const float f = a.scale * scale.back() * (rule.cap ? CAP_SLOPE<T> : 1.f);
+    if constexpr (SPLIT) {
+        join_rows<T, B>(lds, acc, f, min(32, sp.nq - first), a.head_dim, (T*)a.dq + (sp.q0 + first) * a.lddq + head * a.hsdq, a.lddq);
+        return;
+    }
+    if (!live) return;
     for (int d = 0; d < DT; ++d)
         for (int g = 0; g < 4; ++g) {
             const int c = 32 * d + 8 * g + 4 * hi;
@@ -317,11 +335,11 @@ __global__ __launch_bounds__(256, (HD > 96 || (sizeof(T) == 4 && HD > 32) ? 1 : 
         }
 }
 
-template <typename T, int HD>
-__global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_bwd_kv(bigc_seq_attn a, BwdShape sh, const float* row_data, const int2* ranges) {
-    constexpr int DT = HD / 32, ROWS = BwdTile<T, HD>::ROWS, SUBS = ROWS / 32;
-    typedef Tile<T, HD, ROWS> TL;
-    constexpr int TILE = TL::BYTES, BUF = 2 * TILE;
+template <typename T, int HD, bool SPLIT>
+__global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) void attn_bwd_kv(bigc_seq_attn a, BwdShape sh, const float* row_data, const int2* ranges) {
+    typedef BwdTile<T, HD, SPLIT, true> B;
+    typedef typename B::TL TL;
+    constexpr int DT = HD / 32, ROWS = B::ROWS, SUBS = B::SUBS, TILE = B::TILE, BUF = B::BUF;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int2 shared_docs[4];
     __shared__ int shared_bad[4];
@@ -334,9 +352,9 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
     if (!bwd_place(sh.k_pairs, sh.k_tiles, pair, tile)) return;
     const int s = pair / a.n_kv_head, hk = pair % a.n_kv_head, group = a.n_head / a.n_kv_head;
     const SeqSpan sp = seq_span(a, s);
-    const int first = tile * 128;
+    const int first = tile * B::BLOCK_ROWS;
     if (first >= sp.nk) return;
-    const int j0 = first + wave * 32, j = min(j0 + col, sp.nk - 1), shift = sp.nk - sp.nq;
+    const int j0 = first + (SPLIT ? 0 : wave * 32), j = min(j0 + col, sp.nk - 1), shift = sp.nk - sp.nq;
     const bool live = j0 + col < sp.nk, wave_live = j0 < sp.nk;
     const long row = sp.k0 + j;
     const ScoreRule rule(a, T());
@@ -348,13 +366,16 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
     me.prefix = 0; me.doc = 0; me.bias = 0;
 
     // LDS: two buffers of Q and dO tiles; per buffer the rows' -m, 1 / l, delta and documents (64 places each); biases of a head
-    char* const side = lds + 2 * BUF;
-    float* const biases = (float*)(side + 2 * 4 * 256);
+    char* const mine = lds + (SPLIT ? wave * B::NBUF * BUF : 0);
+    char* const side = lds + B::STAGES + (SPLIT ? wave * B::NBUF * B::SIDE : 0);
+    float* const biases = (float*)(lds + B::STAGES + B::SIDES);
+    const auto arrived = [&] { if (SPLIT) wait_copies(); else wait_block(); };
     int doc_min = 0, doc_max = 0, block_doc_min = 0, block_doc_max = 0;
     if (a.q_doc) {
         me.doc = live ? a.k_doc[row] : -1;
-        doc_bounds(me.doc, live, wave, shared_docs, doc_min, doc_max, block_doc_min, block_doc_max);
+        doc_bounds(me.doc, live, wave, shared_docs, doc_min, doc_max, block_doc_min, block_doc_max, B::WAVES);
     }
+    if (SPLIT && rule.table) { load_biases(a, biases, hk * group, group); __syncthreads(); }
     typename Mat<T>::frag kf[TL::STEPS], vf[TL::STEPS];
     load_lane_rows<T, HD>(kf, (const T*)a.k + row * a.ldk + hk * a.hsk, live, a.head_dim);
     load_lane_rows<T, HD>(vf, (const T*)a.v + row * a.ldv + hk * a.hsv, live, a.head_dim);
@@ -364,14 +385,16 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
     list.end = (sp.nq + ROWS - 1) / ROWS;
     list.ahead = first < prefix ? list.end : 0;
     list.first = max(0, tile_floor((long)first - reach.hi - shift, ROWS));
-    list.last = tile_floor((long)min(first + 127, sp.nk - 1) - reach.lo - shift, ROWS);
+    list.last = tile_floor((long)min(first + B::BLOCK_ROWS - 1, sp.nk - 1) - reach.lo - shift, ROWS);
     list.ranges = a.q_doc ? ranges + (long)s * ((a.max_q + 63) / 64) : nullptr;
-    list.per64 = 64 / ROWS; list.doc_min = block_doc_min; list.doc_max = block_doc_max;
+    list.per64 = 64 / ROWS; list.doc_min = block_doc_min; list.doc_max = block_doc_max; list.stride = SPLIT ? B::WAVES : 1;
+    list.wave_min = doc_min; list.wave_max = doc_max;
     const int j_min = min(j0, sp.nk - 1), j_max = min(j0 + 31, sp.nk - 1);
     const long plane = a.n_q * a.n_head;
-    Stage<TL, 4> stage_q, stage_o;
-    stage_q.init(a.ldq, a.head_dim, wave);
-    stage_o.init(a.lddo, a.head_dim, wave);
+    const int sw = SPLIT ? 0 : wave;
+    Stage<TL, B::NW> stage_q, stage_o;
+    stage_q.init(a.ldq, a.head_dim, sw);
+    stage_o.init(a.lddo, a.head_dim, sw);
 
     f32x16 dk[DT], dv[DT];
     GradScale<T> scale;
@@ -382,42 +405,51 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
 #pragma unroll 1
         for (int head = hk * group; head < (hk + 1) * group; ++head) {
             me.slope2 = rule.slopes ? a.slopes[head] * LOG2E : 0.f;
-            if (rule.table) { __syncthreads(); load_biases(a, biases, head, 1); }          // (readable behind the first wait below)
+            if (SPLIT) me.bias = (head - hk * group) * (2 * a.bias_radius + 1);
+            else if (rule.table) { __syncthreads(); load_biases(a, biases, head, 1); }     // (readable behind the first wait below)
             const T* const q_rows = (const T*)a.q + sp.q0 * a.ldq + head * a.hsq;
             const T* const o_rows = (const T*)a.d_o + sp.q0 * a.lddo + head * a.hsdo;
             const auto copy_tile = [&](int k, int buf) {
-                stage_q.load(lds + buf * BUF, q_rows, k * ROWS, sp.nq, wave);
-                stage_o.load(lds + buf * BUF + TILE, o_rows, k * ROWS, sp.nq, wave);
-                const int at = min(k * ROWS + lane, sp.nq - 1);                            // one of -m, 1 / l, delta and the documents a wave
-                if (wave < 3 || a.q_doc) {
-                    const void* from = wave < 3 ? (const void*)(row_data + wave * plane + head * a.n_q + sp.q0 + at) : (const void*)(a.q_doc + sp.q0 + at);
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, LDS_PTR(void, side + (buf * 4 + wave) * 256), 4, 0, 0);
+                stage_q.load(mine + buf * BUF, q_rows, k * ROWS, sp.nq, sw);
+                stage_o.load(mine + buf * BUF + TILE, o_rows, k * ROWS, sp.nq, sw);
+            };
+            const auto copy_side = [&](int k, int buf) {
+                const int at = min(k * ROWS + lane, sp.nq - 1);                            // -m, 1 / l, delta and the documents, one a wave (SPLIT: all by each)
+                for (int what = SPLIT ? 0 : wave; what < (a.q_doc ? 4 : 3); what += SPLIT ? 1 : 4) {
+                    const void* from = what < 3 ? (const void*)(row_data + what * plane + head * a.n_q + sp.q0 + at) : (const void*)(a.q_doc + sp.q0 + at);
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, LDS_PTR(void, side + buf * B::SIDE + what * 256), 4, 0, 0);
                 }
             };
-            int k = list.next(0), buf = 0;
-            const auto finish_tile = [&](int buf) { stage_q.finish(lds + buf * BUF, wave); stage_o.finish(lds + buf * BUF + TILE, wave); };
-            if (k < list.end) { copy_tile(k, 0); finish_tile(0); }
-            wait_block();
+            const auto finish_tile = [&](int buf) {
+                stage_q.finish(mine + buf * BUF, sw);
+                stage_o.finish(mine + buf * BUF + TILE, sw);
+            };
+            list.restart();
+            int k = list.next(SPLIT ? (wave + head) % B::WAVES : 0), buf = 0;
+            bool whole = list.whole;
+            if (k < list.end) { copy_tile(k, 0); copy_side(k, 0); finish_tile(0); }
+            arrived();
             while (k < list.end) {
-                const int after = list.next(k + 1);
-                if (after < list.end) copy_tile(after, buf ^ 1);
-                const char* const qt = lds + buf * BUF;
+                const int after = list.next(k + list.stride), other = buf ^ 1;
+            const bool after_whole = list.whole;
+                if (after < list.end) {
+                    copy_tile(after, other);
+                    copy_side(after, other);
+                }
+                const char* const qt = mine + buf * BUF;
                 const char* const ot = qt + TILE;
                 if constexpr (careful) {
-                    stage_q.clear_tail((char*)qt, wave);
-                    stage_o.clear_tail((char*)ot, wave);
-                    wait_block();
+                    stage_q.clear_tail((char*)qt, sw);
+                    stage_o.clear_tail((char*)ot, sw);
+                    arrived();
                 }
                 const int ib = k * ROWS, p_min = ib + shift, p_max = ib + ROWS - 1 + shift, d_min = j_min - p_max, d_max = j_max - p_min;
                 const bool seen = wave_live && (j_min < prefix || (d_max >= reach.lo && d_min <= reach.hi));
                 bool full = ib + ROWS <= sp.nq && (j_max < prefix || (d_min >= reach.lo && d_max <= reach.hi));
-                if (a.q_doc && full) {
-                    const int2 r = list.ranges[ib / 64];
-                    full = __builtin_amdgcn_readfirstlane(r.x >= 0 && r.x == r.y && doc_min == r.x && doc_max == r.x);
-                }
+                full &= whole;
                 if (seen) {
                     for (int u = 0; u < SUBS; ++u) {
-                        const float* const rows = (const float*)(side + buf * 1024) + 32 * u + 4 * hi;
+                        const float* const rows = (const float*)(side + buf * B::SIDE) + 32 * u + 4 * hi;
                         f32x16 x, y, t;
                         for (int e = 0; e < 16; ++e) x[e] = y[e] = 0.f;
                         for (int c = 0; c < TL::STEPS; ++c) x = Mat<T>::mul(rows_frag<TL>(qt, 32 * u, c), kf[c], x);
@@ -447,18 +479,24 @@ __global__ __launch_bounds__(256, HD > 64 || sizeof(T) == 4 ? 1 : 2) void attn_b
                         else accumulate<TL>(dk, qt, 32 * u, x);
                     }
                 }
-                if (after < list.end) finish_tile(buf ^ 1);
-                wait_block();
-                k = after; buf ^= 1;
+                if (after < list.end) finish_tile(other);
+                arrived();
+                k = after; buf = other; whole = after_whole;
             }
         }
     };
     pass(std::false_type());
     float check = 0.f;
     for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) check += (dk[d][e] + dv[d][e]) * 0.f;
-    if (any_wave(check != 0.f && live, wave, shared_bad)) pass(std::true_type());
-    if (!live) return;
+    if (SPLIT ? __ballot(check != 0.f && live) != 0 : any_wave(check != 0.f && live, wave, shared_bad)) pass(std::true_type());
     const float unlift = P_LIFT<T> == 0.f ? 1.f : 1.f / 16384.f, f = a.scale * scale.back() * unlift * (rule.cap ? CAP_SLOPE<T> : 1.f);
+    if constexpr (SPLIT) {
+        const int n = min(32, sp.nk - first);
+        join_rows<T, B>(lds, dk, f, n, a.head_dim, (T*)a.dk + (sp.k0 + first) * a.lddk + hk * a.hsdk, a.lddk);
+        join_rows<T, B>(lds, dv, unlift, n, a.head_dim, (T*)a.dv + (sp.k0 + first) * a.lddv + hk * a.hsdv, a.lddv);
+        return;
+    }
+    if (!live) return;
     static_assert(P_LIFT<f16_t> == 14.f, "");
     for (int d = 0; d < DT; ++d)
         for (int g = 0; g < 4; ++g) {
@@ -502,12 +540,22 @@ __global__ __launch_bounds__(1024) void rel_table_grad(bigc_seq_attn a, const fl
 
 BwdShape bwd_shape(const bigc_seq_attn& a) {
     BwdShape sh = {};
-    const bool split = a.dtype == BIGC_F32;
-    const int nb = a.rel_table ? 2 * a.bias_radius + 1 : 0;
-    sh.q_tiles = cdiv(a.max_q, 128); sh.k_tiles = cdiv(a.max_k, 128);
+    const bool f32 = a.dtype == BIGC_F32;
+    const int nb = a.rel_table ? 2 * a.bias_radius + 1 : 0, hd = tile_dim(a.head_dim), group = a.n_head / a.n_kv_head;
     sh.q_pairs = a.n_seq * a.n_head; sh.k_pairs = a.n_seq * a.n_kv_head;
-    sh.q_lds = (size_t)4 * tile_bytes(a, split ? 32 : 64, split) + (a.q_doc ? 512 : 0) + sizeof(float) * (nb + (a.d_rel_table ? 4 * (nb + 2 * DIAG_PAD) : 0));
-    sh.k_lds = (size_t)4 * tile_bytes(a, !split && tile_dim(a.head_dim) <= 64 ? 64 : 32, split) + 2048 + sizeof(float) * nb;
+    // Blocks of 128 rows until they are fewer than two a CU; then of 32 (two packed rows of 4096, f16, 256 blocks of dk, dv: 210 us whole, 164 us split).  The dk, dv
+    // form keeps the biases of all heads of a group in LDS.
+    sh.q_split = !f32 && (long)sh.q_pairs * cdiv(a.max_q, 128) < 512;
+    sh.k_split = !f32 && (long)sh.k_pairs * cdiv(a.max_k, 128) < 512 && (long)group * nb <= 4096;
+    sh.q_tiles = cdiv(a.max_q, sh.q_split ? 32 : 128); sh.k_tiles = cdiv(a.max_k, sh.k_split ? 32 : 128);
+    sh.q_lds = (sh.q_split ? 4 * 2 * (2 * tile_bytes(a, 32, false) + (a.q_doc ? 256 : 0)) : 2 * (2 * tile_bytes(a, f32 ? 32 : 64, f32) + (a.q_doc ? 256 : 0)))
+             + sizeof(float) * (nb + (a.d_rel_table ? 4 * (nb + 2 * DIAG_PAD) : 0));
+    sh.k_lds = (sh.k_split ? 4 * 2 * (2 * tile_bytes(a, 32, false) + 1024) : 2 * (2 * tile_bytes(a, !f32 && hd <= 64 ? 64 : 32, f32) + 1024)) + sizeof(float) * nb * (sh.k_split ? group : 1);
+    // what does not fit with the bins of a wide bias goes whole
+    if (sh.q_lds > 160 * 1024 - 512 && sh.q_split) {
+        sh.q_split = 0; sh.q_tiles = cdiv(a.max_q, 128);
+        sh.q_lds = 2 * (2 * tile_bytes(a, f32 ? 32 : 64, f32) + (a.q_doc ? 256 : 0)) + sizeof(float) * (nb + (a.d_rel_table ? 4 * (nb + 2 * DIAG_PAD) : 0));
+    }
     sh.rows = 0;
     sh.q_ranges = round_up(sizeof(float) * 3 * (size_t)a.n_q * a.n_head, 256);
     sh.k_ranges = sh.q_ranges + (a.q_doc ? round_up(sizeof(int2) * (size_t)a.n_seq * ((a.max_q + 63) / 64), 256) : 0);
@@ -520,8 +568,17 @@ template <typename T, int HD>
 void launch_bwd(hipStream_t s, const bigc_seq_attn& a, const BwdShape& sh, char* ws) {
     float* rows = (float*)(ws + sh.rows);
     const long nq = (long)sh.q_pairs * sh.q_tiles, nk = (long)sh.k_pairs * sh.k_tiles;
-    if (nq && a.n_q) attn_bwd_q<T, HD><<<(unsigned)nq, 256, sh.q_lds, s>>>(a, sh, rows, (const int2*)(ws + sh.k_ranges), (float*)(ws + sh.bins));
-    if (nk && a.n_k) attn_bwd_kv<T, HD><<<(unsigned)nk, 256, sh.k_lds, s>>>(a, sh, rows, (const int2*)(ws + sh.q_ranges));
+    const int2 *kr = (const int2*)(ws + sh.k_ranges), *qr = (const int2*)(ws + sh.q_ranges);
+    float* bins = (float*)(ws + sh.bins);
+    constexpr bool CAN = sizeof(T) == 2;
+    if (nq && a.n_q) {
+        if (CAN && sh.q_split) attn_bwd_q<T, HD, CAN><<<(unsigned)nq, 256, sh.q_lds, s>>>(a, sh, rows, kr, bins);
+        else attn_bwd_q<T, HD, false><<<(unsigned)nq, 256, sh.q_lds, s>>>(a, sh, rows, kr, bins);
+    }
+    if (nk && a.n_k) {
+        if (CAN && sh.k_split) attn_bwd_kv<T, HD, CAN><<<(unsigned)nk, 256, sh.k_lds, s>>>(a, sh, rows, qr);
+        else attn_bwd_kv<T, HD, false><<<(unsigned)nk, 256, sh.k_lds, s>>>(a, sh, rows, qr);
+    }
 }
 template <typename T>
 void launch_bwd_dim(hipStream_t s, const bigc_seq_attn& a, const BwdShape& sh, char* ws) {

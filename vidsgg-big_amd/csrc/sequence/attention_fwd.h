@@ -4,6 +4,43 @@
 
 namespace {
 
+// The streamed tiles of a block (or of one of its waves): of those with the right remainder by the stride the ones before `ahead` or in [first, last] whose documents
+// the block has.  64 tiles' document ranges are looked at together and kept as bits, so that a step costs no trip to memory.
+struct TileList {
+    int end, ahead, first, last, stride;
+    const int2* ranges;                                         // by 64 rows, or null
+    int per64;                                                  // tiles of 64 rows
+    int doc_min, doc_max, wave_min, wave_max;                   // the block's documents; the wave's, -1 with padding
+    int base;                                                   // the tile that bit 0 stands for
+    unsigned long long some, one;                               // tiles to visit; those of the wave's only document throughout
+    bool whole;                                                 // of the tile found: nothing of it is another document's
+    __device__ __forceinline__ void restart() { base = -1; some = one = 0; whole = true; }
+    __device__ __forceinline__ int next(int k) {                // the first of k, k + stride, ... that is one
+        if (k >= ahead && k < first) k += (first - k + stride - 1) / stride * stride;
+        if (!ranges) return k >= end || (k >= ahead && k > last) ? end : k;
+        while (k < end) {
+            if (base < 0 || k >= base + 64 * stride) {
+                base = k;
+                const int c = k + (int)(threadIdx.x & 63) * stride;
+                const bool in = c < end && (c < ahead || (c >= first && c <= last));
+                const int2 r = in ? ranges[c / per64] : make_int2(0x7fffffff, -1);
+                some = __ballot(r.x <= doc_max && r.y >= doc_min);
+                one = __ballot(r.x >= 0 && r.x == r.y && r.x == wave_min && r.x == wave_max);
+            }
+            const int at = (k - base) / stride;
+            const unsigned long long m = some >> at;
+            if (m) {
+                const int f = (int)__builtin_ctzll(m);
+                whole = one >> (at + f) & 1;
+                return __builtin_amdgcn_readfirstlane(k + f * stride);
+            }
+            k = base + 64 * stride;
+        }
+        return end;
+    }
+};
+__device__ __forceinline__ int tile_floor(long row, int rows) { return row < 0 ? -1 : (int)min(row / rows, 0x3fffffffl); }
+
 // How a forward call is cut.  A tile's rows are (query, head) pairs of one key head: `pack` of a group's heads side by side, so that a key is read once
 // for all of them and a single token still fills rows.  many: four waves of 32 rows share every tile of keys; few (at most 32 rows in the
 // longest sequence): the four waves take the key tiles of the same 32 rows in turn, each through LDS of its own.
@@ -129,28 +166,15 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
     if (rule.table) __syncthreads();
 
     // the block's key tiles: of its chunk those in the prefix or in reach of any of its rows
-    const int tile_begin = at.split * sh.chunk / F::KEYS, tile_end = min((sp.nk + F::KEYS - 1) / F::KEYS, (at.split + 1) * (sh.chunk / F::KEYS));
-    const int prefix_tiles = (prefix + F::KEYS - 1) / F::KEYS;
-    const long reach_lo = (long)b_min + reach.lo, reach_hi = (long)b_max + reach.hi;
-    const int reach_first = reach_lo <= 0 ? 0 : (int)min(reach_lo / F::KEYS, 0x7fffffl * 64), reach_last = reach_hi < 0 ? -1 : (int)min(reach_hi / F::KEYS, 0x7fffffl * 64);
-    const int stride = FEW ? F::WAVES : 1;
-    const int range_tiles = (a.max_k + 63) / 64;
-    const auto next_tile = [&](int k) {                          // the first of k, k + stride, ... with something to see, or tile_end
-        if (k >= prefix_tiles && k < reach_first) k += (reach_first - k + stride - 1) / stride * stride;
-        if (!a.q_doc) return k >= tile_end || (k >= prefix_tiles && k > reach_last) ? tile_end : k;
-        while (k < tile_end) {
-            const int c = k + lane * stride;
-            bool ok = c < tile_end && (c < prefix_tiles || (c >= reach_first && c <= reach_last));
-            if (ok && a.q_doc) {
-                const int2 r = ranges[(long)s * range_tiles + c * F::KEYS / 64];
-                ok = r.x <= block_doc_max && r.y >= block_doc_min;
-            }
-            const unsigned long long m = __ballot(ok);
-            if (m) return k + (int)__builtin_ctzll(m) * stride;
-            k += 64 * stride;
-        }
-        return tile_end;
-    };
+    const int tile_begin = at.split * sh.chunk / F::KEYS;
+    TileList list;
+    list.end = min((sp.nk + F::KEYS - 1) / F::KEYS, (at.split + 1) * (sh.chunk / F::KEYS));
+    list.ahead = (prefix + F::KEYS - 1) / F::KEYS;
+    list.first = max(0, tile_floor((long)b_min + reach.lo, F::KEYS));
+    list.last = tile_floor((long)b_max + reach.hi, F::KEYS);
+    list.stride = FEW ? F::WAVES : 1;
+    list.ranges = a.q_doc ? ranges + (long)s * ((a.max_k + 63) / 64) : nullptr;
+    list.per64 = 64 / F::KEYS; list.doc_min = block_doc_min; list.doc_max = block_doc_max; list.wave_min = doc_min; list.wave_max = doc_max;
 
     typename Mat<T>::frag q[TL::STEPS];
     load_lane_rows<T, HD>(q, (const T*)a.q + row * a.ldq + head * a.hsq, live, a.head_dim);
@@ -181,12 +205,15 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
         constexpr bool careful = decltype(careful_)::value;
         for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
         m = -INFINITY; l = 0.f;
-        int k = __builtin_amdgcn_readfirstlane(next_tile(tile_begin + (FEW ? wave : 0))), buf = 0;
-        if (k < tile_end) { copy_tile(k, 0); finish_tile(0); }
+        list.restart();
+        int k = list.next(tile_begin + (FEW ? wave : 0)), buf = 0;
+        bool whole = list.whole;
+        if (k < list.end) { copy_tile(k, 0); finish_tile(0); }
         arrived();
-        while (k < tile_end) {
-            const int after = __builtin_amdgcn_readfirstlane(next_tile(k + stride));
-            if (after < tile_end) copy_tile(after, buf ^ 1);
+        while (k < list.end) {
+            const int after = list.next(k + list.stride);
+            const bool after_whole = list.whole;
+            if (after < list.end) copy_tile(after, buf ^ 1);
             const char* const kt = mine + buf * F::BUF;
             const char* const vt = kt + F::TILE;
             if constexpr (careful) {                             // products with the zeros behind head_dim stay zeros
@@ -198,10 +225,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
             const int d_min = kb - p_max, d_max = kb + F::KEYS - 1 - p_min;
             const bool seen = wave_live && (kb < prefix || (d_max >= reach.lo && d_min <= reach.hi));
             bool full = kb + F::KEYS <= sp.nk && (ke <= prefix || (d_min >= reach.lo && d_max <= reach.hi));
-            if (a.q_doc && full) {
-                const int2 r = ranges[(long)s * range_tiles + kb / 64];
-                full = __builtin_amdgcn_readfirstlane(r.x >= 0 && r.x == r.y && doc_min == r.x && doc_max == r.x);
-            }
+            full &= whole;
             if (seen) {
                 for (int u = 0; u < F::SUBS; ++u) {                 // 32 keys at a time
                     f32x16 x;
@@ -231,9 +255,9 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
                     else accumulate<TL>(acc, vt, 32 * u, x, PARTS);
                 }
             }
-            if (after < tile_end) finish_tile(buf ^ 1);
+            if (after < list.end) finish_tile(buf ^ 1);
             arrived();
-            k = after; buf ^= 1;
+            k = after; buf ^= 1; whole = after_whole;
         }
     };
     pass(std::false_type());
