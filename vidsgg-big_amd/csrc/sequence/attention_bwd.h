@@ -56,7 +56,7 @@ template <typename T, int HD, bool SPLIT, bool KV> struct BwdTile {
     static constexpr int PAD = 33, JOIN = WAVES * HD * PAD * 4;
     static_assert(!SPLIT || (JOIN <= STAGES && STAGES <= 140 * 1024), "");
 };
-constexpr int DIAG_PAD = 64;                                    // bins beyond the radius on both sides: a 32 x 32 that touches the radius reaches so far
+constexpr int DIAG_PAD = BIAS_PAD;                              // bins beyond the radius on both sides
 
 // the place of a block among `pairs` x `tiles`, tiles of a pair on one XCD (see fwd_place)
 __device__ __forceinline__ bool bwd_place(int pairs, int tiles, int& pair, int& tile) {
@@ -165,7 +165,8 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
 
     char* const docs_lds = lds + B::STAGES;
     float* const biases = (float*)(docs_lds + (a.q_doc ? B::SIDES : 0));
-    float* const bins = biases + (rule.table ? 2 * a.bias_radius + 1 : 0) + wave * nbins;
+    float* const all_bins = biases + (rule.table ? bias_entries(a) : 0);
+    float* const bins = all_bins + wave * nbins;
     if (rule.table) load_biases(a, biases, head, 1);
     int doc_min = 0, doc_max = 0, block_doc_min = 0, block_doc_max = 0;
     if (a.q_doc) {
@@ -310,12 +311,11 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
         for (int w = 32; w; w >>= 1) { below += __shfl_xor(below, w); above += __shfl_xor(above, w); }
         if (lane == 0) { bins[0] += below; bins[nbins - 1] += above; }
         __syncthreads();
-        const float* all = biases + nb;
         for (int e = threadIdx.x; e < nb; e += 64 * B::WAVES) { // waves in order; the bins beyond the radius belong to the two ends
             float sum = 0.f;
             const int from = e == 0 ? 0 : e + DIAG_PAD, to = e == nb - 1 ? nbins : e + DIAG_PAD + 1;
             for (int w = 0; w < B::WAVES; ++w)
-                for (int b = from; b < to; ++b) sum += all[w * nbins + b];
+                for (int b = from; b < to; ++b) sum += all_bins[w * nbins + b];
             out_bins[e] = sum;
         }
     }
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
 #pragma unroll 1
         for (int head = hk * group; head < (hk + 1) * group; ++head) {
             me.slope2 = rule.slopes ? a.slopes[head] * LOG2E : 0.f;
-            if (SPLIT) me.bias = (head - hk * group) * (2 * a.bias_radius + 1);
+            if (SPLIT) me.bias = (head - hk * group) * bias_entries(a);
             else if (rule.table) { __syncthreads(); load_biases(a, biases, head, 1); }     // (readable behind the first wait below)
             const T* const q_rows = (const T*)a.q + sp.q0 * a.ldq + head * a.hsq;
             const T* const o_rows = (const T*)a.d_o + sp.q0 * a.lddo + head * a.hsdo;
@@ -541,20 +541,20 @@ __global__ __launch_bounds__(1024) void rel_table_grad(bigc_seq_attn a, const fl
 BwdShape bwd_shape(const bigc_seq_attn& a) {
     BwdShape sh = {};
     const bool f32 = a.dtype == BIGC_F32;
-    const int nb = a.rel_table ? 2 * a.bias_radius + 1 : 0, hd = tile_dim(a.head_dim), group = a.n_head / a.n_kv_head;
+    const int nb = a.rel_table ? 2 * a.bias_radius + 1 : 0, be = a.rel_table ? bias_entries(a) : 0, hd = tile_dim(a.head_dim), group = a.n_head / a.n_kv_head;
     sh.q_pairs = a.n_seq * a.n_head; sh.k_pairs = a.n_seq * a.n_kv_head;
     // Blocks of 128 rows until they are fewer than two a CU; then of 32 (two packed rows of 4096, f16, 256 blocks of dk, dv: 210 us whole, 164 us split).  The dk, dv
     // form keeps the biases of all heads of a group in LDS.
     sh.q_split = !f32 && (long)sh.q_pairs * cdiv(a.max_q, 128) < 512;
-    sh.k_split = !f32 && (long)sh.k_pairs * cdiv(a.max_k, 128) < 512 && (long)group * nb <= 4096;
+    sh.k_split = !f32 && (long)sh.k_pairs * cdiv(a.max_k, 128) < 512 && (long)group * be <= 4096;
     sh.q_tiles = cdiv(a.max_q, sh.q_split ? 32 : 128); sh.k_tiles = cdiv(a.max_k, sh.k_split ? 32 : 128);
     sh.q_lds = (sh.q_split ? 4 * 2 * (2 * tile_bytes(a, 32, false) + (a.q_doc ? 256 : 0)) : 2 * (2 * tile_bytes(a, f32 ? 32 : 64, f32) + (a.q_doc ? 256 : 0)))
-             + sizeof(float) * (nb + (a.d_rel_table ? 4 * (nb + 2 * DIAG_PAD) : 0));
-    sh.k_lds = (sh.k_split ? 4 * 2 * (2 * tile_bytes(a, 32, false) + 1024) : 2 * (2 * tile_bytes(a, !f32 && hd <= 64 ? 64 : 32, f32) + 1024)) + sizeof(float) * nb * (sh.k_split ? group : 1);
+             + sizeof(float) * (be + (a.d_rel_table ? 4 * (nb + 2 * DIAG_PAD) : 0));
+    sh.k_lds = (sh.k_split ? 4 * 2 * (2 * tile_bytes(a, 32, false) + 1024) : 2 * (2 * tile_bytes(a, !f32 && hd <= 64 ? 64 : 32, f32) + 1024)) + sizeof(float) * be * (sh.k_split ? group : 1);
     // what does not fit with the bins of a wide bias goes whole
     if (sh.q_lds > 160 * 1024 - 512 && sh.q_split) {
         sh.q_split = 0; sh.q_tiles = cdiv(a.max_q, 128);
-        sh.q_lds = 2 * (2 * tile_bytes(a, f32 ? 32 : 64, f32) + (a.q_doc ? 256 : 0)) + sizeof(float) * (nb + (a.d_rel_table ? 4 * (nb + 2 * DIAG_PAD) : 0));
+        sh.q_lds = 2 * (2 * tile_bytes(a, f32 ? 32 : 64, f32) + (a.q_doc ? 256 : 0)) + sizeof(float) * (be + (a.d_rel_table ? 4 * (nb + 2 * DIAG_PAD) : 0));
     }
     sh.rows = 0;
     sh.q_ranges = round_up(sizeof(float) * 3 * (size_t)a.n_q * a.n_head, 256);

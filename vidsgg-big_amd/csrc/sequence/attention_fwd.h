@@ -143,7 +143,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
     me.prefix = prefix - pos;
     me.doc = 0;
     me.slope2 = rule.slopes ? a.slopes[head] * LOG2E : 0.f;
-    me.bias = (head - head0) * (2 * rule.radius + 1);
+    me.bias = (head - head0) * bias_entries(a);
 
     char* docs_lds = lds + F::STAGES;
     float* biases = (float*)(docs_lds + (a.q_doc ? F::DOCS : 0));
@@ -177,7 +177,6 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
     list.per64 = 64 / F::KEYS; list.doc_min = block_doc_min; list.doc_max = block_doc_max; list.wave_min = doc_min; list.wave_max = doc_max;
 
     typename Mat<T>::frag q[TL::STEPS];
-    load_lane_rows<T, HD>(q, (const T*)a.q + row * a.ldq + head * a.hsq, live, a.head_dim);
     Stage<TL, FEW ? 1 : F::WAVES> stage_k, stage_v;
     const int sw = FEW ? 0 : wave;
     stage_k.init(a.ldk, a.head_dim, sw);
@@ -208,7 +207,9 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
         list.restart();
         int k = list.next(tile_begin + (FEW ? wave : 0)), buf = 0;
         bool whole = list.whole;
-        if (k < list.end) { copy_tile(k, 0); finish_tile(0); }
+        if (k < list.end) copy_tile(k, 0);
+        if (!careful) load_lane_rows<T, HD>(q, (const T*)a.q + row * a.ldq + head * a.hsq, live, a.head_dim);       // (behind the first tile's copies)
+        if (k < list.end) finish_tile(0);
         arrived();
         while (k < list.end) {
             const int after = list.next(k + list.stride);
@@ -349,17 +350,31 @@ __global__ __launch_bounds__(256) void attn_join(bigc_seq_attn a, FwdShape sh, c
     if (i >= sp.nq) return;
     const long row = sp.q0 + i, rh = row * a.n_head + h, stride = a.n_q * a.n_head;
     const int n = max(1, (sp.nk + sh.chunk - 1) / sh.chunk);
-    float top = -INFINITY;
-    for (int k = 0; k < n; ++k) top = fmaxf(top, part_ml[k * stride + rh].x);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, o[2] = {0.f, 0.f};
-    for (int k = 0; k < n; ++k) {
-        const float2 ml = part_ml[k * stride + rh];
+    // 64 chunks at a time: their statistics by a lane each, then their sums with four loads on their way
+    float top = -INFINITY, sum = 0.f, o[2] = {0.f, 0.f};
+    for (int k0 = 0; k0 < n; k0 += 64) {
+        const int m = min(64, n - k0);
+        const float2 ml = lane < m ? part_ml[(k0 + lane) * stride + rh] : make_float2(-INFINITY, 0.f);
+        float now = ml.x;
+        for (int w = 32; w; w >>= 1) now = fmaxf(now, __shfl_xor(now, w));
+        now = fmaxf(now, top);
+        const float base = now == -INFINITY ? 0.f : now, old = __builtin_amdgcn_exp2f(top - base);
         const float f = __builtin_amdgcn_exp2f(ml.x - base);
-        if (f == 0.f && !isnan(ml.y)) continue;
-        sum += f * ml.y;
-        for (int t = 0; t < 2; ++t)
-            if (lane + 64 * t < a.head_dim) o[t] += f * part_o[(k * stride + rh) * a.head_dim + lane + 64 * t];
+        float l = f == 0.f && !isnan(ml.y) ? 0.f : f * ml.y;
+        for (int w = 32; w; w >>= 1) l += __shfl_xor(l, w);
+        sum = sum * old + l;
+        o[0] *= old; o[1] *= old;
+        top = now;
+        const bool none = f == 0.f && !isnan(ml.y);
+        const unsigned long long skip = __ballot(none);
+#pragma unroll 4
+        for (int k = 0; k < m; ++k) {
+            const float w = __shfl(f, k);
+            for (int t = 0; t < 2; ++t) {
+                const float x = lane + 64 * t < a.head_dim ? part_o[((k0 + k) * stride + rh) * a.head_dim + lane + 64 * t] : 0.f;
+                o[t] += skip >> k & 1 ? 0.f : w * x;
+            }
+        }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     for (int t = 0; t < 2; ++t) {
@@ -386,8 +401,8 @@ size_t round_up(size_t n, size_t m) { return (n + m - 1) / m * m; }
 
 FwdShape fwd_shape(const bigc_seq_attn& a) {
     FwdShape sh = {};
-    const int group = a.n_head / a.n_kv_head, nb = a.rel_table ? 2 * a.bias_radius + 1 : 0;
-    // heads packed in a tile: all of a group; with a bias by distance as many as have their biases in 4096 LDS entries (one head's may be 4095)
+    const int group = a.n_head / a.n_kv_head, nb = a.rel_table ? bias_entries(a) : 0;
+    // heads packed in a tile: all of a group; with a bias by distance as many as have their biases in 4096 LDS entries (one head's may be 4223)
     sh.pack = 1;
     for (int p = 1; p <= group; ++p)
         if (group % p == 0 && (long)p * nb <= 4096 && (long)p * a.max_q < (1l << 30)) sh.pack = p;
@@ -396,9 +411,9 @@ FwdShape fwd_shape(const bigc_seq_attn& a) {
     const int rows = sh.few ? 32 : 128, keys = sh.few || a.dtype == BIGC_F32 ? 32 : 64;
     sh.tiles = (int)(((long)a.max_q * sh.pack + rows - 1) / rows);
     sh.pairs = a.n_seq * a.n_kv_head * sh.sub;
-    // Keys a block takes.  While the row tiles alone do not give every CU its blocks (two; eight for few rows, where a block is a stream through memory and
-    // sequences differ in length), the keys are cut: to blocks of equal work over all sequences, none under 512 keys.
-    const long row_blocks = (long)sh.pairs * sh.tiles, want = sh.few ? 2048 : 512;
+    // Keys a block takes.  While the row tiles alone do not give every CU its blocks (two; four for few rows, where a block is a stream through memory and sequences differ
+    // in length: 48 tokens over caches of 1 to 16384, 8 key heads of 128: 377 us with four, 418 with eight, 471 with sixteen), the keys are cut: to blocks of equal work over all sequences, none under 512 keys.
+    const long row_blocks = (long)sh.pairs * sh.tiles, want = sh.few ? 1024 : 512;
     sh.chunk = (int)round_up(a.max_k > 0 ? a.max_k : 1, 64);
     if (row_blocks && row_blocks < want) {
         const long total = a.n_k < (long)a.n_seq * a.max_k ? a.n_k : (long)a.n_seq * a.max_k;        // keys of all sequences together, at most

@@ -360,11 +360,15 @@ struct LaneRow {
     int bias;                                                   // first entry of its head's biases by distance
 };
 
-// bias by distance of `heads` heads from h0 on, times log2 e: the lowest finite value stays finite (it hides nothing), -inf stays -inf
+// Bias by distance of `heads` heads from h0 on, times log2 e: the lowest finite value stays finite (it hides nothing), -inf stays -inf.  Beyond the radius the ends
+// go on for BIAS_PAD entries on both sides, as far as a 32 x 32 that touches the radius reaches: the registers' entries then lie at constants from the lane's.
+constexpr int BIAS_PAD = 64;
+__host__ __device__ __forceinline__ int bias_entries(const bigc_seq_attn& a) { return 2 * (a.bias_radius + BIAS_PAD) + 1; }
 __device__ __forceinline__ void load_biases(const bigc_seq_attn& a, float* biases, int h0, int heads) {
-    const int nb = 2 * a.bias_radius + 1;
+    const int nb = bias_entries(a), r = a.bias_radius;
     for (int e = threadIdx.x; e < heads * nb; e += blockDim.x) {
-        const float b = a.rel_table[(long)min(max(a.rel_map[e % nb], 0), a.n_bucket - 1) * a.n_head + h0 + e / nb];
+        const int at = min(max(e % nb - BIAS_PAD, 0), 2 * r);
+        const float b = a.rel_table[(long)min(max(a.rel_map[at], 0), a.n_bucket - 1) * a.n_head + h0 + e / nb];
         const float s = b * LOG2E;
         biases[e] = isinf(s) && !isinf(b) ? copysignf(3.402823466e38f, b) : s;
     }
@@ -384,7 +388,7 @@ __device__ __forceinline__ Linear make_scores(f32x16& x, f32x16* kept, const Sco
         if (KEEP) *kept = x;
     }
     Linear s = {r.a, r.c};
-    const float* const b = biases + l.bias + r.radius;
+    const float* const b = biases + l.bias + r.radius + BIAS_PAD;                          // of distance 0
     bool one_by_one = r.slopes || r.a == 0.f;
     const bool far = d_min >= r.radius || d_max <= -r.radius;
     if (r.table) {
@@ -404,7 +408,8 @@ __device__ __forceinline__ Linear make_scores(f32x16& x, f32x16* kept, const Sco
             const float v = *LDS_PTR(const float, b + (d_min >= r.radius ? r.radius : -r.radius));
             for (int e = 0; e < 16; ++e) x[e] += v;
         } else if (r.table) {
-            for (int e = 0; e < 16; ++e) x[e] += *LDS_PTR(const float, b + min(max(LANE_IS_QUERY ? d0 + reg_row(e) : d0 - reg_row(e), -r.radius), r.radius));
+            const float* const at = b + (LANE_IS_QUERY ? d0 : d0 - reg_row(15));
+            for (int e = 0; e < 16; ++e) x[e] += *LDS_PTR(const float, at + (LANE_IS_QUERY ? reg_row(e) : reg_row(15) - reg_row(e)));
         }
         s = {1.f, 0.f};
     }
