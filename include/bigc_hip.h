@@ -688,7 +688,8 @@ BIGC_API int bigc_linear_hr8out_f32(void* stream, const float* A, int lda, const
  * -- position biases, caps and masks on the scores, shared key heads, norms and rotations of the heads.  They stand next to
  * bigc_mha_core_f32 (no order, no masks, one key head per query head) and take IEEE f32, f16 and bfloat16 tensors; scores,
  * softmax statistics, sums and parameter gradients are f32 whatever the tensors' type.  (models/ has no caller of its own.)
- * Every row pointer, row stride and head stride has to be a multiple of 16 bytes (with one head its stride is not read), a row stride at most 2^22 elements.
+ * Every row pointer, row stride and head stride has to be a multiple of 16 bytes (with one head, or one row, its stride
+ * is not read), a row stride at most 2^22 elements.  Outputs overlap no input (but where it says so) and no other output.
  * ---------------------------------------------------------------------------------- */
 
 #define BIGC_F32 0
@@ -705,7 +706,7 @@ BIGC_API int bigc_linear_hr8out_f32(void* stream, const float* A, int lda, const
  *             ((!causal or d <= 0) and (window_left < 0 or -d <= window_left) and (window_right < 0 or d <= window_right)))
  *     o = softmax over the seen keys of the scores, times v
  * A query that sees no key (or only scores of -inf) has o = 0 and gives no gradient; what a hidden place holds (NaN, Inf) is never part of a
- * result.  A bias of -inf hides its distances, the lowest finite values (below -2.3e38, which count as one) do not.  slopes, rel_table + rel_map, prefix_len, q_doc + k_doc may be NULL.  Rows outside every sequence
+ * result (rows whose result is NaN or Inf are done twice, the second time value by value: such a call takes many times as long).  A bias of -inf hides its distances, the lowest finite values (below -2.3e38, which count as one) do not.  slopes, rel_table + rel_map, prefix_len, q_doc + k_doc may be NULL.  Rows outside every sequence
  * stay as they were.  Offsets are cut to [0, n_q] and [0, n_k] and lengths to max_q and max_k (which size the launch), map entries to the table. */
 typedef struct {
     int32_t dtype;                     /* BIGC_F32 / BIGC_F16 / BIGC_BF16: q, k, v, o, d_o, dq, dk, dv */

@@ -23,7 +23,7 @@ def attention(q, k, v, q_off, k_off, scale=None, softcap=0.0, slopes=None, rel_t
     """-> dict of float64 results: o, lse and, with d_o, dq, dk, dv, d_rel_table; under "tol_<name>" the bound of every element's error
     for a kernel that takes scores and sums in f32 and rounds P, dS and the results to a type of relative step ``half_eps`` (0: f32).
 
-    The bound: u = 2^-24.  A score is off by at most c = (hd + 16) u (1 + max sum |q_c k_c| scale + max |bias|) (a sum of hd products, the cap and
+    The bound: u = 2^-24.  A score is off by at most c = (hd + 16) u (1 + max sum |q_c k_c scale| + max |bias|) (a sum of hd products, the cap and
     the biases added in f32), P by 2 c + (L + 16) u of itself (numerator and denominator), so o by (that + half_eps / 2) sum P |v| and its own
     rounding; dP - delta by (hd + 16) u sum |dO| (|v| + |o|), and by sum |dO| times the error of the o that delta = dO . o is taken from, which for
     half types is one of P in two parts (half_eps^2 instead of half_eps); dS by P times that plus its own relative error; the gradients sum those.
@@ -59,7 +59,7 @@ def attention(q, k, v, q_off, k_off, scale=None, softcap=0.0, slopes=None, rel_t
             K = torch.where(seen[:, None], kd[e:f, hk], torch.zeros(())).requires_grad_(d_o is not None)
             V = torch.where(seen[:, None], vd[e:f, hk], torch.zeros(())).requires_grad_(d_o is not None)
             x = Q @ K.t() * scale
-            big = float((Q.detach().abs() @ K.detach().abs().t() * scale).max()) if f > e else 0.0
+            big = float((Q.detach().abs() @ K.detach().abs().t() * abs(scale)).max()) if f > e else 0.0
             if softcap > 0:
                 x = softcap * torch.tanh(x / softcap)
             if slopes is not None:

@@ -275,6 +275,88 @@ def test_repeats_bit_for_bit(t):
             assert torch.equal(a[n], b[n]), n
 
 
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-3])
+@pytest.mark.parametrize("cap", [0.0, 3.0])
+def test_scales(t, scale, cap):
+    """scores that fall with the product, and that do not depend on it, with and without masks and biases"""
+    Case(t, [(70, 70), (1, 200), (40, 90)], scale=scale, softcap=cap, causal=True).check()
+    Case(t, [(70, 70), (1, 200)], scale=scale, softcap=cap, rel_table=table(8, 2), rel_map=sequence.rel_bucket_map(8, 30)).check()
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("radius", [0, 1, 700, 1023])
+def test_bias_radius(t, radius):
+    """biases of one distance up to a thousand, in sequences shorter and longer than that"""
+    m = torch.randint(0, 5, (2 * radius + 1,), generator=torch.Generator().manual_seed(radius)).to(torch.int32)
+    Case(t, [(300, 300), (60, 900)], hd=32, rel_table=table(5, 2), rel_map=m, causal=True).check()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_bias_radius_at_its_limit(t):
+    m = torch.randint(0, 5, (4095,), generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    for hd in (64, 128):
+        Case(t, [(100, 100), (3, 700)], hd=hd, heads=(4, 2), rel_table=table(5, 4), rel_map=m).check()
+
+
+def test_a_wide_bias_gradient_of_wide_f32_heads_is_refused():
+    c = Case("f32", [(100, 100)], hd=128, rel_table=table(5, 2), rel_map=torch.zeros(4095, dtype=torch.int32))
+    c.check(train=False)
+    with pytest.raises(AssertionError, match="1023"):
+        c.run()
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+def test_many_blocks_and_few(t):
+    """enough rows for whole blocks of 128, and the same sequences among fewer"""
+    one = [(260, 260), (130, 200)]
+    Case(t, one * 30, heads=(10, 5), hd=32, causal=True, softcap=9.0).check()
+    Case(t, one, heads=(10, 5), hd=32, causal=True, softcap=9.0).check()
+
+
+def test_a_short_sequence_in_a_large_buffer():
+    """the workspace of a call goes by its sequences, not by the buffer they lie in"""
+    rows = 400000
+    g = torch.Generator().manual_seed(3)
+    q = torch.zeros(rows, 2, 64, dtype=torch.bfloat16, device=DEV)
+    k, v = (torch.randn(5000, 2, 64, generator=g).to(torch.bfloat16) for _ in range(2))
+    q[7] = torch.randn(2, 64, generator=g).to(torch.bfloat16).to(DEV)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    off = torch.tensor([7, 8], dtype=torch.int32, device=DEV)
+    out = torch.empty_like(q)
+    sequence.attend(q, k.to(DEV), v.to(DEV), off, torch.tensor([0, 5000], dtype=torch.int32, device=DEV), 1, 5000, out=out)
+    assert torch.cuda.max_memory_allocated() - before < q.numel() * 2 + 20e6
+    want = O.attention(q[7:8].cpu(), k, v, [0, 1], [0, 5000], half_eps=eps_of(torch.bfloat16))
+    near("o", out[7:8], want["o"], want["tol_o"])
+
+
+def test_one_row_of_any_row_stride():
+    x = torch.randn(3 * 128 + 5, device=DEV)
+    q = x[:128].as_strided((1, 2, 64), (131, 64, 1))
+    off = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    assert torch.equal(sequence.attend(q, q, q, off, off, 1, 1), q)
+
+
+def test_two_streams_at_once():
+    cases = [Case("bf16", [(300, 300), (1, 4000)], heads=(4, 2), seed=s, causal=True) for s in (1, 2)]
+    want = [c.run() for c in cases]
+    ins = [(c.args(DEV)[0], c.q_off.to(DEV), c.k_off.to(DEV)) for c in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cases], [[], []]
+    for _ in range(8):
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                (q, k, v, go), qo, ko = ins[i]
+                o, saved = sequence.attend(q, k, v, qo, ko, c.max_q, c.max_k, save=True, causal=True)
+                got[i].append((o,) + sequence.attend_bwd(saved, go)[:3])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            for a, n in zip(g, ("o", "dq", "dk", "dv")):
+                assert torch.equal(a, want[i][n])
+
+
 def test_offsets_beyond_32_bits():
     """a cache whose rows lie more than 2^32 elements apart"""
     ld = 1 << 17

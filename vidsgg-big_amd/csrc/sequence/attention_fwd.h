@@ -100,6 +100,11 @@ __global__ __launch_bounds__(256) void doc_ranges(bigc_seq_attn a, bool keys, in
     if ((threadIdx.x & 63) == 0) ranges[w] = make_int2(lo, hi);
 }
 
+// place of a chunk's result for query i of sequence s, head h
+__device__ __forceinline__ long part_row(const bigc_seq_attn& a, int split, int s, int i, int h) {
+    return (((long)split * a.n_seq + s) * a.max_q + i) * a.n_head + h;
+}
+
 // One pass over the keys with the running maximum m and sum l of every row:  o = sum 2^(s - m) v / l.
 //
 // A row's maximum is only moved when a score passes it by more than SLACK, so that the accumulators are rarely rescaled; p then lies in (0, 2^SLACK].
@@ -300,8 +305,9 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
             const int h = head0 + rt % sh.pack;
             const long rh = qrow * a.n_head + h;
             if (sh.splits > 1) {
-                part_o[((long)at.split * a.n_q * a.n_head + rh) * a.head_dim + c] = o;
-                if (c == 0) part_ml[(long)at.split * a.n_q * a.n_head + rh] = make_float2(top, sum);
+                const long part = part_row(a, at.split, s, rt / sh.pack, h);
+                part_o[part * a.head_dim + c] = o;
+                if (c == 0) part_ml[part] = make_float2(top, sum);
             } else {
                 o *= sum == 0.f ? 0.f : 1.f / sum;
                 ((T*)a.o)[qrow * a.ldo + h * a.hso + c] = (T)o;
@@ -314,13 +320,14 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
     if (!live) return;
     const long rh = row * a.n_head + head;
     if (sh.splits > 1) {
-        float* o = part_o + ((long)at.split * a.n_q * a.n_head + rh) * a.head_dim;
+        const long part = part_row(a, at.split, s, i, head);
+        float* o = part_o + part * a.head_dim;
         for (int d = 0; d < DT; ++d)
             for (int g = 0; g < 4; ++g) {
                 const int c = 32 * d + 8 * g + 4 * hi;
                 if (c < a.head_dim) *(float4*)(o + c) = make_float4(acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]);
             }
-        if (hi == 0) part_ml[(long)at.split * a.n_q * a.n_head + rh] = make_float2(m, l);
+        if (hi == 0) part_ml[part] = make_float2(m, l);
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -348,13 +355,13 @@ __global__ __launch_bounds__(256) void attn_join(bigc_seq_attn a, FwdShape sh, c
     const int s = (int)(r / a.max_q), i = (int)(r % a.max_q);
     const SeqSpan sp = seq_span(a, s);
     if (i >= sp.nq) return;
-    const long row = sp.q0 + i, rh = row * a.n_head + h, stride = a.n_q * a.n_head;
+    const long row = sp.q0 + i, rh = row * a.n_head + h, part = part_row(a, 0, s, i, h), stride = part_row(a, 1, 0, 0, 0);
     const int n = max(1, (sp.nk + sh.chunk - 1) / sh.chunk);
     // 64 chunks at a time: their statistics by a lane each, then their sums with four loads on their way
     float top = -INFINITY, sum = 0.f, o[2] = {0.f, 0.f};
     for (int k0 = 0; k0 < n; k0 += 64) {
         const int m = min(64, n - k0);
-        const float2 ml = lane < m ? part_ml[(k0 + lane) * stride + rh] : make_float2(-INFINITY, 0.f);
+        const float2 ml = lane < m ? part_ml[(k0 + lane) * stride + part] : make_float2(-INFINITY, 0.f);
         float now = ml.x;
         for (int w = 32; w; w >>= 1) now = fmaxf(now, __shfl_xor(now, w));
         now = fmaxf(now, top);
@@ -371,7 +378,7 @@ __global__ __launch_bounds__(256) void attn_join(bigc_seq_attn a, FwdShape sh, c
         for (int k = 0; k < m; ++k) {
             const float w = __shfl(f, k);
             for (int t = 0; t < 2; ++t) {
-                const float x = lane + 64 * t < a.head_dim ? part_o[((k0 + k) * stride + rh) * a.head_dim + lane + 64 * t] : 0.f;
+                const float x = lane + 64 * t < a.head_dim ? part_o[((k0 + k) * stride + part) * a.head_dim + lane + 64 * t] : 0.f;
                 o[t] += skip >> k & 1 ? 0.f : w * x;
             }
         }
@@ -427,8 +434,8 @@ FwdShape fwd_shape(const bigc_seq_attn& a) {
     const int tile = tile_bytes(a, keys, a.dtype == BIGC_F32 && !sh.few), row = tile_dim(a.head_dim) * seq_size(a.dtype);
     sh.lds = (size_t)(!sh.few ? 1 : row > 256 ? 2 : 4) * (4 * tile + (a.q_doc ? 512 : 0)) + sizeof(float) * sh.pack * nb;
     sh.part_o = a.q_doc ? round_up(sizeof(int2) * (size_t)a.n_seq * ((a.max_k + 63) / 64), 256) : 0;
-    sh.part_ml = sh.part_o + (sh.splits > 1 ? round_up(sizeof(float) * (size_t)sh.splits * a.n_q * a.n_head * a.head_dim, 256) : 0);
-    sh.total = sh.part_ml + (sh.splits > 1 ? round_up(sizeof(float2) * (size_t)sh.splits * a.n_q * a.n_head, 256) : 0);
+    sh.part_ml = sh.part_o + (sh.splits > 1 ? round_up(sizeof(float) * (size_t)sh.splits * a.n_seq * a.max_q * a.n_head * a.head_dim, 256) : 0);
+    sh.total = sh.part_ml + (sh.splits > 1 ? round_up(sizeof(float2) * (size_t)sh.splits * a.n_seq * a.max_q * a.n_head, 256) : 0);
     return sh;
 }
 

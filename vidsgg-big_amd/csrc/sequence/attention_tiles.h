@@ -64,14 +64,21 @@ __device__ __forceinline__ void split_pair(float a, float b, unsigned& h, unsign
     m = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), BOTH);
     l = __builtin_amdgcn_perm(__float_as_uint(sb), __float_as_uint(sa), BOTH);
 }
-// the same where values may be Inf or NaN, which are their own first part
-__device__ __forceinline__ void split_pair_any(float a, float b, unsigned& h, unsigned& m, unsigned& l) {
-    split_pair(a, b, h, m, l);
-    const unsigned keep = (isfinite(a) ? 0xffffu : 0u) | (isfinite(b) ? 0xffff0000u : 0u);
-    m &= keep;
-    l &= keep;
-    if (isnan(a)) h |= 0x40u;
-    if (isnan(b)) h |= 0x400000u;
+// The same for four values that may be Inf or NaN, which are their own first part: looked for at a fourth of the cost of taking care of them
+__device__ __forceinline__ void split_four(f32x4 v, unsigned* h, unsigned* m, unsigned* l) {
+    split_pair(v.x, v.y, h[0], m[0], l[0]);
+    split_pair(v.z, v.w, h[1], m[1], l[1]);
+    const float odd = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, v.w * 0.f)));
+    if (__ballot(odd != 0.f)) {
+        for (int p = 0; p < 2; ++p) {
+            const float a = v[2 * p], b = v[2 * p + 1];
+            const unsigned keep = (isfinite(a) ? 0xffffu : 0u) | (isfinite(b) ? 0xffff0000u : 0u);
+            m[p] &= keep;
+            l[p] &= keep;
+            if (isnan(a)) h[p] |= 0x40u;
+            if (isnan(b)) h[p] |= 0x400000u;
+        }
+    }
 }
 template <> struct Mat<f32s> {
     typedef Parts frag;
@@ -210,10 +217,9 @@ __device__ __forceinline__ void load_lane_rows(typename Mat<T>::frag* f, const T
     if constexpr (std::is_same<T, f32s>::value) {
         for (int s = 0; s < HD / 16; ++s) {
             const int c = 16 * s + 8 * hi;
-            union { f32x4 v[2]; float x[8]; } u;
-            for (int q = 0; q < 2; ++q) u.v[q] = live && c < hd ? *(const f32x4*)((const float*)row + c + 4 * q) : f32x4{0.f, 0.f, 0.f, 0.f};
             union { unsigned w[4]; bf16x8 f; } h, m, l;
-            for (int e = 0; e < 4; ++e) split_pair_any(u.x[2 * e], u.x[2 * e + 1], h.w[e], m.w[e], l.w[e]);
+            for (int q = 0; q < 2; ++q)
+                split_four(live && c < hd ? *(const f32x4*)((const float*)row + c + 4 * q) : f32x4{0.f, 0.f, 0.f, 0.f}, h.w + 2 * q, m.w + 2 * q, l.w + 2 * q);
             f[s] = {h.f, m.f, l.f};
         }
         return;
@@ -292,7 +298,7 @@ struct Stage<Tile<f32s, HD, ROWS>, NW> {
         typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
         for (int i = 0; i < N; ++i) {
             unsigned h[2], m[2], l[2];
-            for (int q = 0; q < 2; ++q) split_pair_any(v[i][2 * q], v[i][2 * q + 1], h[q], m[q], l[q]);
+            split_four(v[i], h, m, l);
             char* const at = tile + P::place(row_of(i, wave), 0) + col_of(i, wave) * 2;
             *LDS_PTR(u32x2, at) = u32x2{h[0], h[1]};
             *LDS_PTR(u32x2, at + P::BYTES) = u32x2{m[0], m[1]};
