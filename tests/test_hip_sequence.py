@@ -335,7 +335,33 @@ def test_one_row_of_any_row_stride():
     x = torch.randn(3 * 128 + 5, device=DEV)
     q = x[:128].as_strided((1, 2, 64), (131, 64, 1))
     off = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
-    assert torch.equal(sequence.attend(q, q, q, off, off, 1, 1), q)
+    # one key: o = (p v) (1 / p) with p = 2^r and r what fma(s, c, -m) leaves of m's rounding: three roundings of half a step, 2^-24 of the value each
+    assert ((sequence.attend(q, q, q, off, off, 1, 1) - q).abs() <= 3.01 * 2.0 ** -24 * q.abs()).all()
+
+
+@pytest.mark.parametrize("hd", [32, 64])
+@pytest.mark.parametrize("t", sorted(TYPES))
+def test_the_tables_gradient_has_no_errors_of_one_sign(t, hd):
+    """Over a whole row dS sums to nothing, so that the far bucket's gradient is a small difference of large sums: an error of every dP to one side, however small, adds
+    up over rows and keys.  o takes one rounding (2^-25 at most, at random) for each of its 63 tiles and dP a few: sqrt(63) 2^-25 < 2^-22 each of |d_o| |o| in a
+    row's sum, 2^-21 together, and rows add up as the root of their squares; what the near buckets have of their own is f32 rounding, 2^-21 of the table."""
+    n, h = 2000, 4
+    g = torch.Generator().manual_seed(hd)
+    q, k, v, go = [torch.randn(n, h, hd, generator=g).to(TYPES[t]).to(DEV) for _ in range(4)]
+    table = (0.5 * torch.randn(16, h, generator=g)).to(DEV)
+    bucket = sequence.rel_bucket_map(16, 64).to(DEV)
+    off = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    _, saved = sequence.attend(q, k, v, off, off, n, n, rel_table=table, rel_map=bucket, save=True)
+    got = sequence.attend_bwd(saved, go)[3].double()
+    q, k, v, go = [x.double().transpose(0, 1).contiguous() for x in (q, k, v, go)]
+    place = torch.arange(n, device=DEV)
+    at = bucket.long()[(place[None] - place[:, None]).clamp(-64, 64) + 64]
+    p = torch.softmax(torch.bmm(q, k.transpose(1, 2).contiguous()) * hd ** -0.5 + table.double().T[:, at], -1)
+    dp = torch.bmm(go, v.transpose(1, 2).contiguous())
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    want = torch.stack([torch.zeros(16, dtype=torch.float64, device=DEV).index_add_(0, at.flatten(), x.flatten()) for x in ds], 1)
+    rows = (go.norm(dim=-1) * torch.bmm(p, v).norm(dim=-1)).norm()
+    assert (got - want).norm() <= 2.0 ** -21 * (rows + want.norm())
 
 
 def test_two_streams_at_once():

@@ -4,6 +4,10 @@
 //   dq:     lanes are queries.  S = K q, dP = V dO, dS = P (dP - delta), dq += K^T dS; the sums of dS along the diagonals of equal distance (the
 //           bias table's gradient); first the rows' delta = dO . o, which it also leaves, with m and 1 / l, for the other kernel.
 //   dk, dv: lanes are keys.  S = Q k, dP = dO v, dv += dO^T P, dk += Q^T dS, over all query heads of the key head.
+//
+// Bound by vector instructions and the matrix instructions between them (16 heads of 64 with a learned bias over sequences of up to 2048 rows, bf16: dq and
+// the diagonals' sums 228 us, dk and dv 212, the forward before them 197); with few sequences by the longest one's own chain of tiles (two packed rows of
+// 4096 of documents, f16: 93 and 150 us, the forward 78).
 #pragma once
 #include "attention_fwd.h"
 
@@ -182,26 +186,33 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
     const long rh = row * a.n_head + head;
     const float2 ml = live ? *(const float2*)(a.stats + 2 * rh) : make_float2(0.f, 0.f);
     const float m = ml.x == -INFINITY ? 0.f : ml.x, inv_l = ml.y == 0.f ? 0.f : 1.f / ml.y;
-    float delta = 0.f;
+    double total = 0.;                                          // (the table's gradient adds delta's error up over all keys)
     if (a.o32) {
         for (int c = 0; c < TL::STEPS; ++c)
             for (int e = 0; e < TL::E; ++e) {
                 const int at = (2 * c + hi) * TL::E + e;
-                if (live && at < a.head_dim) delta += (float)go[c][e] * a.o32[rh * a.head_dim + at];
+                if (live && at < a.head_dim) total += (double)(float)go[c][e] * a.o32[rh * a.head_dim + at];
             }
     } else {
         typename Mat<T>::frag o[TL::STEPS];
         load_lane_rows<T, HD>(o, (const T*)a.o + row * a.ldo + head * a.hso, live, a.head_dim);
         for (int c = 0; c < TL::STEPS; ++c)
-            for (int e = 0; e < TL::E; ++e) delta += (float)go[c][e] * (float)o[c][e];
+            for (int e = 0; e < TL::E; ++e) total += (double)(float)go[c][e] * (float)o[c][e];
     }
-    delta += __shfl_xor(delta, 32);
+    total += __shfl_xor(total, 32);
+    float delta = (float)total;
     if (ml.y == 0.f) delta = 0.f;
     if (live && hi == 0 && (!SPLIT || wave == 0)) {
         const long plane = a.n_q * a.n_head, at = head * a.n_q + row;
         row_data[at] = P_LIFT<T> - m; row_data[plane + at] = inv_l; row_data[2 * plane + at] = delta;
     }
     const float minus = -delta * inv_l;                         // dS = p (dP / l - delta / l)
+    // Every other row's dP is taken negated: the matrix instructions cut off a sum's last bits downwards, and the table's gradient, which adds such errors up over all rows
+    // and keys where dP - delta itself cancels, would have them all with one sign (2000 keys of 32 columns, 64 of
+    // them near: f32 12e-6 of the table with one sign, 0.7e-6 with both; f16 1.9e-6 and 0.4e-6).
+    const bool odd = col & 1;
+    const float sign_l = odd ? -inv_l : inv_l;
+    if (odd) for (int c = 0; c < TL::STEPS; ++c) go[c] = -go[c];
 
     TileList list;
     list.end = (sp.nk + KEYS - 1) / KEYS;
@@ -272,14 +283,14 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
                 for (int u = 0; u < SUBS; ++u) {
                     f32x16 x, y, t;
                     for (int e = 0; e < 16; ++e) x[e] = y[e] = 0.f;
-                    for (int c = 0; c < TL::STEPS; ++c) x = Mat<T>::mul(rows_frag<TL>(kt, 32 * u, c), q[c], x);
-                    for (int c = 0; c < TL::STEPS; ++c) y = Mat<T>::mul(rows_frag<TL>(vt, 32 * u, c), go[c], y);
+                    add_products<TL>(x, kt, 32 * u, q);
+                    add_products<TL>(y, vt, 32 * u, go);
                     const int d0 = kb + 32 * u + 4 * hi - pos;
                     const Linear sc = make_scores<T, true, true>(x, &t, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (SUBS - 1 - u));
                     if (!full) hide_scores<true>(x, sc, me, d0, a.q_doc ? docs + buf * 64 + 32 * u + 4 * hi : nullptr);
                     const float base = sc.c - m;
                     for (int e = 0; e < 16; ++e) {              // rows that are not there: 0 (1 / l is 0)
-                        const float p = __builtin_amdgcn_exp2f(fmaf(x[e], sc.a, base)), ds = p * fmaf(y[e], inv_l, minus);
+                        const float p = __builtin_amdgcn_exp2f(fmaf(x[e], sc.a, base)), ds = p * fmaf(y[e], sign_l, minus);
                         x[e] = careful && p == 0.f ? 0.f : ds;
                     }
                     if (nb) {
@@ -452,8 +463,8 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
                         const float* const rows = (const float*)(side + buf * B::SIDE) + 32 * u + 4 * hi;
                         f32x16 x, y, t;
                         for (int e = 0; e < 16; ++e) x[e] = y[e] = 0.f;
-                        for (int c = 0; c < TL::STEPS; ++c) x = Mat<T>::mul(rows_frag<TL>(qt, 32 * u, c), kf[c], x);
-                        for (int c = 0; c < TL::STEPS; ++c) y = Mat<T>::mul(rows_frag<TL>(ot, 32 * u, c), vf[c], y);
+                        add_products<TL>(x, qt, 32 * u, kf);
+                        add_products<TL>(y, ot, 32 * u, vf);
                         const int d0 = j - shift - ib - 32 * u - 4 * hi;
                         const Linear sc = make_scores<T, false, true>(x, &t, rule, me, biases, d0, d_min + 32 * (SUBS - 1 - u), d_max - 32 * u);
                         if (!full) hide_scores<false>(x, sc, me, d0, a.q_doc ? (const int*)rows + 192 : nullptr);
@@ -543,7 +554,7 @@ BwdShape bwd_shape(const bigc_seq_attn& a) {
     const bool f32 = a.dtype == BIGC_F32;
     const int nb = a.rel_table ? 2 * a.bias_radius + 1 : 0, be = a.rel_table ? bias_entries(a) : 0, hd = tile_dim(a.head_dim), group = a.n_head / a.n_kv_head;
     sh.q_pairs = a.n_seq * a.n_head; sh.k_pairs = a.n_seq * a.n_kv_head;
-    // Blocks of 128 rows until they are fewer than two a CU; then of 32 (two packed rows of 4096, f16, 256 blocks of dk, dv: 210 us whole, 164 us split).  The dk, dv
+    // Blocks of 128 rows until they are fewer than two a CU; then of 32 (two packed rows of 4096, f16, 256 blocks of dk, dv: 210 us whole, 150 us split).  The dk, dv
     // form keeps the biases of all heads of a group in LDS.
     sh.q_split = !f32 && (long)sh.q_pairs * cdiv(a.max_q, 128) < 512;
     sh.k_split = !f32 && (long)sh.k_pairs * cdiv(a.max_k, 128) < 512 && (long)group * be <= 4096;

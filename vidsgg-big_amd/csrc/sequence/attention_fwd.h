@@ -107,10 +107,16 @@ __device__ __forceinline__ long part_row(const bigc_seq_attn& a, int split, int 
 
 // One pass over the keys with the running maximum m and sum l of every row:  o = sum 2^(s - m) v / l.
 //
-// A row's maximum is only moved when a score passes it by more than SLACK, so that the accumulators are rarely rescaled; p then lies in (0, 2^SLACK].
+// A row's maximum is only moved when a score passes it by more than SLACK, so that the accumulators are rarely rescaled (and p is what the backward's will be,
+// bit for bit: next to another maximum the exponent is rounded differently); p then lies in (0, 2^SLACK].
+// Bound: few rows over long caches by memory (48 tokens over caches of 1 to 16384, 8 key heads of 128, bf16: 371 us for 1.75 GB, 4.7 TB/s of the 5.1 that a
+// copy reaches); many rows by vector instructions beside the matrix instructions (some ten a score of 2 head_dim x 2 flops; of a SIMD's cycles about half
+// issue those and a quarter of them feed the matrix unit, the two adding up rather than overlapping): 8192 causal rows, 32 + 8 heads of 128, bf16: 785 us, 700
+// TFLOP/s.
+//
 // p is rounded to the tensors' type for its product with v (the one rounding inside; sums and statistics are f32 before it).  f16 ends at 2^-14, so that its p is
 // scaled by 2^LIFT (o32, which the exact gradient of the bias table is taken from, has p in two parts): with 2^(SLACK + LIFT) the largest, values down to 2^-39 of the row's largest still arrive.
-template <typename T> constexpr float SLACK = sizeof(T) == 4 ? 0.f : 8.f;
+template <typename T> constexpr float SLACK = 8.f;
 template <> constexpr float SLACK<f16_t> = 4.f;
 template <typename T> constexpr float LIFT = 0.f;
 template <> constexpr float LIFT<f16_t> = 11.f;
@@ -236,7 +242,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
                 for (int u = 0; u < F::SUBS; ++u) {                 // 32 keys at a time
                     f32x16 x;
                     for (int e = 0; e < 16; ++e) x[e] = 0.f;
-                    for (int c = 0; c < TL::STEPS; ++c) x = Mat<T>::mul(rows_frag<TL>(kt, 32 * u, c), q[c], x);
+                    add_products<TL>(x, kt, 32 * u, q);
                     const int d0 = kb + 32 * u + 4 * hi - pos;
                     const Linear s = make_scores<T, true, false>(x, nullptr, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (F::SUBS - 1 - u));
                     if (!full) hide_scores<true>(x, s, me, d0, a.q_doc ? my_docs + buf * 64 + 32 * u + 4 * hi : nullptr);
@@ -419,7 +425,8 @@ FwdShape fwd_shape(const bigc_seq_attn& a) {
     sh.tiles = (int)(((long)a.max_q * sh.pack + rows - 1) / rows);
     sh.pairs = a.n_seq * a.n_kv_head * sh.sub;
     // Keys a block takes.  While the row tiles alone do not give every CU its blocks (two; four for few rows, where a block is a stream through memory and sequences differ
-    // in length: 48 tokens over caches of 1 to 16384, 8 key heads of 128: 377 us with four, 418 with eight, 471 with sixteen), the keys are cut: to blocks of equal work over all sequences, none under 512 keys.
+    // in length: 48 tokens over caches of 1 to 16384, 8 key heads of 128: 377 us with four, 418 with eight, 471 with sixteen), the keys are cut: to blocks of
+    // equal work over all sequences, none under 512 keys.
     const long row_blocks = (long)sh.pairs * sh.tiles, want = sh.few ? 1024 : 512;
     sh.chunk = (int)round_up(a.max_k > 0 ? a.max_k : 1, 64);
     if (row_blocks && row_blocks < want) {
@@ -440,19 +447,22 @@ FwdShape fwd_shape(const bigc_seq_attn& a) {
 }
 
 // p in as many parts as the use of o32 needs, which the backward takes delta from: two, or for the f32 gradient of a bias table what adds up to f32's bits
+// (f32s: products from zero for every 32 keys, see accumulate).  Two also for few rows whose keys are not cut (about 512 at most): the roundings of p do not average out over few
+// keys (an f16 token over 257 keys: 1.3 - 1.5 times the error of o's own rounding with one part, 1.0 with two), and the time is the launch's; over long caches
+// they do (1.1 - 1.4), and two parts cost 376 -> 386 us (48 tokens).
 template <typename T, int HD>
 void launch_fwd(hipStream_t s, const bigc_seq_attn& a, const FwdShape& sh, const int2* ranges, float* part_o, float2* part_ml) {
     const int threads = sh.few ? 64 * FwdTile<T, HD, true>::WAVES : 256;
     // (f32: few rows wait for memory, which is then copied as it is; many for the products, which then run on its parts)
     typedef typename std::conditional<std::is_same<T, float>::value, f32s, T>::type Many;
 #define LAUNCH(PARTS) do { \
-        if (sh.few) attn_fwd<T, HD, true, PARTS><<<(unsigned)sh.blocks, threads, sh.lds, s>>>(a, sh, ranges, part_o, part_ml); \
+        if (sh.few) attn_fwd<T, HD, true, (sizeof(T) == 4 ? 1 : PARTS)><<<(unsigned)sh.blocks, threads, sh.lds, s>>>(a, sh, ranges, part_o, part_ml); \
         else attn_fwd<Many, HD, false, PARTS><<<(unsigned)sh.blocks, threads, sh.lds, s>>>(a, sh, ranges, part_o, part_ml); \
     } while (0)
-    if constexpr (sizeof(T) == 4) { LAUNCH(1); return; }
+    if constexpr (sizeof(T) == 4) { LAUNCH(2); return; }
     else {
-        if (!a.o32) LAUNCH(1);
-        else if (std::is_same<T, bf16_t>::value && a.rel_table) LAUNCH((std::is_same<T, bf16_t>::value ? 3 : 2));
+        if (!a.o32 && !(sh.few && sh.splits == 1)) LAUNCH(1);
+        else if (std::is_same<T, bf16_t>::value && a.o32 && a.rel_table) LAUNCH((std::is_same<T, bf16_t>::value ? 3 : 2));
         else LAUNCH(2);
     }
 #undef LAUNCH

@@ -5,7 +5,8 @@
 // log2 LPH steps inside a wave and no head leaves its wave.  What is not a head's own value lies in LDS as coefficients per column, built once per
 // row: the forward's y = r (x A + partner B) with A = w cos, B = +- w_partner sin (two multiplies and one fma an element), the backward's cos,
 // +- sin and w.  With few registers (many waves on a CU) rather than loads ahead: prefetching the next head, or two heads in flight with
-// weights and angles in registers, measured 139 - 142 us where this order of work took 79 (16384 rows of 32 + 8 heads of 128, f16).
+// weights and angles in registers, measured 139 - 142 us where this order of work takes 76: 335 MB at 4.4 TB/s (16384 rows of
+// 32 + 8 heads of 128, f16).
 #include "sequence.h"
 #include <math.h>
 
