@@ -568,7 +568,11 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const float* __restr
             const int i = lane + 64 * j;
             if (i < nv)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) { const float t = v[j][c] - mean; ss += t * t; }
+                for (int c = 0; c < 4; ++c) {
+#pragma clang fp contract(off)
+                    const float t = v[j][c] - mean;
+                    ss += t * t;
+                }
         }
         const float rstd = 1.0f / sqrtf(wsum(ss) / (float)d + eps);
         float s1 = 0.f, s2 = 0.f;   // sum(dxhat), sum(dxhat * xhat)

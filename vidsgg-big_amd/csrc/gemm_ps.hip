@@ -599,7 +599,11 @@ __global__ __launch_bounds__(64 * NWV, 1) void gemm_ps_kernel(const PsArgs p) {
 #pragma unroll
             for (int fi = 0; fi < 2; ++fi)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) { const float d = acc[fi][ri][r] - mean[ri]; q += d * d; }
+                for (int r = 0; r < 16; ++r) {
+#pragma clang fp contract(off)
+                    const float d = acc[fi][ri][r] - mean[ri];
+                    q += d * d;
+                }
             q += __shfl_xor(q, 32);
             if (hi == 0) red[TM * 8 + (ri * 32 + l31) * 8 + wf] = q;
         }

@@ -143,7 +143,11 @@ __global__ __launch_bounds__(256) void ln_dwconv_rows_kernel(const float* __rest
         const float mean = gsum((v[0] + v[1]) + (v[2] + v[3])) / (float)(4 * D4);
         float ss = 0.f;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) { const float t = v[c] - mean; ss += t * t; }
+        for (int c = 0; c < 4; ++c) {
+#pragma clang fp contract(off)
+            const float t = v[c] - mean;
+            ss += t * t;
+        }
         const float rstd = 1.0f / sqrtf(gsum(ss) / (float)(4 * D4) + eps);
         f32x4 o;
 #pragma unroll

@@ -158,7 +158,11 @@ __device__ __forceinline__ void ec_stats(EcSmemT<CR>& S, int tid, float eps) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) { const float t = v[i][c] - mean; ss += t * t; }
+        for (int c = 0; c < 4; ++c) {
+#pragma clang fp contract(off)
+            const float t = v[i][c] - mean;
+            ss += t * t;
+        }
     const float rstd = 1.0f / sqrtf(ec_quad_sum(ss) / (float)EC_D + eps);
     if (q == 0) S.stat[row] = make_float2(mean, rstd);
 }

@@ -42,7 +42,8 @@ __global__ __launch_bounds__(256) void layernorm_kernel(const float* __restrict_
         if (i < nv) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const float t = v[j][c] - mean;
+#pragma clang fp contract(off)
+                const float t = v[j][c] - mean;                // (the squares are rounded before they are added, whatever the compiler would make of it)
                 ss += t * t;
             }
         }
@@ -131,7 +132,11 @@ __global__ __launch_bounds__(256) void layernorm_rows_kernel(const float* __rest
 #pragma unroll
         for (int j = 0; j < NVL; ++j)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) { const float t = v[u][j][c] - mean; ss += t * t; }
+            for (int c = 0; c < 4; ++c) {
+#pragma clang fp contract(off)
+                const float t = v[u][j][c] - mean;
+                ss += t * t;
+            }
         const float rstd = 1.0f / sqrtf(gsum(ss) / (float)(4 * D4) + eps);
         const int row = row0 + u * RPW;
         if (row < rows) {
