@@ -303,7 +303,8 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
                             add_diagonals(x, bins, kb + 32 * u - (i0 + shift), low);
                         }
                     }
-                    if (rule.cap) for (int e = 0; e < 16; ++e) x[e] *= cap_slope<T>(t[e]);
+                    if (rule.cap)                               // (the slope of a hidden place's score may be NaN)
+                        for (int e = 0; e < 16; ++e) x[e] = careful && x[e] == 0.f ? 0.f : x[e] * cap_slope<T>(t[e]);
                     scale.fit(x, acc, DT);
                     if constexpr (careful) accumulate_seen<TL>(acc, kt, 32 * u, x);
                     else accumulate<TL>(acc, kt, 32 * u, x);
@@ -484,7 +485,8 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
                                 x[4 * g + e] = careful && p == 0.f ? 0.f : p * (y[4 * g + e] - d4[e]);
                             }
                         }
-                        if (rule.cap) for (int e = 0; e < 16; ++e) x[e] *= cap_slope<T>(t[e]);
+                        if (rule.cap)
+                            for (int e = 0; e < 16; ++e) x[e] = careful && x[e] == 0.f ? 0.f : x[e] * cap_slope<T>(t[e]);
                         scale.fit(x, dk, DT);
                         if constexpr (careful) accumulate_seen<TL>(dk, qt, 32 * u, x);
                         else accumulate<TL>(dk, qt, 32 * u, x);
