@@ -27,3 +27,15 @@ def test_capped_scores_of_hidden_nan(t, what, times):
     got = c.check()
     for n, rows in (("o", 140 * times), ("dq", 140 * times), ("dk", 190 * times), ("dv", 190 * times), ("d_rel_table", 8)):
         assert torch.isfinite(got[n][:rows]).all(), n
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("n", [2, 33, 100])
+@pytest.mark.parametrize("times", [1, 128])
+def test_rows_whose_scores_are_all_far_below_zero(t, n, times):
+    """softmax does not care for an offset that all scores share; nor do the gradients of the last keys, beside which there are lanes without a key"""
+    c = Case(t, [(n, n)] * times, heads=(4, 4), hd=32, qk=0.5)
+    a = (40 / 32 ** 0.5) ** 0.5                                             # a^2 hd / sqrt(hd) = 40
+    c.q = (c.q.float() + a).to(c.t)
+    c.k = (c.k.float() - a).to(c.t)
+    c.check()

@@ -376,6 +376,8 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
     me.lo = j < prefix ? j - (sp.nk - 1) : max(reach.lo, j - (sp.nk - 1));
     me.hi = j < prefix ? 0x7fffffff : reach.hi;
     me.prefix = 0; me.doc = 0; me.bias = 0;
+    if (!live) { me.lo = 0x7fffffff; me.hi = -0x7fffffff; }     // no key: sees nothing (a score of 0 may be far above the row's maximum, and would set the wave's GradScale)
+    const bool all_live = j0 + 32 <= sp.nk;                     // of the wave: only then a tile is seen whole
 
     // LDS: two buffers of Q and dO tiles; per buffer the rows' -m, 1 / l, delta and documents (64 places each); biases of a head
     char* const mine = lds + (SPLIT ? wave * B::NBUF * BUF : 0);
@@ -457,7 +459,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
                 }
                 const int ib = k * ROWS, p_min = ib + shift, p_max = ib + ROWS - 1 + shift, d_min = j_min - p_max, d_max = j_max - p_min;
                 const bool seen = wave_live && (j_min < prefix || (d_max >= reach.lo && d_min <= reach.hi));
-                bool full = ib + ROWS <= sp.nq && (j_max < prefix || (d_min >= reach.lo && d_max <= reach.hi));
+                bool full = all_live && ib + ROWS <= sp.nq && (j_max < prefix || (d_min >= reach.lo && d_max <= reach.hi));
                 full &= whole;
                 if (seen) {
                     for (int u = 0; u < SUBS; ++u) {
