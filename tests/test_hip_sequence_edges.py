@@ -39,3 +39,12 @@ def test_rows_whose_scores_are_all_far_below_zero(t, n, times):
     c.q = (c.q.float() + a).to(c.t)
     c.k = (c.k.float() - a).to(c.t)
     c.check()
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("n", [2, 33, 100])
+@pytest.mark.parametrize("value", [100.0, -100.0])
+@pytest.mark.parametrize("times", [1, 64])
+def test_biases_beyond_the_exponents_range(t, n, value, times):
+    """2^(100 log2 e) is no f32: lanes without a row, whose scores have no maximum taken off, leave nothing in the table's gradient"""
+    Case(t, [(n, n), (n, 2 * n)] * times, heads=(4, 4), hd=32, rel_table=value + table(8, 4), rel_map=sequence.rel_bucket_map(8, 20)).check()

@@ -165,6 +165,8 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
     LaneRow me;
     me.lo = reach.lo; me.hi = min(reach.hi, sp.nk - 1 - pos);
     me.prefix = prefix - pos; me.doc = 0; me.bias = 0;
+    if (!live) { me.lo = 0x7fffffff; me.hi = me.prefix = -0x7fffffff; }      // no query: sees nothing (its scores, a bias at most, have no maximum taken off, and the table's sums add all lanes up)
+    const bool all_live = i0 + 32 <= sp.nq;                     // of the wave: only then a tile is seen whole
     me.slope2 = rule.slopes ? a.slopes[head] * LOG2E : 0.f;
 
     char* const docs_lds = lds + B::STAGES;
@@ -277,7 +279,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
             }
             const int kb = k * KEYS, ke = min(kb + KEYS, sp.nk), d_min = kb - p_max, d_max = kb + KEYS - 1 - p_min;
             const bool seen = wave_live && (kb < prefix || (d_max >= reach.lo && d_min <= reach.hi));
-            bool full = kb + KEYS <= sp.nk && (ke <= prefix || (d_min >= reach.lo && d_max <= reach.hi));
+            bool full = all_live && kb + KEYS <= sp.nk && (ke <= prefix || (d_min >= reach.lo && d_max <= reach.hi));
             full &= whole;
             if (seen) {
                 for (int u = 0; u < SUBS; ++u) {
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
                     const Linear sc = make_scores<T, true, true>(x, &t, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (SUBS - 1 - u));
                     if (!full) hide_scores<true>(x, sc, me, d0, a.q_doc ? docs + buf * 64 + 32 * u + 4 * hi : nullptr);
                     const float base = sc.c - m;
-                    for (int e = 0; e < 16; ++e) {              // rows that are not there: 0 (1 / l is 0)
+                    for (int e = 0; e < 16; ++e) {
                         const float p = __builtin_amdgcn_exp2f(fmaf(x[e], sc.a, base)), ds = p * fmaf(y[e], sign_l, minus);
                         x[e] = careful && p == 0.f ? 0.f : ds;
                     }
