@@ -48,3 +48,52 @@ def test_rows_whose_scores_are_all_far_below_zero(t, n, times):
 def test_biases_beyond_the_exponents_range(t, n, value, times):
     """2^(100 log2 e) is no f32: lanes without a row, whose scores have no maximum taken off, leave nothing in the table's gradient"""
     Case(t, [(n, n), (n, 2 * n)] * times, heads=(4, 4), hd=32, rel_table=value + table(8, 4), rel_map=sequence.rel_bucket_map(8, 20)).check()
+
+
+def even_spread(c, n):
+    """gradients of one sequence of n rows whose every row spreads evenly, P = 1 / n, and the bounds of their errors: P and dS take the half type's rounding r, delta that of an
+    o from P in two parts (2 r^2), and the sums in f32 at most 2 (hd + n + 16) steps of 2^-24 of the absolute values they add"""
+    q, k, v, go = (x[:n, 0].double() for x in (c.q, c.k, c.v, c.go))
+    r, u = eps_of(c.t) / 2, 2.0 ** -24
+    scale, e = c.hd ** -0.5, 2 * (c.hd + n + 16) * u
+    o = v.mean(0, keepdim=True)
+    ds = (go @ v.t() - go @ o.t()) / n
+    reach = (go.abs() @ v.abs().t() + (go.abs() @ v.abs().mean(0, keepdim=True).t())) / n
+    es = reach * (e + 2 * r * r) + r * ds.abs()
+    want = dict(dq=scale * ds @ k, dk=scale * ds.t() @ q, dv=(go.sum(0, keepdim=True) / n).expand(n, -1))
+    tol = dict(dq=scale * es @ k.abs(), dk=scale * es.t() @ q.abs(), dv=((r + e) * go.abs().sum(0, keepdim=True) / n).expand(n, -1))
+    return {name: (w, tol[name] + (r + u) * (w.abs() + tol[name])) for name, w in want.items()}
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("value", [-1e5, -1e7, -1e8, -1e9, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("n", [4, 70])
+def test_gradients_of_rows_with_one_very_low_bias(t, value, n):
+    """Every visible key of every row has the same very low bias.  From -1e9 on no f32 holds bias + score, and the row spreads evenly; at the others the scores' rest in f32 is
+    given its place in the bound by leaving the scores out (scale 0 where they would still count)."""
+    lost = value <= -1e9
+    c = Case(t, [(n, n)], heads=(1, 1), hd=64, rel_table=torch.full((4, 1), value), rel_map=sequence.rel_bucket_map(4, 2 * n), **({} if lost else dict(scale=0.0)))
+    got = c.run()
+    want = even_spread(c, n)
+    near("o", got["o"][:n, 0], c.v[:n, 0].double().mean(0, keepdim=True).expand(n, -1), 2 * (eps_of(c.t) + 2.0 ** -20) * c.v[:n, 0].double().abs().mean(0))
+    for name in ("dq", "dk", "dv"):
+        w, tol = want[name]
+        if not lost and name != "dv":
+            w, tol = torch.zeros_like(w), torch.zeros_like(tol)
+        near(name, got[name][:n, 0], w, tol, tiny_of(c.t))
+    # a row's dS adds up to nothing, its error to that of the bound above: (e + 2 r^2) times sum |d_o| (|v| + |o|)
+    most = (2 * (64 + n + 16) * 2.0 ** -24 + eps_of(c.t) ** 2 / 2) * 2 * float((c.go[:n].double().abs().sum((1, 2)) * c.v[:n].double().abs().max()).sum())
+    assert float(got["d_rel_table"].double().sum().abs()) <= most
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("value", [float("-inf"), torch.finfo(torch.float32).min])
+def test_gradients_with_buckets_of_the_lowest_value(t, value):
+    tab = table(8, 2)
+    tab[3] = value
+    tab[0] = value
+    Case(t, [(60, 60), (1, 1), (5, 90)], rel_table=tab, rel_map=sequence.rel_bucket_map(8, 20)).check()
+    c = Case(t, [(70, 70)], rel_table=torch.full((8, 2), value), rel_map=sequence.rel_bucket_map(8, 20))
+    got = c.run()
+    if value == float("-inf"):
+        assert all((got[n] == 0).all() for n in ("dq", "dk", "dv", "d_rel_table"))

@@ -45,7 +45,7 @@ struct BwdShape {
     int q_tiles, k_tiles;                                       // of a block's rows, of the longest sequence
     int q_pairs, k_pairs;                                       // (sequence, head), (sequence, key head)
     size_t q_lds, k_lds;
-    size_t rows, q_ranges, k_ranges, bins, total;               // workspace: [3][n_head][n_q] P_LIFT - m, 1 / l, delta; document ranges; sums by distance
+    size_t rows, q_ranges, k_ranges, bins, total;               // workspace: [3][n_head][n_q] -m, 2^P_LIFT / l, delta; document ranges; sums by distance
 };
 
 // SPLIT: for launches of few blocks.  A block then has 32 rows instead of 128, and its waves take the streamed tiles of the same rows in turn, each through
@@ -56,7 +56,7 @@ template <typename T, int HD, bool SPLIT, bool KV> struct BwdTile {
     typedef Tile<T, HD, ROWS> TL;
     static constexpr int WAVES = 4, BLOCK_ROWS = SPLIT ? 32 : 128, NW = SPLIT ? 1 : 4, NBUF = 2;
     static constexpr int TILE = TL::BYTES, BUF = 2 * TILE, STAGES = (SPLIT ? WAVES : 1) * NBUF * BUF;
-    static constexpr int SIDE = KV ? 1024 : 256, SIDES = (SPLIT ? WAVES : 1) * NBUF * SIDE;            // beside a tile: the streamed queries' -m, 1 / l, delta, documents; keys' documents
+    static constexpr int SIDE = KV ? 1024 : 256, SIDES = (SPLIT ? WAVES : 1) * NBUF * SIDE;            // beside a tile: the streamed queries' -m, 2^P_LIFT / l, delta, documents; keys' documents
     static constexpr int PAD = 33, JOIN = WAVES * HD * PAD * 4;
     static_assert(!SPLIT || (JOIN <= STAGES && STAGES <= 140 * 1024), "");
 };
@@ -132,7 +132,9 @@ __device__ __forceinline__ void add_diagonals(const f32x16& v, float* bins, int 
     }
 }
 
-template <typename T> constexpr float P_LIFT = 0.f;             // P reaches the product with dO as P 2^P_LIFT (f16 ends at 2^-14)
+// P reaches the product with dO as P 2^P_LIFT (f16 ends at 2^-14).  The lift goes with 1 / l, a power of two on a factor, and not into the exponent beside -m, where it would be
+// rounded away once a row's scores pass 2^24 (biases of -1e9 and the like on all that a row sees).
+template <typename T> constexpr float P_LIFT = 0.f;
 template <> constexpr float P_LIFT<f16_t> = 14.f;
 
 template <typename T, int HD, bool SPLIT>
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
     if (ml.y == 0.f) delta = 0.f;
     if (live && hi == 0 && (!SPLIT || wave == 0)) {
         const long plane = a.n_q * a.n_head, at = head * a.n_q + row;
-        row_data[at] = P_LIFT<T> - m; row_data[plane + at] = inv_l; row_data[2 * plane + at] = delta;
+        row_data[at] = -m; row_data[plane + at] = inv_l * (P_LIFT<T> == 0.f ? 1.f : 16384.f); row_data[2 * plane + at] = delta;
     }
     const float minus = -delta * inv_l;                         // dS = p (dP / l - delta / l)
     // Every other row's dP is taken negated: the matrix instructions cut off a sum's last bits downwards, and the table's gradient, which adds such errors up over all rows
@@ -381,7 +383,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
     if (!live) { me.lo = 0x7fffffff; me.hi = -0x7fffffff; }     // no key: sees nothing (a score of 0 may be far above the row's maximum, and would set the wave's GradScale)
     const bool all_live = j0 + 32 <= sp.nk;                     // of the wave: only then a tile is seen whole
 
-    // LDS: two buffers of Q and dO tiles; per buffer the rows' -m, 1 / l, delta and documents (64 places each); biases of a head
+    // LDS: two buffers of Q and dO tiles; per buffer the rows' -m, 2^P_LIFT / l, delta and documents (64 places each); biases of a head
     char* const mine = lds + (SPLIT ? wave * B::NBUF * BUF : 0);
     char* const side = lds + B::STAGES + (SPLIT ? wave * B::NBUF * B::SIDE : 0);
     float* const biases = (float*)(lds + B::STAGES + B::SIDES);
@@ -430,7 +432,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
                 stage_o.load(mine + buf * BUF + TILE, o_rows, k * ROWS, sp.nq, sw);
             };
             const auto copy_side = [&](int k, int buf) {
-                const int at = min(k * ROWS + lane, sp.nq - 1);                            // -m, 1 / l, delta and the documents, one a wave (SPLIT: all by each)
+                const int at = min(k * ROWS + lane, sp.nq - 1);                            // -m, 2^P_LIFT / l, delta and the documents, one a wave (SPLIT: all by each)
                 for (int what = SPLIT ? 0 : wave; what < (a.q_doc ? 4 : 3); what += SPLIT ? 1 : 4) {
                     const void* from = what < 3 ? (const void*)(row_data + what * plane + head * a.n_q + sp.q0 + at) : (const void*)(a.q_doc + sp.q0 + at);
                     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, LDS_PTR(void, side + buf * B::SIDE + what * 256), 4, 0, 0);
