@@ -97,3 +97,29 @@ def test_gradients_with_buckets_of_the_lowest_value(t, value):
     got = c.run()
     if value == float("-inf"):
         assert all((got[n] == 0).all() for n in ("dq", "dk", "dv", "d_rel_table"))
+
+
+CLEAN = {}
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("what", [float("inf"), float("-inf")])
+@pytest.mark.parametrize("where", ["q", "k", "v", "go"])
+@pytest.mark.parametrize("times", [1, 160])
+def test_a_document_with_infinities_leaves_the_others_alone(t, what, where, times):
+    """a document of Inf that shares blocks, waves and tiles with one that ends long behind it, and one before (160 times the same sequence: blocks of 128 rows)"""
+    n = 600
+    doc = torch.tensor([0] * 70 + [1] * 50 + [2] * 480 + [0] * 3, dtype=torch.int32)
+    c = Case(t, [(n, n)], hd=32, q_doc=doc, k_doc=doc)
+    if t not in CLEAN:
+        CLEAN[t] = c.want()
+    want = CLEAN[t]
+    getattr(c, where)[70:120, :, 3] = what                               # (one column: dS is Inf then, not NaN)
+    q, k, v, go = (x[:n].repeat(times, 1, 1).to(DEV) for x in (c.q, c.k, c.v, c.go))
+    docs = doc[:n].repeat(times).to(DEV)
+    off = n * torch.arange(times + 1, dtype=torch.int32, device=DEV)
+    o, saved = sequence.attend(q, k, v, off, off, n, n, q_doc=docs, k_doc=docs, save=True)
+    keep = torch.cat([torch.arange(70), torch.arange(120, n)])
+    for name, g in zip(("o", "dq", "dk", "dv"), (o,) + sequence.attend_bwd(saved, go)[:3]):
+        for s in range(0, times, 53):
+            near(name, g[n * s:n * (s + 1)][keep.to(DEV)], want[name][keep], want["tol_" + name][keep], tiny_of(c.t))

@@ -25,8 +25,12 @@ template <> struct GradScale<f16_t> {
         float top = fabsf(v[0]);
         for (int e = 1; e < 16; ++e) top = fmaxf(top, fabsf(v[e]));
         if (__ballot(s == 0.f ? top > 0.f : top * s > 32768.f)) {
+            if (__ballot(top == INFINITY)) {                    // of finite values: a row of Inf takes its neighbours in the wave nothing
+                top = 0.f;
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
+            }
             for (int m = 32; m; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
-            if (top > 0.f && top < INFINITY) {
+            if (s == 0.f ? top > 0.f : top * s > 32768.f) {
                 const float now = ldexpf(1.f, min(14 - ilogbf(top), 120));
                 if (s != 0.f) {
                     const float c = now / s;
