@@ -123,3 +123,20 @@ def test_a_document_with_infinities_leaves_the_others_alone(t, what, where, time
     for name, g in zip(("o", "dq", "dk", "dv"), (o,) + sequence.attend_bwd(saved, go)[:3]):
         for s in range(0, times, 53):
             near(name, g[n * s:n * (s + 1)][keep.to(DEV)], want[name][keep], want["tol_" + name][keep], tiny_of(c.t))
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("nq", [1, 40, 300])
+def test_a_score_of_minus_infinity_takes_no_weight(t, nq):
+    """a seen key with -Inf in a column where every query holds 1: the score is -Inf whatever the other bits of 1 are, in rows few or many"""
+    c = Case(t, [(nq, 300)], heads=(2, 2), hd=32)
+    c.q[..., 5] = 1.0
+    c.k[20, :, 5] = float("-inf")
+    got = c.run()
+    doc = torch.zeros(303, dtype=torch.int32)
+    doc[20] = -1                                                            # the same key behind a mask
+    c.kw.update(q_doc=torch.zeros(nq + 3, dtype=torch.int32), k_doc=doc)
+    want = c.want()
+    for name in ("o", "lse", "dq", "dk", "dv"):
+        n = nq if name in ("o", "lse", "dq") else 300
+        near(name, got[name][:n], want[name][:n], want["tol_" + name][:n], tiny_of(c.t))

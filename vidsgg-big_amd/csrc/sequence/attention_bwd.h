@@ -291,8 +291,13 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
                 for (int u = 0; u < SUBS; ++u) {
                     f32x16 x, y, t;
                     for (int e = 0; e < 16; ++e) x[e] = y[e] = 0.f;
-                    add_products<TL>(x, kt, 32 * u, q);
-                    add_products<TL>(y, vt, 32 * u, go);
+                    if constexpr (careful) {
+                        add_products_seen<TL>(x, kt, 32 * u, q);
+                        add_products_seen<TL>(y, vt, 32 * u, go);
+                    } else {
+                        add_products<TL>(x, kt, 32 * u, q);
+                        add_products<TL>(y, vt, 32 * u, go);
+                    }
                     const int d0 = kb + 32 * u + 4 * hi - pos;
                     const Linear sc = make_scores<T, true, true>(x, &t, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (SUBS - 1 - u));
                     if (!full) hide_scores<true>(x, sc, me, d0, a.q_doc ? docs + buf * 64 + 32 * u + 4 * hi : nullptr);
@@ -474,8 +479,13 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
                         const float* const rows = (const float*)(side + buf * B::SIDE) + 32 * u + 4 * hi;
                         f32x16 x, y, t;
                         for (int e = 0; e < 16; ++e) x[e] = y[e] = 0.f;
-                        add_products<TL>(x, qt, 32 * u, kf);
-                        add_products<TL>(y, ot, 32 * u, vf);
+                        if constexpr (careful) {
+                            add_products_seen<TL>(x, qt, 32 * u, kf);
+                            add_products_seen<TL>(y, ot, 32 * u, vf);
+                        } else {
+                            add_products<TL>(x, qt, 32 * u, kf);
+                            add_products<TL>(y, ot, 32 * u, vf);
+                        }
                         const int d0 = j - shift - ib - 32 * u - 4 * hi;
                         const Linear sc = make_scores<T, false, true>(x, &t, rule, me, biases, d0, d_min + 32 * (SUBS - 1 - u), d_max - 32 * u);
                         if (!full) hide_scores<false>(x, sc, me, d0, a.q_doc ? (const int*)rows + 192 : nullptr);

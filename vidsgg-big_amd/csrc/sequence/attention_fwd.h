@@ -242,7 +242,8 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
                 for (int u = 0; u < F::SUBS; ++u) {                 // 32 keys at a time
                     f32x16 x;
                     for (int e = 0; e < 16; ++e) x[e] = 0.f;
-                    add_products<TL>(x, kt, 32 * u, q);
+                    if constexpr (careful) add_products_seen<TL>(x, kt, 32 * u, q);
+                    else add_products<TL>(x, kt, 32 * u, q);
                     const int d0 = kb + 32 * u + 4 * hi - pos;
                     const Linear s = make_scores<T, true, false>(x, nullptr, rule, me, biases, d0, d_min + 32 * u, d_max - 32 * (F::SUBS - 1 - u));
                     if (!full) hide_scores<true>(x, s, me, d0, a.q_doc ? my_docs + buf * 64 + 32 * u + 4 * hi : nullptr);

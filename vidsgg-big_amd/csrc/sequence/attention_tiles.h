@@ -139,6 +139,19 @@ __device__ __forceinline__ void add_products(f32x16& x, const char* tile, int ro
     for (int c = 0; c < TL::STEPS; ++c) x = Mat<typename TL::T>::mul(rows_frag<TL>(tile, row0, c), lanes[c], x);
 }
 
+// The same for tiles or lanes that may hold Inf (x was 0 before).  f32s: Inf times a second or third part that is 0 is NaN where Inf times the value is Inf; the products of the
+// first parts, which no nonzero value lacks, have then what the sum comes to.
+template <typename TL>
+__device__ __forceinline__ void add_products_seen(f32x16& x, const char* tile, int row0, const typename Mat<typename TL::T>::frag* lanes) {
+    add_products<TL>(x, tile, row0, lanes);
+    if constexpr (std::is_same<typename TL::T, f32s>::value) {
+        f32x16 first;
+        for (int e = 0; e < 16; ++e) first[e] = 0.f;
+        for (int c = 0; c < TL::STEPS; ++c) first = Mat<bf16_t>::mul(rows_frag<typename TL::Part>(tile, row0, c), lanes[c].h, first);
+        for (int e = 0; e < 16; ++e) x[e] = isnan(x[e]) ? first[e] : x[e];
+    }
+}
+
 // A operand, transposed: columns col0 .. col0 + 31, the 16 rows from row0 on (a multiple of 16) in the order in which a product's registers 8 u .. 8 u + 7
 // hold them (half types)
 template <typename TL>
