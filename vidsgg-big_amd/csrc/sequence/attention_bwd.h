@@ -171,8 +171,6 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
     LaneRow me;
     me.lo = reach.lo; me.hi = min(reach.hi, sp.nk - 1 - pos);
     me.prefix = prefix - pos; me.doc = 0; me.bias = 0;
-    if (!live) { me.lo = 0x7fffffff; me.hi = me.prefix = -0x7fffffff; }      // no query: sees nothing (its scores, a bias at most, have no maximum taken off, and the table's sums add all lanes up)
-    const bool all_live = i0 + 32 <= sp.nq;                     // of the wave: only then a tile is seen whole
     me.slope2 = rule.slopes ? a.slopes[head] * LOG2E : 0.f;
 
     char* const docs_lds = lds + B::STAGES;
@@ -193,7 +191,8 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
     load_lane_rows<T, HD>(go, (const T*)a.d_o + row * a.lddo + head * a.hsdo, live, a.head_dim);
     const long rh = row * a.n_head + head;
     const float2 ml = live ? *(const float2*)(a.stats + 2 * rh) : make_float2(0.f, 0.f);
-    const float m = ml.x == -INFINITY ? 0.f : ml.x, inv_l = ml.y == 0.f ? 0.f : 1.f / ml.y;
+    // A lane without a query has P = 0 by a maximum of Inf: its scores, a bias at most, would otherwise have none taken off, and the table's sums add all lanes up.
+    const float m = !live ? INFINITY : ml.x == -INFINITY ? 0.f : ml.x, inv_l = ml.y == 0.f ? 0.f : 1.f / ml.y;
     double total = 0.;                                          // (the table's gradient adds delta's error up over all keys)
     if (a.o32) {
         for (int c = 0; c < TL::STEPS; ++c)
@@ -285,7 +284,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
             }
             const int kb = k * KEYS, ke = min(kb + KEYS, sp.nk), d_min = kb - p_max, d_max = kb + KEYS - 1 - p_min;
             const bool seen = wave_live && (kb < prefix || (d_max >= reach.lo && d_min <= reach.hi));
-            bool full = all_live && kb + KEYS <= sp.nk && (ke <= prefix || (d_min >= reach.lo && d_max <= reach.hi));
+            bool full = kb + KEYS <= sp.nk && (ke <= prefix || (d_min >= reach.lo && d_max <= reach.hi));
             full &= whole;
             if (seen) {
                 for (int u = 0; u < SUBS; ++u) {
@@ -304,7 +303,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
                     const float base = sc.c - m;
                     for (int e = 0; e < 16; ++e) {
                         const float p = __builtin_amdgcn_exp2f(fmaf(x[e], sc.a, base)), ds = p * fmaf(y[e], sign_l, minus);
-                        x[e] = careful && p == 0.f ? 0.f : ds;
+                        x[e] = careful && (p == 0.f || !live) ? 0.f : ds;
                     }
                     if (nb) {
                         const int lo = d_min + 32 * u, up = d_max - 32 * (SUBS - 1 - u);
@@ -389,8 +388,8 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
     me.lo = j < prefix ? j - (sp.nk - 1) : max(reach.lo, j - (sp.nk - 1));
     me.hi = j < prefix ? 0x7fffffff : reach.hi;
     me.prefix = 0; me.doc = 0; me.bias = 0;
-    if (!live) { me.lo = 0x7fffffff; me.hi = -0x7fffffff; }     // no key: sees nothing (a score of 0 may be far above the row's maximum, and would set the wave's GradScale)
-    const bool all_live = j0 + 32 <= sp.nk;                     // of the wave: only then a tile is seen whole
+    // A lane without a key has P = 0 by an offset of -Inf: its score of 0 may be far above a row's maximum, and would set the wave's GradScale.
+    const float none = live ? 0.f : -INFINITY;
 
     // LDS: two buffers of Q and dO tiles; per buffer the rows' -m, 2^P_LIFT / l, delta and documents (64 places each); biases of a head
     char* const mine = lds + (SPLIT ? wave * B::NBUF * BUF : 0);
@@ -472,7 +471,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
                 }
                 const int ib = k * ROWS, p_min = ib + shift, p_max = ib + ROWS - 1 + shift, d_min = j_min - p_max, d_max = j_max - p_min;
                 const bool seen = wave_live && (j_min < prefix || (d_max >= reach.lo && d_min <= reach.hi));
-                bool full = all_live && ib + ROWS <= sp.nq && (j_max < prefix || (d_min >= reach.lo && d_max <= reach.hi));
+                bool full = ib + ROWS <= sp.nq && (j_max < prefix || (d_min >= reach.lo && d_max <= reach.hi));
                 full &= whole;
                 if (seen) {
                     for (int u = 0; u < SUBS; ++u) {
@@ -489,10 +488,11 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
                         const int d0 = j - shift - ib - 32 * u - 4 * hi;
                         const Linear sc = make_scores<T, false, true>(x, &t, rule, me, biases, d0, d_min + 32 * (SUBS - 1 - u), d_max - 32 * u);
                         if (!full) hide_scores<false>(x, sc, me, d0, a.q_doc ? (const int*)rows + 192 : nullptr);
+                        const float offset = sc.c + none;
                         for (int g = 0; g < 4; ++g) {
                             const f32x4 m4 = *LDS_PTR(const f32x4, rows + 8 * g), l4 = *LDS_PTR(const f32x4, rows + 64 + 8 * g);
                             for (int e = 0; e < 4; ++e) {
-                                const float p = __builtin_amdgcn_exp2f(fmaf(x[4 * g + e], sc.a, sc.c + m4[e]));
+                                const float p = __builtin_amdgcn_exp2f(fmaf(x[4 * g + e], sc.a, offset + m4[e]));
                                 x[4 * g + e] = careful && p == 0.f ? 0.f : p * l4[e];
                             }
                         }
