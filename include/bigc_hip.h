@@ -707,7 +707,8 @@ BIGC_API int bigc_linear_hr8out_f32(void* stream, const float* A, int lda, const
  *     o = softmax over the seen keys of the scores, times v
  * A query that sees no key (or only scores of -inf) has o = 0 and gives no gradient; what a hidden place holds (NaN, Inf) is never part of a
  * result (rows whose result is NaN or Inf are done twice, the second time value by value: such a call takes many times as long).  A bias of -inf hides its distances, the lowest finite values (below -2.3e38, which count as one) do not.  slopes, rel_table + rel_map, prefix_len, q_doc + k_doc may be NULL.  Rows outside every sequence
- * stay as they were.  Offsets are cut to [0, n_q] and [0, n_k] and lengths to max_q and max_k (which size the launch), map entries to the table. */
+ * stay as they were.  Offsets are cut to [0, n_q] and [0, n_k], map entries to the table, and lengths to max_q and max_k, which size the launch: a
+ * sequence is then its first rows, and those behind the cut are rows outside every sequence. */
 typedef struct {
     int32_t dtype;                     /* BIGC_F32 / BIGC_F16 / BIGC_BF16: q, k, v, o, d_o, dq, dk, dv */
     int32_t n_seq, n_head, n_kv_head;  /* n_head a multiple of n_kv_head */

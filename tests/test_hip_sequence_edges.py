@@ -140,3 +140,26 @@ def test_a_score_of_minus_infinity_takes_no_weight(t, nq):
     for name in ("o", "lse", "dq", "dk", "dv"):
         n = nq if name in ("o", "lse", "dq") else 300
         near(name, got[name][:n], want[name][:n], want["tol_" + name][:n], tiny_of(c.t))
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+def test_rows_behind_a_cut_are_zero(t, monkeypatch):
+    """sequences longer than max_q and max_k are cut to them; what lies behind the cut is a row outside every sequence"""
+    c = Case(t, [(5, 5), (90, 90), (0, 7), (70, 20)], heads=(4, 2), hd=40)
+    (q, k, v, go), _ = c.args(DEV)
+    off = c.q_off.to(DEV), c.k_off.to(DEV)
+    for max_q, max_k in ((64, 16), (0, 16), (64, 0), (3, 90)):
+        monkeypatch.setattr(torch.Tensor, "new_empty", lambda self, shape, dtype=None: self.new_full(shape, 99, dtype=dtype or self.dtype))
+        o, saved = sequence.attend(q, k, v, *off, max_q, max_k, save=True)
+        got = dict(zip(("dq", "dk", "dv"), sequence.attend_bwd(saved, go)), o=o)
+        kept = torch.full(q.shape, 7.0, dtype=c.t, device=DEV)
+        sequence.attend(q, k, v, *off, max_q, max_k, out=kept, save=True)      # (as above: without, half types keep fewer bits of P)
+        monkeypatch.undo()
+        for name, offs, longest in (("o", c.q_off, max_q), ("dq", c.q_off, max_q), ("dk", c.k_off, max_k), ("dv", c.k_off, max_k)):
+            own = torch.zeros(got[name].shape[0], dtype=torch.bool)
+            for a, b in zip(offs[:-1].tolist(), offs[1:].tolist()):
+                own[a:min(b, a + longest)] = True
+            assert (got[name].cpu()[~own] == 0).all(), name
+            assert (got[name].cpu()[own] != 99).all(), name
+            if name == "o":
+                assert (kept.cpu()[~own] == 7).all() and torch.equal(kept.cpu()[own], got["o"].cpu()[own])

@@ -63,7 +63,7 @@ extern "C" int bigc_seq_attn_fwd(void* stream, const bigc_seq_attn* ap, void* wo
     ProfScope prof(stream, FAM_MHA, 0, 0);
     if (sh.blocks == 0) {                                       // no sequence, or none with a query
         if (a.zero_rest) {
-#define F(T) zero_rows<T><<<256, 256, 0, hs>>>((T*)a.o, a.ldo, a.hso, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq);
+#define F(T) zero_rows<T><<<256, 256, 0, hs>>>((T*)a.o, a.ldo, a.hso, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq, a.max_q);
             SEQ_DISPATCH(a.dtype, F);
 #undef F
         }
@@ -112,10 +112,10 @@ extern "C" int bigc_seq_attn_bwd(void* stream, const bigc_seq_attn* ap, void* wo
     }
 #define F(T) \
     launch_bwd_dim<typename std::conditional<std::is_same<T, float>::value, f32s, T>::type>(hs, a, sh, ws); \
-    if (a.zero_rest && a.n_q && !q_blocks) zero_rows<T><<<256, 256, 0, hs>>>((T*)a.dq, a.lddq, a.hsdq, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq); \
+    if (a.zero_rest && a.n_q && !q_blocks) zero_rows<T><<<256, 256, 0, hs>>>((T*)a.dq, a.lddq, a.hsdq, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq, a.max_q); \
     if (a.zero_rest && a.n_k && !k_blocks) { \
-        zero_rows<T><<<256, 256, 0, hs>>>((T*)a.dk, a.lddk, a.hsdk, a.n_k, a.n_kv_head, a.head_dim, a.k_off, a.n_seq); \
-        zero_rows<T><<<256, 256, 0, hs>>>((T*)a.dv, a.lddv, a.hsdv, a.n_k, a.n_kv_head, a.head_dim, a.k_off, a.n_seq); \
+        zero_rows<T><<<256, 256, 0, hs>>>((T*)a.dk, a.lddk, a.hsdk, a.n_k, a.n_kv_head, a.head_dim, a.k_off, a.n_seq, a.max_k); \
+        zero_rows<T><<<256, 256, 0, hs>>>((T*)a.dv, a.lddv, a.hsdv, a.n_k, a.n_kv_head, a.head_dim, a.k_off, a.n_seq, a.max_k); \
     }
     SEQ_DISPATCH(a.dtype, F);
 #undef F

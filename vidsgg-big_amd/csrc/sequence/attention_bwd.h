@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
     __shared__ int2 shared_docs[4];
     __shared__ int shared_bad[4];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
-    if (a.zero_rest) zero_outside((T*)a.dq, a.lddq, a.hsdq, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq);
+    if (a.zero_rest) zero_outside((T*)a.dq, a.lddq, a.hsdq, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq, a.max_q);
     int pair, tile;
     if (!bwd_place(sh.q_pairs, sh.q_tiles, pair, tile)) return;
     if (a.causal) tile = sh.q_tiles - 1 - tile;                 // the longest first
@@ -369,8 +369,8 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
     __shared__ int shared_bad[4];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
     if (a.zero_rest) {
-        zero_outside((T*)a.dk, a.lddk, a.hsdk, a.n_k, a.n_kv_head, a.head_dim, a.k_off, a.n_seq);
-        zero_outside((T*)a.dv, a.lddv, a.hsdv, a.n_k, a.n_kv_head, a.head_dim, a.k_off, a.n_seq);
+        zero_outside((T*)a.dk, a.lddk, a.hsdk, a.n_k, a.n_kv_head, a.head_dim, a.k_off, a.n_seq, a.max_k);
+        zero_outside((T*)a.dv, a.lddv, a.hsdv, a.n_k, a.n_kv_head, a.head_dim, a.k_off, a.n_seq, a.max_k);
     }
     int pair, tile;
     if (!bwd_place(sh.k_pairs, sh.k_tiles, pair, tile)) return;

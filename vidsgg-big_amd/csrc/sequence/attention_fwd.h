@@ -76,15 +76,20 @@ __device__ __forceinline__ FwdPlace fwd_place(const FwdShape& sh, bool last_firs
     return {pair, last_first ? sh.tiles - 1 - tile : tile, in / sh.tiles};
 }
 
-// rows of `t` outside [off[0], off[n_seq]) -> 0
+// rows of `t` outside every sequence -> 0: those before the first and behind the last, and what of a sequence lies behind its first `longest` rows, to which it is cut
 template <typename T>
-__device__ __forceinline__ void zero_outside(T* t, long ld, long hs, long n, int heads, int hd, const int* off, int n_seq) {
+__device__ __forceinline__ void zero_outside(T* t, long ld, long hs, long n, int heads, int hd, const int* off, int n_seq, int longest) {
     const long first = n_seq ? min(max((long)off[0], 0l), n) : 0, last = n_seq ? min(max((long)off[n_seq], first), n) : 0;
     const int chunks = hd / (16 / (int)sizeof(T));
+    const auto zero = [&](long r, long e) { *(uint4*)(t + r * ld + e / chunks % heads * hs + e % chunks * (16 / sizeof(T))) = make_uint4(0, 0, 0, 0); };
     const long all = (first + n - last) * heads * chunks;
     for (long e = (long)blockIdx.x * blockDim.x + threadIdx.x; e < all; e += (long)gridDim.x * blockDim.x) {
         const long r = e / chunks / heads;
-        *(uint4*)(t + (r < first ? r : r - first + last) * ld + e / chunks % heads * hs + e % chunks * (16 / sizeof(T))) = make_uint4(0, 0, 0, 0);
+        zero(r < first ? r : r - first + last, e);
+    }
+    for (int s = blockIdx.x; s < n_seq; s += gridDim.x) {
+        const long begin = min(max((long)off[s], 0l), n), cut = begin + longest, rest = (min((long)off[s + 1], n) - cut) * heads * chunks;
+        for (long e = threadIdx.x; e < rest; e += blockDim.x) zero(cut + e / chunks / heads, e);
     }
 }
 
@@ -131,7 +136,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
     __shared__ int shared_bad[4];
     __shared__ int2 shared_docs[4];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
-    if (a.zero_rest) zero_outside((T*)a.o, a.ldo, a.hso, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq);
+    if (a.zero_rest) zero_outside((T*)a.o, a.ldo, a.hso, a.n_q, a.n_head, a.head_dim, a.q_off, a.n_seq, a.max_q);
 
     const FwdPlace at = fwd_place(sh, a.causal);
     if (at.pair >= sh.pairs) return;
@@ -401,8 +406,8 @@ __global__ __launch_bounds__(256) void attn_join(bigc_seq_attn a, FwdShape sh, c
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void zero_rows(T* t, long ld, long hs, long n, int heads, int hd, const int* off, int n_seq) {
-    zero_outside(t, ld, hs, n, heads, hd, off, n_seq);
+__global__ __launch_bounds__(256) void zero_rows(T* t, long ld, long hs, long n, int heads, int hd, const int* off, int n_seq, int longest) {
+    zero_outside(t, ld, hs, n, heads, hd, off, n_seq, longest);
 }
 
 int tile_dim(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 96 ? 96 : 128; }
