@@ -717,7 +717,7 @@ typedef struct {
     int32_t causal, window_left, window_right; /* windows: -1 = none */
     int32_t zero_rest;                 /* not 0: rows outside every sequence of o (forward), dq, dk, dv (backward) become 0 instead of staying as they were */
     int32_t bias_radius, n_bucket;     /* rel_map has 2 * bias_radius + 1 entries (bias_radius <= 2047), rel_table n_bucket rows of n_head */
-    float scale, softcap;              /* softcap 0: none */
+    float scale, softcap;              /* softcap 0: none; else 4 scale / softcap a finite number */
     int64_t n_q, n_k;                  /* rows of q / o and of k / v, below 2^31 */
     const int32_t* q_off; const int32_t* k_off; /* (n_seq + 1) */
     const float* slopes;               /* (n_head) */

@@ -163,3 +163,11 @@ def test_rows_behind_a_cut_are_zero(t, monkeypatch):
             assert (got[name].cpu()[own] != 99).all(), name
             if name == "o":
                 assert (kept.cpu()[~own] == 7).all() and torch.equal(kept.cpu()[own], got["o"].cpu()[own])
+
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("cap", [64.0, 65.0, 1e3, 1e4, 1e6, 1e20, 1e37])
+def test_caps_far_above_the_scores(t, cap):
+    """a cap that hardly bends a score leaves it with all its bits"""
+    Case(t, [(70, 70), (1, 200), (40, 90)], softcap=cap, causal=True, rel_table=table(8, 2), rel_map=sequence.rel_bucket_map(8, 30)).check()
+    Case(t, [(1, 300), (1, 7)], softcap=cap, causal=True).check(train=False)

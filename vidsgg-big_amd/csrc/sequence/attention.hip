@@ -29,6 +29,7 @@ int check_args(const bigc_seq_attn* ap, const char* who) {
     BIGC_CHECK_ARG(a.n_seq == 0 || (a.q_off && a.k_off), "%s: offsets are NULL", who);
     BIGC_CHECK_ARG(a.window_left >= -1 && a.window_right >= -1, "%s: window (%d, %d)", who, a.window_left, a.window_right);
     BIGC_CHECK_ARG(isfinite(a.scale) && isfinite(a.softcap) && a.softcap >= 0.f, "%s: scale %g, softcap %g", who, a.scale, a.softcap);
+    BIGC_CHECK_ARG(a.softcap == 0.f || isfinite(a.scale / a.softcap * 4.f), "%s: softcap %g too small for scale %g", who, a.softcap, a.scale);
     BIGC_CHECK_ARG(!a.q_doc == !a.k_doc || a.n_q == 0 || a.n_k == 0, "%s: q_doc and k_doc come together", who);
     BIGC_CHECK_ARG(!a.rel_table == !a.rel_map, "%s: rel_table and rel_map come together", who);
     if (a.rel_table) BIGC_CHECK_ARG(a.n_bucket > 0 && a.bias_radius >= 0 && a.bias_radius <= 2047, "%s: %d buckets, radius %d (at most 2047)", who, a.n_bucket, a.bias_radius);

@@ -315,8 +315,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
                             add_diagonals(x, bins, kb + 32 * u - (i0 + shift), low);
                         }
                     }
-                    if (rule.cap)                               // (the slope of a hidden place's score may be NaN)
-                        for (int e = 0; e < 16; ++e) x[e] = careful && x[e] == 0.f ? 0.f : x[e] * cap_slope<T>(t[e]);
+                    if (rule.cap) for (int e = 0; e < 16; ++e) x[e] = careful && x[e] == 0.f ? 0.f : x[e] * t[e];     // (the slope of a hidden place's score may be NaN)
                     scale.fit(x, acc, DT);
                     if constexpr (careful) accumulate_seen<TL>(acc, kt, 32 * u, x);
                     else accumulate<TL>(acc, kt, 32 * u, x);
@@ -343,7 +342,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 96 || (sizeof(T) == 4 && HD > 3
             out_bins[e] = sum;
         }
     }
-    const float f = a.scale * scale.back() * (rule.cap ? CAP_SLOPE<T> : 1.f);
+    const float f = a.scale * scale.back() * slope_unit<T>(rule);
     if constexpr (SPLIT) {
         join_rows<T, B>(lds, acc, f, min(32, sp.nq - first), a.head_dim, (T*)a.dq + (sp.q0 + first) * a.lddq + head * a.hsdq, a.lddq);
         return;
@@ -505,8 +504,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
                                 x[4 * g + e] = careful && p == 0.f ? 0.f : p * (y[4 * g + e] - d4[e]);
                             }
                         }
-                        if (rule.cap)
-                            for (int e = 0; e < 16; ++e) x[e] = careful && x[e] == 0.f ? 0.f : x[e] * cap_slope<T>(t[e]);
+                        if (rule.cap) for (int e = 0; e < 16; ++e) x[e] = careful && x[e] == 0.f ? 0.f : x[e] * t[e];     // (the slope of a hidden place's score may be NaN)
                         scale.fit(x, dk, DT);
                         if constexpr (careful) accumulate_seen<TL>(dk, qt, 32 * u, x);
                         else accumulate<TL>(dk, qt, 32 * u, x);
@@ -522,7 +520,7 @@ __global__ __launch_bounds__(256, (SPLIT || HD > 64 || sizeof(T) == 4 ? 1 : 2)) 
     float check = 0.f;
     for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) check += (dk[d][e] + dv[d][e]) * 0.f;
     if (SPLIT ? __ballot(check != 0.f && live) != 0 : any_wave(check != 0.f && live, wave, shared_bad)) pass(std::true_type());
-    const float unlift = P_LIFT<T> == 0.f ? 1.f : 1.f / 16384.f, f = a.scale * scale.back() * unlift * (rule.cap ? CAP_SLOPE<T> : 1.f);
+    const float unlift = P_LIFT<T> == 0.f ? 1.f : 1.f / 16384.f, f = a.scale * scale.back() * unlift * slope_unit<T>(rule);
     if constexpr (SPLIT) {
         const int n = min(32, sp.nk - first);
         join_rows<T, B>(lds, dk, f, n, a.head_dim, (T*)a.dk + (sp.k0 + first) * a.lddk + hk * a.hsdk, a.lddk);

@@ -355,34 +355,51 @@ __device__ __forceinline__ void wait_block() {
 
 // What every score of a call has in common; scores are kept times log2 e (exp is then one instruction).  Without a bias by distance a score is linear,
 // a v + c, in a value v: the product itself, or what the cap makes of it.
+constexpr float COARSE_CAP = 64.f, MAX_CAP = 0x1p100f;         // (a larger cap leaves every score under 2^88 as it is)
 struct ScoreRule {
     float a, c;
     float cap_in, cap_y;                                        // 2 scale log2 e / cap: the argument of tanh doubled, for 2^x; scale / cap
-    bool cap, slopes, table;
+    bool cap, coarse, slopes, table;                            // coarse: see cap_values
     int radius;
     template <typename T> __device__ __forceinline__ ScoreRule(const bigc_seq_attn& q, T)
-        : a(q.scale * LOG2E), c(0.f), cap_in(0.f), cap_y(0.f), cap(q.softcap > 0.f), slopes(q.slopes != nullptr), table(q.rel_table != nullptr), radius(q.bias_radius) {
+        : a(q.scale * LOG2E), c(0.f), cap_in(0.f), cap_y(0.f), cap(q.softcap > 0.f && q.softcap < MAX_CAP), coarse(sizeof(T) < 4 && q.softcap <= COARSE_CAP), slopes(q.slopes != nullptr), table(q.rel_table != nullptr), radius(q.bias_radius) {
         if (!cap) return;
         cap_in = 2.f * q.scale / q.softcap * LOG2E;
         cap_y = q.scale / q.softcap;
         a = q.softcap * LOG2E;
-        if (sizeof(T) < 4) { c = a; a = -2.f * a; }
+        if (coarse) { c = a; a = -2.f * a; }
     }
 };
 
-// The capped product's value.  Half types: v = 1 / (e^2y + 1), tanh y = 1 - 2 v -- its error is a step of 1, not of the value, which scores of half operands
-// live with.  f32: v = tanh y, small arguments through the odd series (to y^13: 2^-26 of the value at 0.5), the others with a division in full.
-template <typename T>
-__device__ __forceinline__ float cap_value(float x, const ScoreRule& r) {
-    const float e = __builtin_amdgcn_exp2f(x * r.cap_in) + 1.f;
-    if (sizeof(T) < 4) return __builtin_amdgcn_rcpf(e);
-    const float y = x * r.cap_y, z = y * y;
-    const float p = 1.f + z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315 + z * (62.f / 2835 + z * (-1382.f / 155925 + z * (21844.f / 6081075))))));
-    return fabsf(y) < 0.5f ? y * p : 1.f - 2.f / e;
+// The capped products' values.  f32: v = tanh y, small arguments through the odd series (to y^13: 2^-26 of the value at 0.5), the others with a division in full.
+// Half types under caps of up to 64 (coarse): v = 1 / (e^2y + 1), tanh y = 1 - 2 v -- its error is a step of 1, not of the value, so that a score is off by up to 2^-23 of the
+// cap: 8e-6 at 64, which scores of half operands live with, 0.1 at a million.  Larger caps: v = tanh y, by the series to y^7 up to 0.25, where both are off by 2^-21 of the value.
+// KEEP: the cap's slopes 1 - tanh^2 too, coarse a fourth of them (slope_unit).
+template <typename T, bool KEEP>
+__device__ __forceinline__ void cap_values(f32x16& x, f32x16* slopes, const ScoreRule& r) {
+    if (sizeof(T) < 4 && r.coarse) {
+        for (int e = 0; e < 16; ++e) {
+            const float v = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x[e] * r.cap_in) + 1.f);
+            if (KEEP) (*slopes)[e] = v - v * v;
+            x[e] = v;
+        }
+        return;
+    }
+    for (int e = 0; e < 16; ++e) {
+        const float y = x[e] * r.cap_y, z = y * y, f = __builtin_amdgcn_exp2f(x[e] * r.cap_in) + 1.f;
+        float v;
+        if (sizeof(T) < 4) {
+            const float p = y * (1.f + z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315))));
+            v = fabsf(y) < 0.25f ? p : 1.f - 2.f * __builtin_amdgcn_rcpf(f);
+        } else {
+            const float p = 1.f + z * (-1.f / 3 + z * (2.f / 15 + z * (-17.f / 315 + z * (62.f / 2835 + z * (-1382.f / 155925 + z * (21844.f / 6081075))))));
+            v = fabsf(y) < 0.5f ? y * p : 1.f - 2.f / f;
+        }
+        if (KEEP) (*slopes)[e] = 1.f - v * v;
+        x[e] = v;
+    }
 }
-// 1 - tanh^2, for half types without the factor CAP_SLOPE
-template <typename T> __device__ __forceinline__ float cap_slope(float v) { return sizeof(T) < 4 ? v - v * v : 1.f - v * v; }
-template <typename T> constexpr float CAP_SLOPE = sizeof(T) < 4 ? 4.f : 1.f;
+template <typename T> __device__ __forceinline__ float slope_unit(const ScoreRule& r) { return sizeof(T) < 4 && r.cap && r.coarse ? 4.f : 1.f; }
 
 // What a call lets a row see, by d = key - position of the query: [lo, hi] (wide enough for any two int32 places), and a prefix
 struct Reach {
@@ -420,14 +437,11 @@ __device__ __forceinline__ constexpr int reg_row(int e) { return (e & 3) + 8 * (
 
 // Products of 32 streamed rows with the lanes' rows -> values v with score = a v + c (c the lane's own).  d0: d of register 0; streamed keys count d up,
 // streamed queries down.  d_min, d_max: the least and the greatest d of the 32 x 32: where all are beyond the radius one bias serves and goes into c; else the
-// biased scores themselves become the values.  kept: the capped values, for the backward.
+// biased scores themselves become the values.  slopes: the cap's, for the backward (KEEP).
 struct Linear { float a, c; };
 template <typename T, bool LANE_IS_QUERY, bool KEEP>
-__device__ __forceinline__ Linear make_scores(f32x16& x, f32x16* kept, const ScoreRule& r, const LaneRow& l, const float* biases, int d0, int d_min, int d_max) {
-    if (r.cap) {
-        for (int e = 0; e < 16; ++e) x[e] = cap_value<T>(x[e], r);
-        if (KEEP) *kept = x;
-    }
+__device__ __forceinline__ Linear make_scores(f32x16& x, f32x16* slopes, const ScoreRule& r, const LaneRow& l, const float* biases, int d0, int d_min, int d_max) {
+    if (r.cap) cap_values<T, KEEP>(x, slopes, r);
     Linear s = {r.a, r.c};
     const float* const b = biases + l.bias + r.radius + BIAS_PAD;                          // of distance 0
     bool one_by_one = r.slopes || r.a == 0.f;
