@@ -688,6 +688,7 @@ BIGC_API int bigc_linear_hr8out_f32(void* stream, const float* A, int lda, const
  * -- position biases, caps and masks on the scores, shared key heads, norms and rotations of the heads.  They stand next to
  * bigc_mha_core_f32 (no order, no masks, one key head per query head) and take IEEE f32, f16 and bfloat16 tensors; scores,
  * softmax statistics, sums and parameter gradients are f32 whatever the tensors' type.  (models/ has no caller of its own.)
+ * Sizes have to fit a launch: n_seq * n_head * (blocks of 32 or 128 rows of the longest sequence) below 2^24, n_seq times max_q or max_k below 2^32.
  * Every row pointer, row stride and head stride has to be a multiple of 16 bytes (with one head, or one row, its stride
  * is not read), a row stride at most 2^22 elements.  Outputs overlap no input (but where it says so) and no other output.
  * ---------------------------------------------------------------------------------- */

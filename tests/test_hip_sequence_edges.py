@@ -171,3 +171,17 @@ def test_caps_far_above_the_scores(t, cap):
     """a cap that hardly bends a score leaves it with all its bits"""
     Case(t, [(70, 70), (1, 200), (40, 90)], softcap=cap, causal=True, rel_table=table(8, 2), rel_map=sequence.rel_bucket_map(8, 30)).check()
     Case(t, [(1, 300), (1, 7)], softcap=cap, causal=True).check(train=False)
+
+
+def test_many_short_caches_beside_room_for_long_ones():
+    """one token for each of 256 streams with 64 heads over one key head, where max_k is that of a cache of 131072 rows"""
+    g = torch.Generator().manual_seed(7)
+    lens = torch.randint(1, 40, (256,), generator=g)
+    k_off = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)]).to(torch.int32)
+    q_off = torch.arange(257, dtype=torch.int32)
+    q, k, v = (torch.randn(n, h, 32, generator=g).to(torch.bfloat16) for n, h in ((256, 64), (int(lens.sum()), 1), (int(lens.sum()), 1)))
+    o = sequence.attend(q.to(DEV), k.to(DEV), v.to(DEV), q_off.to(DEV), k_off.to(DEV), 1, 131072, causal=True)
+    want = O.attention(q[:8], k, v, q_off[:9], k_off[:9], causal=True, half_eps=eps_of(torch.bfloat16))
+    near("o", o[:8], want["o"], want["tol_o"])
+    want = O.attention(q[248:], k, v, q_off[:9], k_off[248:], causal=True, half_eps=eps_of(torch.bfloat16))
+    near("o", o[248:], want["o"], want["tol_o"])

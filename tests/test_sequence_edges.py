@@ -3,7 +3,7 @@ import ctypes
 
 import pytest
 
-from test_sequence import FAKE, attn, lib  # noqa: F401
+from test_sequence import FAKE, attn, lib, norm  # noqa: F401
 
 
 @pytest.mark.parametrize("softcap", [1e-45, 1e-39])
@@ -11,3 +11,27 @@ def test_a_cap_whose_reciprocal_is_no_number_is_refused(lib, softcap):
     a = attn(softcap=softcap)
     assert lib.bigc_seq_attn_fwd(None, ctypes.byref(a), FAKE, 1 << 40) == -1
     assert lib.bigc_seq_attn_bwd(None, ctypes.byref(a), FAKE, 1 << 40) == -1
+
+
+def test_many_streams_over_long_caches_are_taken(lib):
+    """what counts is the launch's blocks, not sequences x longest cache x heads: one token for each of 256 streams, the longest cache of 131072 rows, 64 heads"""
+    a = attn(n_seq=256, n_head=64, n_kv_head=1, max_q=1, max_k=131072, n_q=256, n_k=1 << 20, ldq=4096, ldo=4096)
+    need = lib.bigc_seq_attn_workspace_bytes(ctypes.byref(a), 0)
+    assert need > 0
+    assert lib.bigc_seq_attn_fwd(None, ctypes.byref(a), FAKE, need - 1) == -4
+
+
+def test_more_blocks_than_a_launch_holds_are_refused(lib):
+    for kw in (dict(n_seq=1 << 22, n_head=4, n_kv_head=4), dict(n_seq=1 << 14, max_q=1 << 17, n_q=1 << 20), dict(n_seq=1 << 23, n_head=2, n_kv_head=2)):
+        a = attn(**kw)
+        assert lib.bigc_seq_attn_fwd(None, ctypes.byref(a), FAKE, 1 << 60) == -1, kw
+        assert lib.bigc_seq_attn_bwd(None, ctypes.byref(a), FAKE, 1 << 60) == -1, kw
+        assert lib.bigc_seq_attn_workspace_bytes(ctypes.byref(a), 0) == lib.bigc_seq_attn_workspace_bytes(ctypes.byref(a), 1) == 0, kw
+
+
+def test_the_stride_of_a_single_row_is_not_read(lib):
+    a = attn(n_q=1, n_k=1, max_q=1, max_k=1, **{n: -4 for n in ("ldq", "ldk", "ldv", "ldo")})
+    a.ldq = 1 << 40
+    assert lib.bigc_seq_attn_bwd(None, ctypes.byref(a), FAKE, 0) == -4
+    n = norm(n_rows=1, ldq=-4, lddqo=-8)
+    assert lib.bigc_head_norm_rope_bwd(None, ctypes.byref(n), FAKE, 0) == -4

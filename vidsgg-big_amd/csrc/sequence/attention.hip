@@ -11,7 +11,7 @@ int check_rows(const bigc_seq_attn& a, const char* who, const char* what, const 
     BIGC_CHECK_ARG(p, "%s: %s is NULL", who, what);
     BIGC_CHECK_ARG((uintptr_t)p % 16 == 0 && (rows == 1 || ld % e == 0) && (heads == 1 || hs % e == 0),
                    "%s: %s: address, row stride %ld and head stride %ld have to be multiples of 16 bytes", who, what, (long)ld, (long)hs);
-    BIGC_CHECK_ARG(ld >= 0 && ld <= (1 << 22) && (heads == 1 || hs >= 0), "%s: %s: row stride %ld (0 to 2^22 elements), head stride %ld", who, what, (long)ld, (long)hs);
+    BIGC_CHECK_ARG((rows == 1 || (ld >= 0 && ld <= (1 << 22))) && (heads == 1 || hs >= 0), "%s: %s: row stride %ld (0 to 2^22 elements), head stride %ld", who, what, (long)ld, (long)hs);
     return BIGC_OK;
 }
 
@@ -33,17 +33,32 @@ int check_args(const bigc_seq_attn* ap, const char* who) {
     BIGC_CHECK_ARG(!a.q_doc == !a.k_doc || a.n_q == 0 || a.n_k == 0, "%s: q_doc and k_doc come together", who);
     BIGC_CHECK_ARG(!a.rel_table == !a.rel_map, "%s: rel_table and rel_map come together", who);
     if (a.rel_table) BIGC_CHECK_ARG(a.n_bucket > 0 && a.bias_radius >= 0 && a.bias_radius <= 2047, "%s: %d buckets, radius %d (at most 2047)", who, a.n_bucket, a.bias_radius);
-    BIGC_CHECK_ARG((double)a.n_seq * a.max_q * a.n_head < 2147483648.0 && (double)a.n_seq * a.max_k * a.n_head < 2147483648.0,
-                   "%s: %d sequences of up to %d queries and %d keys with %d heads are too many for one launch", who, a.n_seq, a.max_q, a.max_k, a.n_head);
+    BIGC_CHECK_ARG((double)a.n_seq * a.n_head < 2147483648.0 && (double)a.n_seq * a.max_q < 4294967296.0 && (double)a.n_seq * a.max_k < 4294967296.0,
+                   "%s: %d sequences of up to %d queries and %d keys with %d heads are too many", who, a.n_seq, a.max_q, a.max_k, a.n_head);
     return BIGC_OK;
 }
+
+// the launches of a call: a grid holds less than 2^32 threads, 2^24 blocks of 256
+int check_blocks(const bigc_seq_attn& a, const char* who, long blocks) {
+    const long ranges = a.q_doc ? ((long)a.n_seq * cdiv(a.max_q > a.max_k ? a.max_q : a.max_k, 64) + 3) / 4 : 0;
+    BIGC_CHECK_ARG(blocks < (1 << 24) && ranges < (1 << 24), "%s: %d sequences of up to %d queries and %d keys with %d heads need %ld blocks, too many for one launch", who,
+                   a.n_seq, a.max_q, a.max_k, a.n_head, blocks > ranges ? blocks : ranges);
+    return BIGC_OK;
+}
+int check_blocks(const bigc_seq_attn& a, const char* who, const FwdShape& sh) { return check_blocks(a, who, sh.blocks); }
+int check_blocks(const bigc_seq_attn& a, const char* who, const BwdShape& sh) {
+    const long q = (long)sh.q_pairs * sh.q_tiles, k = (long)sh.k_pairs * sh.k_tiles, table = a.d_rel_table ? 4l * a.n_head : 0, most = q > k ? q : k;    // (the table's blocks are of 1024)
+    return check_blocks(a, who, most > table ? most : table);
+}
+template <typename Shape>
+size_t workspace_of(const bigc_seq_attn& a, const Shape& sh) { return check_blocks(a, "seq_attn_workspace_bytes", sh) == BIGC_OK ? sh.total : 0; }
 
 #define SEQ_DISPATCH(dtype, F) do { if ((dtype) == BIGC_F32) { F(float) } else if ((dtype) == BIGC_F16) { F(f16_t) } else { F(bf16_t) } } while (0)
 }  // namespace
 
 extern "C" size_t bigc_seq_attn_workspace_bytes(const bigc_seq_attn* a, int backward) {
     if (check_args(a, "seq_attn_workspace_bytes") != BIGC_OK) return 0;
-    return backward ? bwd_shape(*a).total : fwd_shape(*a).total;
+    return backward ? workspace_of(*a, bwd_shape(*a)) : workspace_of(*a, fwd_shape(*a));
 }
 
 extern "C" int bigc_seq_attn_fwd(void* stream, const bigc_seq_attn* ap, void* workspace, size_t workspace_bytes) {
@@ -57,6 +72,7 @@ extern "C" int bigc_seq_attn_fwd(void* stream, const bigc_seq_attn* ap, void* wo
     if ((rc = check_rows(a, who, "o", a.o, a.ldo, a.hso, a.n_q, a.n_head)) != BIGC_OK) return rc;
     BIGC_CHECK_ARG((uintptr_t)a.stats % 8 == 0 && (uintptr_t)a.o32 % 16 == 0, "%s: stats has to lie at a multiple of 8 bytes, o32 of 16", who);
     const FwdShape sh = fwd_shape(a);
+    if ((rc = check_blocks(a, who, sh)) != BIGC_OK) return rc;
     if (workspace_bytes < sh.total || (sh.total && (!workspace || (uintptr_t)workspace % 16)))
         return bigc_fail(BIGC_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, sh.total);
     if (a.n_q == 0) return BIGC_OK;
@@ -100,6 +116,7 @@ extern "C" int bigc_seq_attn_bwd(void* stream, const bigc_seq_attn* ap, void* wo
     BIGC_CHECK_ARG(!a.d_rel_table || a.rel_table, "%s: d_rel_table without rel_table", who);
     BIGC_CHECK_ARG(!a.d_rel_table || a.dtype != BIGC_F32 || a.head_dim <= 64 || a.bias_radius <= 1023, "%s: d_rel_table of f32 heads over 64 columns: radius %d (at most 1023)", who, a.bias_radius);
     const BwdShape sh = bwd_shape(a);
+    if ((rc = check_blocks(a, who, sh)) != BIGC_OK) return rc;
     if (workspace_bytes < sh.total || (sh.total && (!workspace || (uintptr_t)workspace % 16)))
         return bigc_fail(BIGC_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, sh.total);
     hipStream_t hs = (hipStream_t)stream;

@@ -252,7 +252,7 @@ int check_rows(const bigc_head_norm& a, const char* who, const char* what, const
     BIGC_CHECK_ARG(p, "%s: %s is NULL", who, what);
     BIGC_CHECK_ARG((uintptr_t)p % 16 == 0 && (a.n_rows == 1 || ld % e == 0) && (heads == 1 || hs % e == 0),
                    "%s: %s: address, row stride %ld and head stride %ld have to be multiples of 16 bytes", who, what, (long)ld, (long)hs);
-    BIGC_CHECK_ARG(ld >= 0 && (heads == 1 || hs >= 0), "%s: %s: negative stride", who, what);
+    BIGC_CHECK_ARG((a.n_rows == 1 || ld >= 0) && (heads == 1 || hs >= 0), "%s: %s: negative stride", who, what);
     return BIGC_OK;
 }
 
