@@ -714,7 +714,7 @@ typedef struct {
     int32_t dtype;                     /* BIGC_F32 / BIGC_F16 / BIGC_BF16: q, k, v, o, d_o, dq, dk, dv */
     int32_t n_seq, n_head, n_kv_head;  /* n_head a multiple of n_kv_head */
     int32_t head_dim;                  /* a multiple of 8, at most 128 */
-    int32_t max_q, max_k;              /* the longest sequence's rows */
+    int32_t max_q, max_k;              /* the longest sequence's rows; together at most 2^31 - 2^20 */
     int32_t causal, window_left, window_right; /* windows: -1 = none */
     int32_t zero_rest;                 /* not 0: rows outside every sequence of o (forward), dq, dk, dv (backward) become 0 instead of staying as they were */
     int32_t bias_radius, n_bucket;     /* rel_map has 2 * bias_radius + 1 entries (bias_radius <= 2047), rel_table n_bucket rows of n_head */

@@ -35,3 +35,18 @@ def test_the_stride_of_a_single_row_is_not_read(lib):
     assert lib.bigc_seq_attn_bwd(None, ctypes.byref(a), FAKE, 0) == -4
     n = norm(n_rows=1, ldq=-4, lddqo=-8)
     assert lib.bigc_head_norm_rope_bwd(None, ctypes.byref(n), FAKE, 0) == -4
+
+
+@pytest.mark.parametrize("kw", [dict(max_k=2 ** 31 - 10), dict(max_q=2 ** 31 - 10, max_k=1), dict(max_q=2 ** 30, max_k=2 ** 30)], ids=str)
+def test_places_that_int32_cannot_count_are_refused(lib, kw):
+    a = attn(n_head=1, n_kv_head=1, **kw)
+    assert lib.bigc_seq_attn_fwd(None, ctypes.byref(a), FAKE, 1 << 60) == -1
+    assert lib.bigc_seq_attn_bwd(None, ctypes.byref(a), FAKE, 1 << 60) == -1
+    assert lib.bigc_seq_attn_workspace_bytes(ctypes.byref(a), 0) == 0
+
+
+def test_a_cache_of_almost_all_places_is_split(lib):
+    n = 2 ** 31 - 2 ** 20 - 8
+    a = attn(n_head=2, n_kv_head=2, max_q=1, n_q=1, max_k=n, n_k=n)
+    one = 2 * (64 + 2) * 4                                                 # a chunk's sums and statistics, two heads
+    assert lib.bigc_seq_attn_workspace_bytes(ctypes.byref(a), 0) > 100 * one

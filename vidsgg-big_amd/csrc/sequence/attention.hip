@@ -24,7 +24,8 @@ int check_args(const bigc_seq_attn* ap, const char* who) {
     BIGC_CHECK_ARG(a.head_dim > 0 && a.head_dim <= 128 && a.head_dim % 8 == 0, "%s: head_dim %d (a multiple of 8 up to 128)", who, a.head_dim);
     BIGC_CHECK_ARG(a.n_q >= 0 && a.n_k >= 0 && a.n_q < (1ll << 31) && a.n_k < (1ll << 31) && a.max_q >= 0 && a.max_k >= 0, "%s: %ld query and %ld key rows, longest %d and %d",
                    who, (long)a.n_q, (long)a.n_k, a.max_q, a.max_k);
-    BIGC_CHECK_ARG((long)a.max_q + a.max_k < (1l << 31), "%s: %d queries and %d keys are too far apart", who, a.max_q, a.max_k);
+    // (places, their distances and what a tile or a chunk adds to them are int32)
+    BIGC_CHECK_ARG((long)a.max_q + a.max_k <= (1l << 31) - (1 << 20), "%s: %d queries and %d keys are too far apart", who, a.max_q, a.max_k);
     BIGC_CHECK_ARG((double)a.n_q * a.n_head < 2147483648.0, "%s: %ld rows of %d heads are too many", who, (long)a.n_q, a.n_head);
     BIGC_CHECK_ARG(a.n_seq == 0 || (a.q_off && a.k_off), "%s: offsets are NULL", who);
     BIGC_CHECK_ARG(a.window_left >= -1 && a.window_right >= -1, "%s: window (%d, %d)", who, a.window_left, a.window_right);

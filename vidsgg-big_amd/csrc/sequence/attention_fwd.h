@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void attn_join(bigc_seq_attn a, FwdShape sh, c
     const SeqSpan sp = seq_span(a, s);
     if (i >= sp.nq) return;
     const long row = sp.q0 + i, rh = row * a.n_head + h, part = part_row(a, 0, s, i, h), stride = part_row(a, 1, 0, 0, 0);
-    const int n = max(1, (sp.nk + sh.chunk - 1) / sh.chunk);
+    const int n = max(1, (int)(((long)sp.nk + sh.chunk - 1) / sh.chunk));
     // 64 chunks at a time: their statistics by a lane each, then their sums with four loads on their way
     float top = -INFINITY, sum = 0.f, o[2] = {0.f, 0.f};
     for (int k0 = 0; k0 < n; k0 += 64) {
@@ -441,7 +441,7 @@ FwdShape fwd_shape(const bigc_seq_attn& a) {
         chunk = chunk < 512 ? 512 : chunk;
         if (chunk < sh.chunk) sh.chunk = (int)round_up(chunk, 4 * keys);
     }
-    sh.splits = (int)((a.max_k + sh.chunk - 1) / sh.chunk);
+    sh.splits = (int)(((long)a.max_k + sh.chunk - 1) / sh.chunk);
     if (sh.splits < 1) sh.splits = 1;
     sh.blocks = row_blocks * sh.splits;
     const int tile = tile_bytes(a, keys, a.dtype == BIGC_F32 && !sh.few), row = tile_dim(a.head_dim) * seq_size(a.dtype);
