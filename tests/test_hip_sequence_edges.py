@@ -185,3 +185,26 @@ def test_many_short_caches_beside_room_for_long_ones():
     near("o", o[:8], want["o"], want["tol_o"])
     want = O.attention(q[248:], k, v, q_off[:9], k_off[248:], causal=True, half_eps=eps_of(torch.bfloat16))
     near("o", o[248:], want["o"], want["tol_o"])
+
+
+@pytest.mark.parametrize("value", [-1e8, -3e7, 1e8])
+def test_a_large_common_bias_takes_no_second_pass(value):
+    """f16: a bias of 1e8 on every distance costs no more than none (the pass over non-finite results took 6.2 times as long here)"""
+    n, h = 2048, 8
+    g = torch.Generator().manual_seed(5)
+    q, k, v = (torch.randn(n, h, 64, generator=g).to(torch.float16).to(DEV) for _ in range(3))
+    off = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    bucket = sequence.rel_bucket_map(4, 8).to(DEV)
+
+    def fastest(bias):
+        table, times = torch.full((4, h), bias, device=DEV), []
+        for _ in range(12):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            sequence.attend(q, k, v, off, off, n, n, rel_table=table, rel_map=bucket)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    assert fastest(value) < 3 * fastest(0.0)

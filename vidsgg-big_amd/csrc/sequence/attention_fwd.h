@@ -125,6 +125,9 @@ template <typename T> constexpr float SLACK = 8.f;
 template <> constexpr float SLACK<f16_t> = 4.f;
 template <typename T> constexpr float LIFT = 0.f;
 template <> constexpr float LIFT<f16_t> = 11.f;
+// What p is taken beside: the maximum less the lift.  From 2^20 on, where f32 holds no more than eighths of a score and soon rounds the lift itself (by 5 at 2^27: p would pass f16's
+// end), without one.  The running maximum, the chunks' and waves' statistics and `stats` are all this.
+template <typename T> __device__ __forceinline__ float lifted(float top) { return LIFT<T> != 0.f && fabsf(top) < 0x1p20f ? top - LIFT<T> : top; }
 
 // PARTS: of p (see o32).
 template <typename T, int HD, bool FEW, int PARTS>
@@ -256,7 +259,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
                     if (s.a < 0.f) { for (int e = 1; e < 16; ++e) top = fminf(top, x[e]); }
                     else { for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]); }
                     top = fmaf(top, s.a, s.c);
-                    top = fmaxf(top, __shfl_xor(top, 32));
+                    top = lifted<T>(fmaxf(top, __shfl_xor(top, 32)));
                     const bool move = top > m + SLACK<T>;
                     if (__ballot(move)) {
                         const float c = move ? __builtin_amdgcn_exp2f(m - top) : 1.f;
@@ -264,7 +267,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
                         l *= c;
                         for (int d = 0; d < DT; ++d) for (int e = 0; e < 16; ++e) acc[d][e] *= c;
                     }
-                    const float base = s.c - ((m == -INFINITY ? 0.f : m) - LIFT<T>);
+                    const float base = s.c - (m == -INFINITY ? 0.f : m);
                     for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], s.a, base));
                     float sum = x[0];
                     for (int e = 1; e < 16; ++e) sum += x[e];
@@ -324,7 +327,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
                 o *= sum == 0.f ? 0.f : 1.f / sum;
                 ((T*)a.o)[qrow * a.ldo + h * a.hso + c] = (T)o;
                 if (a.o32) a.o32[rh * a.head_dim + c] = o;
-                if (a.stats && c == 0) *(float2*)(a.stats + 2 * rh) = make_float2(top - LIFT<T>, sum);
+                if (a.stats && c == 0) *(float2*)(a.stats + 2 * rh) = make_float2(top, sum);
             }
         }
         return;
@@ -354,7 +357,7 @@ __global__ __launch_bounds__((64 * FwdTile<T, HD, FEW>::WAVES), (FEW || (sizeof(
             *(Four*)((T*)a.o + row * a.ldo + head * a.hso + c) = *(const Four*)z;
             if (a.o32) *(float4*)(a.o32 + rh * a.head_dim + c) = make_float4(y[0], y[1], y[2], y[3]);
         }
-    if (a.stats && hi == 0) *(float2*)(a.stats + 2 * rh) = make_float2(m - LIFT<T>, l);
+    if (a.stats && hi == 0) *(float2*)(a.stats + 2 * rh) = make_float2(m, l);
 }
 
 // Joins the chunks of every (row, head): a wave each
@@ -402,7 +405,7 @@ __global__ __launch_bounds__(256) void attn_join(bigc_seq_attn a, FwdShape sh, c
         ((T*)a.o)[row * a.ldo + h * a.hso + c] = (T)(o[t] * inv);
         if (a.o32) a.o32[rh * a.head_dim + c] = o[t] * inv;
     }
-    if (a.stats && lane == 0) *(float2*)(a.stats + 2 * rh) = make_float2(top - LIFT<T>, sum);
+    if (a.stats && lane == 0) *(float2*)(a.stats + 2 * rh) = make_float2(top, sum);
 }
 
 template <typename T>
