@@ -50,3 +50,31 @@ def test_a_cache_of_almost_all_places_is_split(lib):
     a = attn(n_head=2, n_kv_head=2, max_q=1, n_q=1, max_k=n, n_k=n)
     one = 2 * (64 + 2) * 4                                                 # a chunk's sums and statistics, two heads
     assert lib.bigc_seq_attn_workspace_bytes(ctypes.byref(a), 0) > 100 * one
+
+
+STRIDES = [(0, 64), (8, 64), (256, 0), (256, 32), (64, 64), (128, 64), (64, 128), (192, 128), (320, 192), (256, 64), (64, 512), (72, 1024), (512, 64), (384, 64), (520, 136)]
+
+
+@pytest.mark.parametrize("strides", STRIDES, ids=str)
+def test_outputs_that_overlap_themselves_are_refused(lib, strides):
+    """rows or heads that share a place would be written by two blocks at once; any other layout is taken (such a call ends at its workspace of no bytes)"""
+    ld, hs = strides
+
+    def due(heads):                                                        # 8 rows of 64 columns
+        return -1 if any(abs(r * ld - h * hs) < 64 for h in range(heads) for r in range(-7, 8) if (r, h) != (0, 0)) else -4
+
+    split = dict(n_q=8, max_q=1, n_seq=1, n_k=1 << 20, max_k=1 << 20)      # (a forward that needs a workspace)
+    assert lib.bigc_seq_attn_fwd(None, ctypes.byref(attn(ldo=ld, hso=hs, **split)), FAKE, 0) == due(4)
+    for n, heads in (("q", 4), ("k", 2), ("v", 2)):
+        assert lib.bigc_seq_attn_bwd(None, ctypes.byref(attn(**{"ldd" + n: ld, "hsd" + n: hs})), FAKE, 0) == due(heads), n
+    for n, heads in (("q", 4), ("k", 2)):
+        a = norm(**{"d" + n: FAKE << 1, "ldd" + n: ld, "hsd" + n: hs})
+        assert lib.bigc_head_norm_rope_bwd(None, ctypes.byref(a), FAKE, 0) == due(heads), n
+        if due(heads) == -1:
+            a = norm(**{n + "_out": FAKE << 1, "ld" + n + "o": ld, "hs" + n + "o": hs})
+            assert lib.bigc_head_norm_rope_fwd(None, ctypes.byref(a)) == -1
+
+
+def test_in_place_with_other_strides_is_refused(lib):
+    assert lib.bigc_head_norm_rope_fwd(None, ctypes.byref(norm(ldqo=320))) == -1
+    assert lib.bigc_head_norm_rope_bwd(None, ctypes.byref(norm(lddk=512)), FAKE, 0) == -1

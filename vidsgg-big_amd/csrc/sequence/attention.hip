@@ -15,6 +15,13 @@ int check_rows(const bigc_seq_attn& a, const char* who, const char* what, const 
     return BIGC_OK;
 }
 
+int check_out(const bigc_seq_attn& a, const char* who, const char* what, const void* p, int64_t ld, int64_t hs, int64_t rows, int heads) {
+    const int rc = check_rows(a, who, what, p, ld, hs, rows, heads);
+    if (rc != BIGC_OK || rows == 0) return rc;
+    BIGC_CHECK_ARG(!rows_overlap(ld, hs, a.head_dim, rows, heads), "%s: %s: rows or heads overlap (row stride %ld, head stride %ld)", who, what, (long)ld, (long)hs);
+    return BIGC_OK;
+}
+
 int check_args(const bigc_seq_attn* ap, const char* who) {
     BIGC_CHECK_ARG(ap, "%s: arguments are NULL", who);
     const bigc_seq_attn& a = *ap;
@@ -70,7 +77,7 @@ extern "C" int bigc_seq_attn_fwd(void* stream, const bigc_seq_attn* ap, void* wo
     if ((rc = check_rows(a, who, "q", a.q, a.ldq, a.hsq, a.n_q, a.n_head)) != BIGC_OK) return rc;
     if ((rc = check_rows(a, who, "k", a.k, a.ldk, a.hsk, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
     if ((rc = check_rows(a, who, "v", a.v, a.ldv, a.hsv, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
-    if ((rc = check_rows(a, who, "o", a.o, a.ldo, a.hso, a.n_q, a.n_head)) != BIGC_OK) return rc;
+    if ((rc = check_out(a, who, "o", a.o, a.ldo, a.hso, a.n_q, a.n_head)) != BIGC_OK) return rc;
     BIGC_CHECK_ARG((uintptr_t)a.stats % 8 == 0 && (uintptr_t)a.o32 % 16 == 0, "%s: stats has to lie at a multiple of 8 bytes, o32 of 16", who);
     const FwdShape sh = fwd_shape(a);
     if ((rc = check_blocks(a, who, sh)) != BIGC_OK) return rc;
@@ -110,9 +117,9 @@ extern "C" int bigc_seq_attn_bwd(void* stream, const bigc_seq_attn* ap, void* wo
     if ((rc = check_rows(a, who, "v", a.v, a.ldv, a.hsv, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
     if (!a.o32 && (rc = check_rows(a, who, "o", a.o, a.ldo, a.hso, a.n_q, a.n_head)) != BIGC_OK) return rc;
     if ((rc = check_rows(a, who, "d_o", a.d_o, a.lddo, a.hsdo, a.n_q, a.n_head)) != BIGC_OK) return rc;
-    if ((rc = check_rows(a, who, "dq", a.dq, a.lddq, a.hsdq, a.n_q, a.n_head)) != BIGC_OK) return rc;
-    if ((rc = check_rows(a, who, "dk", a.dk, a.lddk, a.hsdk, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
-    if ((rc = check_rows(a, who, "dv", a.dv, a.lddv, a.hsdv, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
+    if ((rc = check_out(a, who, "dq", a.dq, a.lddq, a.hsdq, a.n_q, a.n_head)) != BIGC_OK) return rc;
+    if ((rc = check_out(a, who, "dk", a.dk, a.lddk, a.hsdk, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
+    if ((rc = check_out(a, who, "dv", a.dv, a.lddv, a.hsdv, a.n_k, a.n_kv_head)) != BIGC_OK) return rc;
     BIGC_CHECK_ARG(a.n_q == 0 || (a.stats && (uintptr_t)a.stats % 8 == 0), "%s: stats is NULL or not a multiple of 8 bytes", who);
     BIGC_CHECK_ARG(!a.d_rel_table || a.rel_table, "%s: d_rel_table without rel_table", who);
     BIGC_CHECK_ARG(!a.d_rel_table || a.dtype != BIGC_F32 || a.head_dim <= 64 || a.bias_radius <= 1023, "%s: d_rel_table of f32 heads over 64 columns: radius %d (at most 1023)", who, a.bias_radius);

@@ -256,6 +256,15 @@ int check_rows(const bigc_head_norm& a, const char* who, const char* what, const
     return BIGC_OK;
 }
 
+// an output: no two of its rows and heads share a place, and one that is its input's place has its strides (a row's partner columns are read before it is written, other rows' not)
+int check_out(const bigc_head_norm& a, const char* who, const char* what, const void* p, int64_t ld, int64_t hs, int heads, const void* in, int64_t ldi, int64_t hsi) {
+    const int rc = check_rows(a, who, what, p, ld, hs, heads);
+    if (rc != BIGC_OK || a.n_rows == 0 || heads == 0) return rc;
+    BIGC_CHECK_ARG(!rows_overlap(ld, hs, a.head_dim, a.n_rows, heads), "%s: %s: rows or heads overlap (row stride %ld, head stride %ld)", who, what, (long)ld, (long)hs);
+    BIGC_CHECK_ARG(p != in || ((a.n_rows == 1 || ld == ldi) && (heads == 1 || hs == hsi)), "%s: %s: in place of its input with other strides", who, what);
+    return BIGC_OK;
+}
+
 int check_args(const bigc_head_norm* ap, const char* who) {
     BIGC_CHECK_ARG(ap, "%s: arguments are NULL", who);
     const bigc_head_norm& a = *ap;
@@ -288,8 +297,8 @@ extern "C" int bigc_head_norm_rope_fwd(void* stream, const bigc_head_norm* ap) {
     const bigc_head_norm a = *ap;
     if ((rc = check_rows(a, who, "q", a.q, a.ldq, a.hsq, a.n_q_head)) != BIGC_OK) return rc;
     if ((rc = check_rows(a, who, "k", a.k, a.ldk, a.hsk, a.n_k_head)) != BIGC_OK) return rc;
-    if ((rc = check_rows(a, who, "q_out", a.q_out, a.ldqo, a.hsqo, a.n_q_head)) != BIGC_OK) return rc;
-    if ((rc = check_rows(a, who, "k_out", a.k_out, a.ldko, a.hsko, a.n_k_head)) != BIGC_OK) return rc;
+    if ((rc = check_out(a, who, "q_out", a.q_out, a.ldqo, a.hsqo, a.n_q_head, a.q, a.ldq, a.hsq)) != BIGC_OK) return rc;
+    if ((rc = check_out(a, who, "k_out", a.k_out, a.ldko, a.hsko, a.n_k_head, a.k, a.ldk, a.hsk)) != BIGC_OK) return rc;
     if (a.n_rows == 0) return BIGC_OK;
     ProfScope prof(stream, FAM_LAYERNORM, 0, 0);
     // Four rows a block, all heads of each; while that would leave CUs without a block, one row and one round of heads a block instead (a call of a
@@ -319,8 +328,8 @@ extern "C" int bigc_head_norm_rope_bwd(void* stream, const bigc_head_norm* ap, v
     if ((rc = check_rows(a, who, "k", a.k, a.ldk, a.hsk, a.n_k_head)) != BIGC_OK) return rc;
     if ((rc = check_rows(a, who, "dq_out", a.dq_out, a.lddqo, a.hsdqo, a.n_q_head)) != BIGC_OK) return rc;
     if ((rc = check_rows(a, who, "dk_out", a.dk_out, a.lddko, a.hsdko, a.n_k_head)) != BIGC_OK) return rc;
-    if ((rc = check_rows(a, who, "dq", a.dq, a.lddq, a.hsdq, a.n_q_head)) != BIGC_OK) return rc;
-    if ((rc = check_rows(a, who, "dk", a.dk, a.lddk, a.hsdk, a.n_k_head)) != BIGC_OK) return rc;
+    if ((rc = check_out(a, who, "dq", a.dq, a.lddq, a.hsdq, a.n_q_head, a.dq_out, a.lddqo, a.hsdqo)) != BIGC_OK) return rc;
+    if ((rc = check_out(a, who, "dk", a.dk, a.lddk, a.hsdk, a.n_k_head, a.dk_out, a.lddko, a.hsdko)) != BIGC_OK) return rc;
     const size_t need = bigc_head_norm_rope_workspace_bytes(ap);
     if (workspace_bytes < need || !workspace || (uintptr_t)workspace % 16)
         return bigc_fail(BIGC_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);

@@ -13,6 +13,18 @@ template <> struct SeqType<bf16_t> { static constexpr int size = 2; };
 
 static inline int seq_size(int dtype) { return dtype == BIGC_F32 ? 4 : 2; }
 
+// whether two of `rows` x `heads` pieces of hd elements at r ld + h hs share a place, as outputs must not (strides not negative; one row's or one head's is not looked at)
+static inline bool rows_overlap(int64_t ld, int64_t hs, int hd, int64_t rows, int heads) {
+    if (rows > 1 && ld < hd) return true;
+    if (heads == 1) return false;
+    if (hs < hd) return true;
+    if (rows <= 1 || ld >= (heads - 1) * hs + hd || hs >= (rows - 1) * ld + hd) return false;       // heads inside rows, or rows inside heads
+    for (int64_t h = 1; h < heads; ++h)
+        for (int64_t r = h * hs / ld, end = r + 2; r < end && r < rows; ++r)
+            if (r * ld - h * hs < hd && h * hs - r * ld < hd) return true;
+    return false;
+}
+
 // the place of sequence s: rows cut to what the tensors hold and lengths to what the launch was sized for, so that no offset leads outside
 struct SeqSpan { int q0, nq, k0, nk; };
 __device__ __forceinline__ SeqSpan seq_span(const bigc_seq_attn& a, int s) {
