@@ -2,7 +2,9 @@
 import ctypes
 
 import pytest
+import torch
 
+from bigc_hip import sequence
 from test_sequence import FAKE, attn, lib, norm  # noqa: F401
 
 
@@ -78,3 +80,20 @@ def test_outputs_that_overlap_themselves_are_refused(lib, strides):
 def test_in_place_with_other_strides_is_refused(lib):
     assert lib.bigc_head_norm_rope_fwd(None, ctypes.byref(norm(ldqo=320))) == -1
     assert lib.bigc_head_norm_rope_bwd(None, ctypes.byref(norm(lddk=512)), FAKE, 0) == -1
+
+
+def test_tensor_functions_refuse_what_the_structure_cannot_hold():
+    """(the message names the argument: on a machine without a GPU every call ends in an AssertionError, for its device)"""
+    off = torch.tensor([0, 4], dtype=torch.int32)
+    q = torch.zeros(4, 2, 64)
+    base = dict(q=q, k=q, v=q, q_off=off, k_off=off, max_q=4, max_k=4)
+    for name, kw in (("max_q", dict(max_q=(1 << 32) + 4)), ("max_k", dict(max_k=1 << 31)), ("max_k", dict(max_k=4.0)), ("max_q", dict(max_q=None)), ("window", dict(window=((1 << 32) - 1, -1))),
+                     ("window", dict(window=(2, 1 << 33))), ("window", dict(window=3)), ("window", dict(window=(1, 2, 3))), ("q_off", dict(q_off=None)), ("k_off", dict(k_off=[0, 4])),
+                     ("q_off", dict(q_off=torch.tensor(4, dtype=torch.int32))), ("q_off", dict(q_off=off[:0])), ("softcap", dict(softcap="no")), ("scale", dict(scale=[1.0, 2.0])),
+                     ("rel_table", dict(rel_table=[[0.0]], rel_map=off)), ("rel_map", dict(rel_table=torch.zeros(3, 2), rel_map=off[0])), ("a GPU", {})):
+        with pytest.raises(AssertionError, match=name):
+            sequence.attend(**dict(base, **kw))
+    w, pos, inv = torch.ones(64), torch.zeros(4, dtype=torch.int32), torch.ones(32, dtype=torch.float64)
+    for name, kw in (("inv_freq", dict(inv_freq=inv[0])), ("inv_freq", dict(inv_freq=[1.0])), ("eps", dict(eps=None)), ("out", dict(out=q)), ("out", dict(out=(q,))), ("a GPU", {})):
+        with pytest.raises(AssertionError, match=name):
+            sequence.head_norm_rope(**dict(dict(q=q, k=q, wq=w, wk=w, pos=pos, inv_freq=inv), **kw))

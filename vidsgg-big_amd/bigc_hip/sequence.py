@@ -9,6 +9,7 @@ calls them from its ``backward``, as the training steps of this package do with 
 """
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -62,6 +63,24 @@ def _heads(name, t):
     return t.shape
 
 
+def _whole(name, x):
+    """x as an int32 of the C structure (ctypes would take any whole number modulo 2^32)"""
+    try:
+        n = operator.index(x)
+    except TypeError:
+        n = None
+    assert n is not None and -1 << 31 <= n < 1 << 31, "%s: %r is no int32" % (name, x)
+    return n
+
+
+def _number(name, x):
+    """x as a float of the C structure"""
+    try:
+        return float(x)
+    except (TypeError, ValueError):
+        raise AssertionError("%s: %r is no number" % (name, x))
+
+
 def _on(device):
     """A guard that makes the tensors' device the current one (a launch goes to the current device), or None where it is"""
     assert device.type == "cuda", "the operators run on a GPU (tensors are on %s)" % device
@@ -99,6 +118,12 @@ def attend(q, k, v, q_off, k_off, max_q, max_k, scale=None, softcap=0.0, slopes=
     -> o (n_q, n_head, head_dim), or (o, SavedAttention) with ``save``; rows outside every sequence are not written (0 unless ``out`` is given)."""
     shape = _heads("q", q)
     dtype, dev, hd = q.dtype, q.device, shape[2]
+    max_q, max_k, scale, softcap = _whole("max_q", max_q), _whole("max_k", max_k), _number("scale", max(1, hd) ** -0.5 if scale is None else scale), _number("softcap", softcap)
+    assert isinstance(window, (tuple, list)) and len(window) == 2, "window: (left, right)"
+    left, right = _whole("window", window[0]), _whole("window", window[1])
+    assert isinstance(q_off, torch.Tensor) and isinstance(k_off, torch.Tensor) and q_off.dim() == 1 and q_off.shape[0] > 0, "q_off, k_off: int32 tensors (n_seq + 1)"
+    for name, t, dim in (("rel_table", rel_table, 2), ("rel_map", rel_map, 1)):
+        assert t is None or (isinstance(t, torch.Tensor) and t.dim() == dim), "%s: a tensor of %d dimensions" % (name, dim)
     guard = _on(dev)
     if guard is not None:
         with guard:
@@ -110,7 +135,7 @@ def attend(q, k, v, q_off, k_off, max_q, max_k, scale=None, softcap=0.0, slopes=
     n_bucket = radius = 0
     if rel_table is not None or rel_map is not None:
         assert rel_table is not None and rel_map is not None, "rel_table and rel_map come together"
-        assert rel_table.dim() == 2 and rel_map.dim() == 1 and rel_map.shape[0] % 2 == 1, "rel_table (n_bucket, n_head), rel_map (2 R + 1)"
+        assert rel_map.shape[0] % 2 == 1, "rel_table (n_bucket, n_head), rel_map (2 R + 1)"
         n_bucket, radius = rel_table.shape[0], rel_map.shape[0] // 2
     i32, f32 = torch.int32, torch.float32
     o = q.new_empty(shape) if out is None else out
@@ -120,8 +145,8 @@ def attend(q, k, v, q_off, k_off, max_q, max_k, scale=None, softcap=0.0, slopes=
         if dtype is not f32:                                             # see o32 in bigc_hip.h
             o32 = q.new_empty(shape, dtype=f32)
     a = bigc_seq_attn(                                                   # the fields in the structure's order
-        _DTYPES[dtype], n_seq, n_head, kshape[1], hd, max_q, max_k, 1 if causal else 0, window[0], window[1], 1 if out is None else 0, radius, n_bucket,
-        hd ** -0.5 if scale is None else scale, softcap, n_q, kshape[0],
+        _DTYPES[dtype], n_seq, n_head, kshape[1], hd, max_q, max_k, 1 if causal else 0, left, right, 1 if out is None else 0, radius, n_bucket,
+        scale, softcap, n_q, kshape[0],
         _vector("q_off", q_off, i32, (n_seq + 1,), dev), _vector("k_off", k_off, i32, (n_seq + 1,), dev), _vector("slopes", slopes, f32, (n_head,), dev),
         _vector("rel_table", rel_table, f32, (n_bucket, n_head), dev), _vector("rel_map", rel_map, i32, (2 * radius + 1,), dev),
         _vector("prefix_len", prefix_len, i32, (n_seq,), dev), _vector("q_doc", q_doc, i32, (n_q,), dev), _vector("k_doc", k_doc, i32, (kshape[0],), dev),
@@ -165,11 +190,12 @@ def attend_bwd(saved, d_o):
 def _norm_args(q, k, wq, wk, pos, inv_freq, eps, interleaved):
     shape, kshape = _heads("q", q), _heads("k", k)
     dtype, dev, n, hd = q.dtype, q.device, shape[0], shape[2]
+    assert inv_freq is None or (isinstance(inv_freq, torch.Tensor) and inv_freq.dim() == 1), "inv_freq: a float64 tensor (n_freq)"
     n_freq = 0 if inv_freq is None else inv_freq.shape[0]
     assert inv_freq is None or pos is not None, "inv_freq without pos"
     f32 = torch.float32
     return bigc_head_norm(                                               # the fields in the structure's order
-        _DTYPES[dtype], shape[1], kshape[1], hd, n_freq, 1 if interleaved else 0, eps, n, _vector("pos", pos, torch.int32, (n,), dev),
+        _DTYPES[dtype], shape[1], kshape[1], hd, n_freq, 1 if interleaved else 0, _number("eps", eps), n, _vector("pos", pos, torch.int32, (n,), dev),
         _vector("inv_freq", inv_freq, torch.float64, (n_freq,), dev), _vector("wq", wq, f32, (hd,), dev), _vector("wk", wk, f32, (hd,), dev),
         *_rows("q", q, dtype, dev, shape), *_rows("k", k, dtype, dev, (n, kshape[1], hd)))
 
@@ -180,6 +206,7 @@ def head_norm_rope(q, k, wq, wk, pos, inv_freq, eps=1e-6, interleaved=False, out
     slices of one projection's output (16-byte strides); ``out``: a pair of tensors, which may be (q, k) themselves.  -> (q', k')"""
     a = _norm_args(q, k, wq, wk, pos, inv_freq, eps, interleaved)
     dtype, dev = q.dtype, q.device
+    assert out is None or (isinstance(out, (tuple, list)) and len(out) == 2), "out: a pair of tensors"
     guard = _on(dev)
     if guard is not None:
         with guard:
