@@ -755,7 +755,7 @@ typedef struct {
     int32_t dtype, n_q_head, n_k_head, head_dim; /* head_dim a multiple of 8, at most 256; either head count may be 0 */
     int32_t n_freq, interleaved;       /* 2 * n_freq <= head_dim */
     float eps;
-    int64_t n_rows;                    /* below 2^31 */
+    int64_t n_rows;                    /* below 2^31; forward: rows / 4 x the threads of a row, 64 to 512, below 2^32 */
     const int32_t* pos;                /* (n_rows) */
     const double* inv_freq;            /* (n_freq) */
     const float* wq; const float* wk;  /* (head_dim) */

@@ -97,3 +97,11 @@ def test_tensor_functions_refuse_what_the_structure_cannot_hold():
     for name, kw in (("inv_freq", dict(inv_freq=inv[0])), ("inv_freq", dict(inv_freq=[1.0])), ("eps", dict(eps=None)), ("out", dict(out=q)), ("out", dict(out=(q,))), ("a GPU", {})):
         with pytest.raises(AssertionError, match=name):
             sequence.head_norm_rope(**dict(dict(q=q, k=q, wq=w, wk=w, pos=pos, inv_freq=inv), **kw))
+
+
+def test_head_norm_goes_by_what_a_launch_holds(lib):
+    a = norm(n_rows=1 << 28, n_q_head=4, n_k_head=4, head_dim=8, n_freq=4, ldq=32)
+    assert lib.bigc_head_norm_rope_bwd(None, ctypes.byref(a), FAKE, 0) == -4       # (its blocks take rows in turn)
+    a = norm(n_rows=(1 << 31) - 1, n_q_head=1, n_k_head=0, head_dim=8, n_freq=4)
+    assert lib.bigc_head_norm_rope_fwd(None, ctypes.byref(a)) == -1
+    assert b"launch" in lib.bigc_last_error()

@@ -275,8 +275,6 @@ int check_args(const bigc_head_norm* ap, const char* who) {
     BIGC_CHECK_ARG(a.n_freq >= 0 && 2 * (long)a.n_freq <= a.head_dim, "%s: %d frequencies on head_dim %d", who, a.n_freq, a.head_dim);
     BIGC_CHECK_ARG(a.n_freq == 0 || a.n_rows == 0 || (a.pos && a.inv_freq), "%s: pos or inv_freq is NULL", who);
     BIGC_CHECK_ARG(isfinite(a.eps) && a.eps >= 0.f, "%s: eps %g", who, a.eps);
-    BIGC_CHECK_ARG((double)a.n_rows * (a.n_q_head + a.n_k_head) < 2147483648.0, "%s: %ld rows of %d heads are too many for one launch", who, (long)a.n_rows,
-                   a.n_q_head + a.n_k_head);
     return BIGC_OK;
 }
 
@@ -300,13 +298,14 @@ extern "C" int bigc_head_norm_rope_fwd(void* stream, const bigc_head_norm* ap) {
     if ((rc = check_out(a, who, "q_out", a.q_out, a.ldqo, a.hsqo, a.n_q_head, a.q, a.ldq, a.hsq)) != BIGC_OK) return rc;
     if ((rc = check_out(a, who, "k_out", a.k_out, a.ldko, a.hsko, a.n_k_head, a.k, a.ldk, a.hsk)) != BIGC_OK) return rc;
     if (a.n_rows == 0) return BIGC_OK;
-    ProfScope prof(stream, FAM_LAYERNORM, 0, 0);
     // Four rows a block, all heads of each; while that would leave CUs without a block, one row and one round of heads a block instead (a call of a
     // few rows is latency: its threads then make one trip through memory).
     const Shape sh = shape_of(a);
     const bool few = a.n_rows < ROWS_PER_BLOCK * 1024;
     const int rows = few ? 1 : ROWS_PER_BLOCK;
     const dim3 grid((unsigned)((a.n_rows + rows - 1) / rows), few ? sh.rounds : 1);
+    BIGC_CHECK_ARG((double)grid.x * grid.y * 64 * sh.waves < 4294967296.0, "%s: %ld rows of %d heads are too many for one launch", who, (long)a.n_rows, a.n_q_head + a.n_k_head);
+    ProfScope prof(stream, FAM_LAYERNORM, 0, 0);
 #define F(T) TURNS(sh.turn, T, head_norm_fwd, grid, 64 * sh.waves, sizeof(float) * rows * 4 * a.head_dim, (hipStream_t)stream, a, sh.lph, rows)
     SEQ_DISPATCH(a.dtype, F);
 #undef F
