@@ -49,7 +49,7 @@ struct FwdShape {
     int few, tiles, pairs;                                      // row tiles of the longest sequence; (sequence, key head, pack) triples
     int chunk, splits;                                          // keys a block takes; chunks of the longest sequence
     long blocks;
-    size_t lds, ranges, part_o, part_ml, total;                 // LDS; workspace: offsets of the parts and its size
+    size_t lds, part_o, part_ml, total;                         // LDS; workspace (document ranges first): offsets of the parts and its size
 };
 
 template <typename T, int HD, bool FEW> struct FwdTile {

@@ -6,11 +6,6 @@
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
-template <typename T> struct SeqType;
-template <> struct SeqType<float> { static constexpr int size = 4; };
-template <> struct SeqType<f16_t> { static constexpr int size = 2; };
-template <> struct SeqType<bf16_t> { static constexpr int size = 2; };
-
 static inline int seq_size(int dtype) { return dtype == BIGC_F32 ? 4 : 2; }
 
 // whether two of `rows` x `heads` pieces of hd elements at r ld + h hs share a place, as outputs must not (strides not negative; one row's or one head's is not looked at)
@@ -31,10 +26,4 @@ __device__ __forceinline__ SeqSpan seq_span(const bigc_seq_attn& a, int s) {
     const int q0 = min(max(a.q_off[s], 0), (int)a.n_q), q1 = min(max(a.q_off[s + 1], q0), (int)a.n_q);
     const int k0 = min(max(a.k_off[s], 0), (int)a.n_k), k1 = min(max(a.k_off[s + 1], k0), (int)a.n_k);
     return {q0, min(q1 - q0, a.max_q), k0, min(k1 - k0, a.max_k)};
-}
-
-// whether the key at place j is seen from position pos (documents apart)
-__device__ __forceinline__ bool seq_near(const bigc_seq_attn& a, int prefix, int pos, int j) {
-    const int d = j - pos;
-    return j < prefix || ((!a.causal || d <= 0) && (a.window_left < 0 || -d <= a.window_left) && (a.window_right < 0 || d <= a.window_right));
 }
