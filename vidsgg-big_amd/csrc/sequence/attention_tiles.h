@@ -397,6 +397,7 @@ __device__ __forceinline__ void cap_values(f32x16& x, f32x16* slopes, const Scor
         }
         if (KEEP) (*slopes)[e] = 1.f - v * v;
         x[e] = v;
+        if (sizeof(T) < 4) __builtin_amdgcn_sched_barrier(0);    // one value after the other: side by side they would take registers that the other calls' loop is short of
     }
 }
 template <typename T> __device__ __forceinline__ float slope_unit(const ScoreRule& r) { return sizeof(T) < 4 && r.cap && r.coarse ? 4.f : 1.f; }
