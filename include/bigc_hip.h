@@ -708,8 +708,9 @@ BIGC_API int bigc_linear_hr8out_f32(void* stream, const float* A, int lda, const
  *     o = softmax over the seen keys of the scores, times v
  * A query that sees no key (or only scores of -inf) has o = 0 and gives no gradient; what a hidden place holds (NaN, Inf) is never part of a
  * result (rows whose result is NaN or Inf are done twice, the second time value by value: such a call takes many times as long).  A bias of -inf hides its distances, the lowest finite values (below -2.3e38, which count as one) do not.  slopes, rel_table + rel_map, prefix_len, q_doc + k_doc may be NULL.  Rows outside every sequence
- * stay as they were.  Offsets are cut to [0, n_q] and [0, n_k], map entries to the table, and lengths to max_q and max_k, which size the launch: a
- * sequence is then its first rows, and those behind the cut are rows outside every sequence. */
+ * stay as they were.  Offsets ascend; they are cut to [0, n_q] and [0, n_k], map entries to the table, and lengths to max_q and max_k, which size the launch: a
+ * sequence is then its first rows, and those behind the cut are rows outside every sequence.
+ * f32's range holds what is added up: the number of keys times the largest |v| below 2^120.  Half types under a cap of up to 64 have their scores to 2^-23 of the cap. */
 typedef struct {
     int32_t dtype;                     /* BIGC_F32 / BIGC_F16 / BIGC_BF16: q, k, v, o, d_o, dq, dk, dv */
     int32_t n_seq, n_head, n_kv_head;  /* n_head a multiple of n_kv_head */
@@ -750,7 +751,7 @@ BIGC_API int bigc_seq_attn_bwd(void* stream, const bigc_seq_attn* a, void* works
 
 /* RMS norm of every query and key head and the rotation of its first 2 * n_freq columns by the row's position, in one launch:
  *     y = x / sqrt(mean(x^2) + eps) * w;   (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = pos[row] * inv_freq[f]
- * with t taken in 64 bits (any int32 position), pairs (f, f + n_freq), or (2 f, 2 f + 1) when interleaved.  w NULL: 1. n_freq 0: no rotation. */
+ * with the squares added up in f32 (|x| below 2^60), t taken in 64 bits (any int32 position), pairs (f, f + n_freq), or (2 f, 2 f + 1) when interleaved.  w NULL: 1. n_freq 0: no rotation. */
 typedef struct {
     int32_t dtype, n_q_head, n_k_head, head_dim; /* head_dim a multiple of 8, at most 256; either head count may be 0 */
     int32_t n_freq, interleaved;       /* 2 * n_freq <= head_dim */

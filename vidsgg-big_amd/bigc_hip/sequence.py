@@ -110,9 +110,9 @@ def attend(q, k, v, q_off, k_off, max_q, max_k, scale=None, softcap=0.0, slopes=
            prefix_len=None, q_doc=None, k_doc=None, out=None, save=False):
     """Attention of the rows of ``q`` (n_q, n_head, head_dim) over those of ``k``, ``v`` (n_k, n_kv_head, head_dim), f32, f16 or bf16, any row and
     head strides of whole 16 bytes.  Sequence s owns rows q_off[s]:q_off[s + 1] and k_off[s]:k_off[s + 1] (int32, on the device) of at most
-    max_q and max_k rows; its queries are its last rows (one query per sequence: a decoding step).  scale: 1 / sqrt(head_dim) unless given;
+    max_q and max_k rows (a longer one is cut to its first); its queries are its last rows (one query per sequence: a decoding step).  scale: 1 / sqrt(head_dim) unless given;
     softcap: scores become softcap * tanh(score / softcap); slopes (n_head) f32: minus slope times distance; rel_table (n_bucket, n_head) f32 and
-    rel_map (2 R + 1) int32: the bias of a distance clipped to [-R, R] (``rel_bucket_map``); causal; window (left, right): keys at most so far
+    rel_map (2 R + 1) int32: the bias of a distance clipped to [-R, R] (``rel_bucket_map``; R at most 2047, 1023 for the gradient of f32 heads over 64 columns); causal; window (left, right): keys at most so far
     behind / ahead, -1 for no limit; prefix_len (n_seq) int32: the first keys of a sequence are seen by all its rows; q_doc, k_doc (n_q), (n_k)
     int32: rows see keys of their own document, a negative number is padding.  A row that sees nothing gives 0.
     -> o (n_q, n_head, head_dim), or (o, SavedAttention) with ``save``; rows outside every sequence are not written (0 unless ``out`` is given)."""

@@ -5,9 +5,12 @@
 //           bias table's gradient); first the rows' delta = dO . o, which it also leaves, with m and 1 / l, for the other kernel.
 //   dk, dv: lanes are keys.  S = Q k, dP = dO v, dv += dO^T P, dk += Q^T dS, over all query heads of the key head.
 //
+// Half types round P and dS once each, to their own type, for the products that they enter (errors of the gradients 1.4 times those of an f32 computation rounded at its end, of the
+// kind that the outputs' own rounding makes; a second part of each would be two more products of seven); scores, statistics, delta and every sum, the bias table's among them, are f32.
+//
 // Bound by vector instructions and the matrix instructions between them (16 heads of 64 with a learned bias over sequences of up to 2048 rows, bf16: dq and
-// the diagonals' sums 228 us, dk and dv 212, the forward before them 197); with few sequences by the longest one's own chain of tiles (two packed rows of
-// 4096 of documents, f16: 93 and 150 us, the forward 78).
+// the diagonals' sums 207 us, dk and dv 187, the forward before them 182); with few sequences by the longest one's own chain of tiles (two packed rows of
+// 4096 of documents, f16: 93 and 146 us, the forward 76).
 #pragma once
 #include "attention_fwd.h"
 

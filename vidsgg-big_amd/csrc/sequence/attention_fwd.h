@@ -114,9 +114,9 @@ __device__ __forceinline__ long part_row(const bigc_seq_attn& a, int split, int 
 //
 // A row's maximum is only moved when a score passes it by more than SLACK, so that the accumulators are rarely rescaled (and p is what the backward's will be,
 // bit for bit: next to another maximum the exponent is rounded differently); p then lies in (0, 2^SLACK].
-// Bound: few rows over long caches by memory (48 tokens over caches of 1 to 16384, 8 key heads of 128, bf16: 371 us for 1.75 GB, 4.7 TB/s of the 5.1 that a
+// Bound: few rows over long caches by memory (48 tokens over caches of 1 to 16384, 8 key heads of 128, bf16: 378 us for 1.75 GB, 4.6 TB/s of the 5.1 that a
 // copy reaches); many rows by vector instructions beside the matrix instructions (some ten a score of 2 head_dim x 2 flops; of a SIMD's cycles about half
-// issue those and a quarter of them feed the matrix unit, the two adding up rather than overlapping): 8192 causal rows, 32 + 8 heads of 128, bf16: 785 us, 700
+// issue those and a quarter of them feed the matrix unit, the two adding up rather than overlapping): 8192 causal rows, 32 + 8 heads of 128, bf16: 790 us, 696
 // TFLOP/s.
 //
 // p is rounded to the tensors' type for its product with v (the one rounding inside; sums and statistics are f32 before it).  f16 ends at 2^-14, so that its p is
